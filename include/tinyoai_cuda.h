@@ -379,6 +379,171 @@ int tcu_batch_close(tcu_batch* batch);
 int tcu_shortlist_static(int32_t device, const float* logits, int32_t vocab, int32_t k, void* stream, int32_t* ids,
                          float* values, double* logsumexp, int32_t* n_out);
 
+/* ---------------------------------------------------------------------------
+ * Operators over a paged KV cache the caller holds in device memory.
+ *
+ * One serving step of a host that keeps its own cache: tcu_plan_step builds
+ * the step's block tables, positions and slots; tcu_paged_append normalises
+ * and rotates the step's queries and keys and appends keys and values;
+ * tcu_paged_means keeps the mean key of every completed page;
+ * tcu_paged_attend and tcu_paged_attend_sparse attend. No counterpart in the
+ * reference, whose native sessions own their KV (mlx_native.go:24-45): these
+ * serve hosts that already hold their activations and cache on the GPU.
+ *
+ * Conventions of the section
+ *  - Pointers named in a structure or argument list are device memory of
+ *    `device` unless stated; counts, strides and the structures themselves
+ *    are host values read during the call.
+ *  - Work is queued on `stream` (a cudaStream_t of that device; NULL: the
+ *    legacy default stream) and the call returns. Nothing is allocated,
+ *    synchronised or kept, so the calls can be captured into CUDA graphs and
+ *    may run concurrently as long as their outputs and workspaces differ. The
+ *    caller's current device is left as it was.
+ *  - Types: TCU_F32, TCU_F16 or TCU_BF16. Query rows and outputs have the
+ *    cache's type, or are float32 over a TCU_F16 cache. Sums, norms and
+ *    softmax statistics are float32 or wider; a result is rounded once, when
+ *    it is stored (softmax weights over 16-bit caches also to 16 bits, each
+ *    by at most half a step of the cache's type).
+ *  - Strides count values, and the last dimension (a head's values) is
+ *    contiguous. Rows, strides and bases of q, out, k and v are multiples of
+ *    16 bytes. Head sizes: multiples of 8 up to TCU_PAGED_MAX_HEAD_DIM.
+ *  - Page ids outside [0, num_pages) stand for no page: their positions are
+ *    not attended and nothing is written there. Values in a page behind a
+ *    request's length are never read into a result.
+ * ------------------------------------------------------------------------ */
+#define TCU_PAGED_MAX_HEAD_DIM 256
+#define TCU_PAGED_MAX_GROUP 64           /* query heads per KV head */
+#define TCU_PAGED_MAX_PAGE_TOKENS 65536
+#define TCU_PAGED_MAX_SELECTED 65536     /* first + last + top of a sparse call */
+
+/* Value d of position r of page p, KV head g of k (and of v) is at
+ * p * page_stride + g * head_stride + r * token_stride + d. */
+typedef struct {
+  void* k;
+  void* v;
+  int32_t dtype;
+  int32_t num_pages, page_tokens, kv_heads, head_dim;
+  int64_t page_stride, head_stride, token_stride;
+} tcu_paged_kv;
+
+/* Block tables, positions and slots of a step, from request lengths. Request
+ * i holds held[i] positions and adds fresh[i] >= 0 tokens. Its table (row i,
+ * table_width entries, rows table_stride apart) maps its pages; entries for
+ * the positions it holds are read, ceil((held + fresh) / P) - ceil(held / P)
+ * entries after them are written with pages from the front of free_pages, in
+ * request order; other entries are left as they were. Outputs:
+ *   starts[0 .. n]      first token of each request; starts[n] = tokens planned
+ *   lengths[0 .. n)     held + fresh
+ *   positions[t], slots[t] (t < capacity)  position of token t and its place
+ *                       page * P + offset in the pool; -1 and -1 behind the
+ *                       last token, and slot -1 where the table has no page
+ *   counts[0 .. 3)      requests planned, tokens planned, pages taken
+ * Requests are planned in order up to the first that does not fit (capacity
+ * tokens, n_free pages, table_width) or has a negative count; that one and
+ * the later ones keep lengths[i] = held[i] and get no tokens. A page that a
+ * request appends to (its last, partly filled one) must be its own.
+ * page_tokens P: 1 .. TCU_PAGED_MAX_PAGE_TOKENS. */
+int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, const int32_t* fresh, int32_t page_tokens, int32_t* tables,
+                  int32_t table_width, int64_t table_stride, const int32_t* free_pages, int32_t n_free, int32_t capacity, int32_t* starts,
+                  int32_t* lengths, int32_t* positions, int64_t* slots, int32_t* counts);
+
+/* Rotary table: max_positions x pairs float32 pairs (cos, sin), 8-byte
+ * aligned. Pair i is features (i, i + pairs) of a head, or (2i, 2i + 1) when
+ * adjacent != 0; features from 2 * pairs on pass unchanged. */
+typedef struct {
+  const float* table;
+  int32_t max_positions, pairs, adjacent;
+} tcu_rotary;
+
+/* Norm of each query and key head over its head_dim features, before the
+ * rotation: x / sqrt(mean x^2 + eps) * w (TCU_NORM_RMS) or (x - mean) /
+ * sqrt(variance + eps) * w (TCU_NORM_LAYER). Weights are float32, one row of
+ * head_dim for all heads (head_stride 0) or a row per head (head_stride
+ * head_dim): q_weight for the query heads, k_weight for the KV heads. */
+#define TCU_NORM_NONE 0
+#define TCU_NORM_RMS 1
+#define TCU_NORM_LAYER 2
+typedef struct {
+  int32_t kind;
+  double eps;
+  const float* q_weight;
+  const float* k_weight;
+  int64_t head_stride;
+} tcu_head_norm;
+
+/* Normalises (norm, may be NULL) and rotates (rotary, may be NULL) the query
+ * and key heads of `rows` rows [heads | kv_heads | kv_heads] x head_dim of
+ * type dtype, rows qkv_stride apart; writes queries to q_out (rows q_stride
+ * apart, same type) and keys and values to the cache at slots[row] =
+ * page * page_tokens + offset. Rows whose slot is outside the pool (-1: a
+ * padding row) or whose position is outside the rotary table are skipped:
+ * nothing of theirs is written. Two rows must not name one slot. q_out must
+ * not overlap qkv. */
+int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t dtype, int32_t rows, int32_t heads, const void* qkv,
+                     int64_t qkv_stride, const int32_t* positions, const int64_t* slots, const tcu_rotary* rotary, const tcu_head_norm* norm,
+                     void* q_out, int64_t q_stride);
+
+/* For every slot that is the last of its page: means[page][g] = mean over the
+ * page's positions of its keys, for each KV head g. means: [num_pages]
+ * [kv_heads][head_dim], contiguous, the cache's type. The pages' other
+ * positions must hold their keys already (an append of the same slots before
+ * it on the stream); slots of other positions and outside the pool do
+ * nothing. kv->v is not read. */
+int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t rows, const int64_t* slots, void* means);
+
+/* The queries of a ragged step. Rows starts[i] .. starts[i + 1] of q (rows
+ * rows in all, heads x head_dim values each) are request i's last tokens:
+ * row starts[i] + j is at position lengths[i] - (starts[i + 1] - starts[i])
+ * + j and attends to the request's positions up to its own. Row i of tables
+ * maps its pages. max_fresh is at least the largest starts[i + 1] - starts[i]
+ * (later rows of a longer request are left as they were), and rows behind
+ * starts[requests] are left as they were. A row at a negative position
+ * attends to nothing and is zero. heads is a multiple of kv_heads; query head
+ * h reads KV head h / (heads / kv_heads). The weight of position t is
+ * softmax(scale * q . k_t). */
+typedef struct {
+  int32_t dtype;
+  int32_t requests, rows, heads, max_fresh;
+  int32_t table_width;
+  const void* q;
+  int64_t q_token_stride, q_head_stride;
+  void* out;
+  int64_t out_token_stride, out_head_stride;
+  const int32_t* starts;
+  const int32_t* lengths;
+  const int32_t* tables;
+  int64_t table_stride;
+  float scale;
+} tcu_paged_queries;
+
+/* Attention of the step. The first prefix_pages pages of every request are
+ * prefix[0 .. prefix_pages) (a long prompt they share): they are read from
+ * there, once for all requests, and the tables' entries for them are not
+ * read. prefix_pages 0: nothing is shared. max_length bounds the requests'
+ * lengths (0: what the tables and the prefix map); positions from it on are
+ * not attended. workspace: at least the bytes that the _workspace call
+ * reports for the same arguments (it reads no device memory), 256-byte
+ * aligned, its content irrelevant before and after; calls that may run at
+ * the same time (two streams, two captured graphs) need one each. */
+int tcu_paged_attend_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* queries, int32_t prefix_pages, int32_t max_length,
+                               uint64_t* bytes);
+int tcu_paged_attend(int32_t device, void* stream, const tcu_paged_kv* kv, const tcu_paged_queries* queries, const int32_t* prefix,
+                     int32_t prefix_pages, int32_t max_length, void* workspace, uint64_t workspace_bytes);
+
+/* Attention of each query over the pages that a cheap score selects. A query
+ * at position p has npages = p / page_tokens + 1 pages. For each KV head it
+ * attends to the first `first` pages, the last `last` pages (at least 1, so
+ * that the page being filled is among them) and, of those between, the `top`
+ * with the largest max over the KV head's query heads h of q_h . means[page]
+ * (float64; ties to the lower page, NaN and missing pages last). means is
+ * tcu_paged_means' array, read for complete pages only. pages
+ * [rows][kv_heads][first + last + top] receives the logical pages attended
+ * to, ascending, -1 behind them. The workspace is as for tcu_paged_attend. */
+int tcu_paged_attend_sparse_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* queries, int32_t first, int32_t last, int32_t top,
+                                      uint64_t* bytes);
+int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv, const tcu_paged_queries* queries, const void* means,
+                            int32_t first, int32_t last, int32_t top, int32_t* pages, void* workspace, uint64_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,8 @@ EXPORTS = [
     "tcu_tp_unique_id", "tcu_stablelm_load_tp", "tcu_tp_plan", "tcu_tp_exchange_handle", "tcu_tp_exchange_open",
     "tcu_gguf_open", "tcu_gguf_config", "tcu_gguf_tensor_count", "tcu_gguf_tensor", "tcu_gguf_load_stablelm", "tcu_gguf_close",
     "tcu_session_save_cache", "tcu_session_load_cache",
+    "tcu_plan_step", "tcu_paged_append", "tcu_paged_means", "tcu_paged_attend_workspace", "tcu_paged_attend",
+    "tcu_paged_attend_sparse_workspace", "tcu_paged_attend_sparse",
 ]
 
 
@@ -52,6 +54,34 @@ class TpOptions(C.Structure):
 
 class LoadOptions(C.Structure):
     _fields_ = [("device", C.c_int32), ("kv_page_tokens", C.c_int32), ("kv_pool_bytes", C.c_int64)]
+
+
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class PagedKV(C.Structure):
+    """tcu_paged_kv: a paged cache in device memory the caller holds."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("num_pages", C.c_int32), ("page_tokens", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("token_stride", C.c_int64)]
+
+
+class Rotary(C.Structure):
+    """tcu_rotary: (cos, sin) per position and pair."""
+    _fields_ = [("table", C.c_void_p), ("max_positions", C.c_int32), ("pairs", C.c_int32), ("adjacent", C.c_int32)]
+
+
+class HeadNorm(C.Structure):
+    """tcu_head_norm: the norm of each query and key head."""
+    _fields_ = [("kind", C.c_int32), ("eps", C.c_double), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("head_stride", C.c_int64)]
+
+
+class PagedQueries(C.Structure):
+    """tcu_paged_queries: the queries of a ragged step."""
+    _fields_ = [("dtype", C.c_int32), ("requests", C.c_int32), ("rows", C.c_int32), ("heads", C.c_int32), ("max_fresh", C.c_int32),
+                ("table_width", C.c_int32), ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64), ("starts", C.c_void_p),
+                ("lengths", C.c_void_p), ("tables", C.c_void_p), ("table_stride", C.c_int64), ("scale", C.c_float)]
 
 
 _lib = None
@@ -119,6 +149,17 @@ def lib():
         "tcu_gguf_close": ([P], C.c_int),
         "tcu_session_save_cache": ([P, C.c_char_p, C.POINTER(C.c_uint8), i32p, C.c_int32], C.c_int),
         "tcu_session_load_cache": ([P, C.c_char_p, C.POINTER(C.c_uint8), i32p, C.c_int32, i32p], C.c_int),
+    }
+    i32, i64, u64p = C.c_int32, C.c_int64, C.POINTER(C.c_uint64)
+    kvp, qp = C.POINTER(PagedKV), C.POINTER(PagedQueries)
+    sig |= {
+        "tcu_plan_step": ([i32, P, i32, P, P, i32, P, i32, i64, P, i32, i32, P, P, P, P, P], C.c_int),
+        "tcu_paged_append": ([i32, P, kvp, i32, i32, i32, P, i64, P, P, C.POINTER(Rotary), C.POINTER(HeadNorm), P, i64], C.c_int),
+        "tcu_paged_means": ([i32, P, kvp, i32, P, P], C.c_int),
+        "tcu_paged_attend_workspace": ([kvp, qp, i32, i32, u64p], C.c_int),
+        "tcu_paged_attend": ([i32, P, kvp, qp, P, i32, i32, P, C.c_uint64], C.c_int),
+        "tcu_paged_attend_sparse_workspace": ([kvp, qp, i32, i32, i32, u64p], C.c_int),
+        "tcu_paged_attend_sparse": ([i32, P, kvp, qp, P, i32, i32, i32, P, P, C.c_uint64], C.c_int),
     }
     for name, (args, res) in sig.items():
         fn = getattr(L, name)

@@ -1,7 +1,9 @@
 """Builds libtinyoai_cuda.so in-tree with nvcc for sm_100a.
 
-The library is a single translation unit (csrc/runtime.cu) with the C ABI of
-include/tinyoai_cuda.h. nvcc cross-compiles without a GPU.
+Two sources carry the C ABI of include/tinyoai_cuda.h: csrc/runtime.cu (models
+and sessions) and csrc/paged.cu (operators over a caller's paged cache). They
+compile side by side; an object is rebuilt when a file it includes is newer.
+nvcc cross-compiles without a GPU.
 """
 import os
 import subprocess
@@ -11,13 +13,14 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 LIB = PKG / "libtinyoai_cuda.so"
-SOURCES = [PKG / "csrc" / "runtime.cu"]
-DEPS = sorted((PKG / "csrc").glob("*.cu*")) + [ROOT / "include" / "tinyoai_cuda.h"]
+OBJ_DIR = PKG / "_build"
+SOURCES = [PKG / "csrc" / "runtime.cu", PKG / "csrc" / "paged.cu"]
+DEPS = sorted((PKG / "csrc").glob("*.cu*")) + sorted((PKG / "csrc").glob("*.h")) + [ROOT / "include" / "tinyoai_cuda.h"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xcudafe", "--diag_suppress=177",
 ]
 
@@ -36,10 +39,35 @@ def stale():
     return any(p.stat().st_mtime > t for p in DEPS)
 
 
+def object_stale(obj, depfile):
+    """Whether obj is older than a file its last compilation read."""
+    if not obj.exists() or not depfile.exists():
+        return True
+    named = depfile.read_text().split(":", 1)[1].replace("\\\n", " ").split()
+    t = obj.stat().st_mtime
+    return any(not os.path.exists(p) or os.stat(p).st_mtime > t for p in named if not p.startswith("/usr/"))
+
+
 def build(force=False, verbose=False):
     if not force and not stale():
         return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", str(LIB) + ".tmp", *map(str, SOURCES)]
+    OBJ_DIR.mkdir(exist_ok=True)
+    objects, running = [], []
+    for src in SOURCES:
+        obj, dep = OBJ_DIR / (src.stem + ".o"), OBJ_DIR / (src.stem + ".d")
+        objects.append(str(obj))
+        if not force and not object_stale(obj, dep):
+            continue
+        cmd = [nvcc(), *NVCC_FLAGS, "-MMD", "-MF", str(dep), "-c", "-o", str(obj), str(src)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        running.append((cmd, obj, subprocess.Popen(cmd)))
+    failed = [(cmd, obj) for cmd, obj, p in running if p.wait() != 0]
+    for cmd, obj in failed:
+        obj.unlink(missing_ok=True)
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0][0])
+    cmd = [nvcc(), *NVCC_FLAGS, "-shared", "-o", str(LIB) + ".tmp", *objects]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

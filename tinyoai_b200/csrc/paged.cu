@@ -1,0 +1,558 @@
+// Host side of the paged-cache operators declared in include/tinyoai_cuda.h
+// (section "Operators over a paged KV cache the caller holds"): argument
+// checks, kernel selection, workspace layout and launches. Nothing here
+// allocates, synchronises or keeps anything between calls.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+
+#include "../../include/tinyoai_cuda.h"
+#include "paged.cuh"
+#include "status.h"
+
+using namespace tcu;
+
+namespace {
+
+int fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return set_error(code, buf);
+}
+
+#define TRY(x)                   \
+  do {                           \
+    int r_ = (x);                \
+    if (r_ != TCU_OK) return r_; \
+  } while (0)
+#define CK(x)                                                                                                        \
+  do {                                                                                                               \
+    cudaError_t e_ = (x);                                                                                            \
+    if (e_ != cudaSuccess) return fail(TCU_ECUDA, "%s (%s:%d): %s", #x, __FILE__, __LINE__, cudaGetErrorString(e_)); \
+  } while (0)
+
+// Makes `device` current for one call and puts the caller's device back.
+struct OnDevice {
+  int before = -1, rc = TCU_OK;
+  explicit OnDevice(int device) {
+    rc = require_device(device);
+    if (rc != TCU_OK) return;
+    int cur = -1;
+    if (cudaGetDevice(&cur) == cudaSuccess && cur != device) {
+      before = cur;
+      if (cudaSetDevice(device) != cudaSuccess) rc = fail(TCU_ECUDA, "device %d cannot be made current", device);
+    }
+  }
+  ~OnDevice() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+// A pointer the kernels read or write: memory of this device, aligned.
+int check_ptr(const char* name, const void* p, int device, size_t align) {
+  if (!p) return fail(TCU_EINVAL, "%s is null", name);
+  if (reinterpret_cast<uintptr_t>(p) % align) return fail(TCU_EINVAL, "%s is not %zu-byte aligned", name, align);
+  cudaPointerAttributes pa;
+  cudaError_t e = cudaPointerGetAttributes(&pa, p);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TCU_EINVAL, "%s: %s", name, cudaGetErrorString(e));
+  }
+  if ((pa.type != cudaMemoryTypeDevice && pa.type != cudaMemoryTypeManaged) || pa.device != device)
+    return fail(TCU_EINVAL, "%s must be device memory on device %d", name, device);
+  return TCU_OK;
+}
+
+int elem_bytes(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
+bool dtype_ok(int dtype) { return dtype == TCU_F32 || dtype == TCU_F16 || dtype == TCU_BF16; }
+
+// Rows are the cache's type, or float32 over a binary16 cache (what the
+// models of this library compute and store).
+int check_pair(int rows, int cache) {
+  if (!dtype_ok(rows) || !dtype_ok(cache)) return fail(TCU_EUNSUP, "paged operators take float32, binary16 and bfloat16 values");
+  if (rows != cache && !(rows == TCU_F32 && cache == TCU_F16))
+    return fail(TCU_EUNSUP, "rows have the cache's type, or are float32 over a binary16 cache");
+  return TCU_OK;
+}
+
+int check_kv(const tcu_paged_kv* kv) {
+  if (!kv) return fail(TCU_EINVAL, "null cache");
+  if (!dtype_ok(kv->dtype)) return fail(TCU_EUNSUP, "paged operators take float32, binary16 and bfloat16 values");
+  if (kv->num_pages < 1 || kv->page_tokens < 1 || kv->kv_heads < 1) return fail(TCU_EINVAL, "the cache has no pages, positions or heads");
+  if (kv->page_tokens > TCU_PAGED_MAX_PAGE_TOKENS) return fail(TCU_EINVAL, "%d positions a page, at most %d", kv->page_tokens, TCU_PAGED_MAX_PAGE_TOKENS);
+  if (kv->kv_heads > 65535) return fail(TCU_EINVAL, "%d KV heads, at most 65535", kv->kv_heads);
+  if (kv->head_dim < 8 || kv->head_dim > TCU_PAGED_MAX_HEAD_DIM || kv->head_dim % 8)
+    return fail(TCU_EUNSUP, "head size %d is not a multiple of 8 in 8..%d", kv->head_dim, TCU_PAGED_MAX_HEAD_DIM);
+  const int64_t per16 = 16 / elem_bytes(kv->dtype);
+  if (kv->page_stride < 0 || kv->head_stride < 0 || kv->token_stride < 0) return fail(TCU_EINVAL, "negative cache stride");
+  if (kv->page_stride % per16 || kv->head_stride % per16 || kv->token_stride % per16)
+    return fail(TCU_EINVAL, "cache strides must be multiples of 16 bytes");
+  return TCU_OK;
+}
+
+PagedView view_of(const tcu_paged_kv* kv) {
+  PagedView v;
+  v.k = kv->k;
+  v.v = kv->v;
+  v.num_pages = kv->num_pages;
+  v.P = kv->page_tokens;
+  v.kvh = kv->kv_heads;
+  v.hd = kv->head_dim;
+  v.sp = kv->page_stride;
+  v.sh = kv->head_stride;
+  v.st = kv->token_stride;
+  v.divP = FastDiv::of((uint32_t)kv->page_tokens);
+  return v;
+}
+
+int launched(const char* name) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(TCU_ECUDA, "%s: %s", name, cudaGetErrorString(e));
+  return TCU_OK;
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// ---------------------------------------------------------------------------
+// Append
+
+template <typename TQ, typename TK>
+void launch_append(const AppendArgs& a, cudaStream_t s) {
+  const int chunks = (a.hd + 3) / 4;
+  const int64_t items = (int64_t)a.T * (a.H + 2 * a.KVH);
+  auto go = [&](auto kern, int lph) { kern<<<(unsigned)ceil_div(items, APPEND_THREADS / lph), APPEND_THREADS, 0, s>>>(a); };
+  if (chunks <= 8)
+    go(k_append<TQ, TK, 8, 1>, 8);
+  else if (chunks <= 16)
+    go(k_append<TQ, TK, 16, 1>, 16);
+  else if (chunks <= 32)
+    go(k_append<TQ, TK, 32, 1>, 32);
+  else
+    go(k_append<TQ, TK, 32, 2>, 32);
+}
+
+// ---------------------------------------------------------------------------
+// Attention
+
+struct AttendPlan {
+  int prefix_chunk = 0, prefix_slots = 0, own_chunk = 0, own_slots = 0, slots = 0;
+  size_t part_o = 0, part_ml = 0, keys = 0, pages = 0, bytes = 0;  // offsets of the workspace regions
+};
+
+// Positions per part: enough CTAs for four on each SM, but parts of at least
+// 128 positions, whose own cost (its queries, its partial) a shorter one
+// would not earn back.
+int chunk_of(int64_t positions, int64_t ctas_per_part, int sms) {
+  const int64_t want = std::max<int64_t>(1, 4LL * sms / std::max<int64_t>(1, ctas_per_part));
+  int64_t c = std::max<int64_t>(128, ceil_div(ceil_div(positions, want), 64) * 64);
+  c = std::max<int64_t>(c, ceil_div(ceil_div(positions, 256), 64) * 64);  // at most 256 parts
+  return (int)std::min<int64_t>(c, 1 << 30);
+}
+
+constexpr int SM_COUNT = 148;  // B200
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+int rows_per_cta(int hd) { return hd <= 128 ? 4 : 2; }
+
+AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, int max_length, int budget) {
+  AttendPlan p;
+  const int G = q->heads / kv->kv_heads, R = rows_per_cta(kv->head_dim), P = kv->page_tokens;
+  const int64_t T = q->rows;
+  if (budget > 0) {
+    p.own_chunk = chunk_of((int64_t)budget * P, T * kv->kv_heads * ceil_div(G, R), SM_COUNT);
+    p.own_slots = (int)ceil_div((int64_t)budget * P, p.own_chunk);
+  } else {
+    const int64_t shared = (int64_t)prefix_pages * P;
+    if (shared > 0) {
+      p.prefix_chunk = chunk_of(shared, ceil_div(T * G, R) * kv->kv_heads, SM_COUNT);
+      p.prefix_slots = (int)ceil_div(shared, p.prefix_chunk);
+    }
+    const int64_t own = std::max<int64_t>(0, (int64_t)max_length - shared);
+    p.own_chunk = chunk_of(own, (int64_t)q->requests * kv->kv_heads * ceil_div((int64_t)q->max_fresh * G, R), SM_COUNT);
+    p.own_slots = (int)ceil_div(own, p.own_chunk);
+  }
+  p.slots = std::max(1, p.prefix_slots + p.own_slots);
+  size_t off = 0;
+  const size_t rows = (size_t)T * q->heads;
+  p.part_o = off;
+  off += align256(rows * p.slots * kv->head_dim * sizeof(float));
+  p.part_ml = off;
+  off += align256(rows * p.slots * sizeof(float2));
+  if (budget > 0) {
+    p.keys = off;
+    off += align256((size_t)T * kv->kv_heads * q->table_width * sizeof(unsigned long long));
+  }
+  p.bytes = off;
+  return p;
+}
+
+template <typename TQ, typename TK, int NCH, int R, int SRC>
+int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
+  int64_t x;
+  int tiles;
+  if (SRC == SRC_PREFIX) {
+    tiles = (int)ceil_div((int64_t)a.T * a.G, R);
+    x = tiles;
+  } else if (SRC == SRC_OWN) {
+    tiles = (int)ceil_div((int64_t)a.max_fresh * a.G, R);
+    x = (int64_t)a.n * tiles;
+  } else {
+    tiles = (int)ceil_div(a.G, R);
+    x = (int64_t)a.n * a.max_fresh * tiles;
+  }
+  const size_t smem = sizeof(float) * CC_GROUPS * (NCH * 32 + 2);
+  k_attend_cc<TQ, TK, NCH, R, SRC><<<dim3((unsigned)x, a.KVH, parts), CC_WARPS * 32, smem, s>>>(a, tiles);
+  return launched("k_attend_cc");
+}
+
+template <typename TQ, typename TK, int SRC>
+int launch_cc(const AttendArgs& a, int parts, cudaStream_t s) {
+  if (parts == 0) return TCU_OK;
+  const int nch = (a.hd + 31) / 32;
+  if (nch <= 2) return launch_cc_r<TQ, TK, 2, 4, SRC>(a, parts, s);
+  if (nch <= 3) return launch_cc_r<TQ, TK, 3, 4, SRC>(a, parts, s);
+  if (nch <= 4) return launch_cc_r<TQ, TK, 4, 4, SRC>(a, parts, s);
+  return launch_cc_r<TQ, TK, 8, 2, SRC>(a, parts, s);
+}
+
+template <typename TQ, typename TK>
+int launch_attend(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
+  TRY((launch_cc<TQ, TK, SRC_PREFIX>(a, p.prefix_slots, s)));
+  TRY((launch_cc<TQ, TK, SRC_OWN>(a, p.own_slots, s)));
+  k_attend_join<TQ, 0><<<dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s>>>(a);
+  return launched("k_attend_join");
+}
+
+template <typename TQ, typename TK>
+int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p, cudaStream_t s) {
+  const unsigned queries = (unsigned)((int64_t)a.n * a.max_fresh);
+  if (c.top > 0 && c.width > 0) {
+    const size_t smem = sizeof(double) * a.G * a.hd;
+    if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_page_scores<TQ, TK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    k_page_scores<TQ, TK><<<dim3(queries, a.KVH, (unsigned)ceil_div(c.width, 64)), 128, smem, s>>>(a, c);
+    TRY(launched("k_page_scores"));
+  }
+  k_page_choose<<<dim3(queries, a.KVH), CHOOSE_THREADS, 0, s>>>(a, c);
+  TRY(launched("k_page_choose"));
+  TRY((launch_cc<TQ, TK, SRC_LIST>(a, p.own_slots, s)));
+  k_attend_join<TQ, 1><<<dim3(queries, (a.H + 3) / 4), 128, 0, s>>>(a);
+  return launched("k_attend_join");
+}
+
+int check_queries(const tcu_paged_kv* kv, const tcu_paged_queries* q) {
+  if (!q) return fail(TCU_EINVAL, "null queries");
+  TRY(check_pair(q->dtype, kv->dtype));
+  if (q->requests < 0 || q->rows < 0 || q->table_width < 0) return fail(TCU_EINVAL, "negative count");
+  if (q->heads < 1 || q->heads % kv->kv_heads) return fail(TCU_EINVAL, "%d query heads over %d KV heads", q->heads, kv->kv_heads);
+  if (q->heads / kv->kv_heads > TCU_PAGED_MAX_GROUP) return fail(TCU_EUNSUP, "%d query heads a KV head, at most %d", q->heads / kv->kv_heads, TCU_PAGED_MAX_GROUP);
+  if (q->max_fresh < 1) return fail(TCU_EINVAL, "max_fresh %d", q->max_fresh);
+  if (q->table_stride < q->table_width) return fail(TCU_EINVAL, "table stride %lld below the width %d", (long long)q->table_stride, q->table_width);
+  if ((int64_t)q->table_width * kv->page_tokens > 0x7fffffffll) return fail(TCU_EINVAL, "tables of %d pages pass 2^31 positions", q->table_width);
+  const int G = q->heads / kv->kv_heads;
+  if ((int64_t)q->requests * q->max_fresh * G > 0x7fffffffll || (int64_t)q->rows * q->heads > 0x7fffffffll)
+    return fail(TCU_EINVAL, "too many rows for one call");
+  const int64_t per16 = 16 / elem_bytes(q->dtype);
+  if (q->q_token_stride % per16 || q->q_head_stride % per16 || q->out_token_stride % per16 || q->out_head_stride % per16)
+    return fail(TCU_EINVAL, "query and output strides must be multiples of 16 bytes");
+  if (q->q_token_stride < 0 || q->q_head_stride < 0 || q->out_token_stride < 0 || q->out_head_stride < 0) return fail(TCU_EINVAL, "negative query stride");
+  if (!(q->scale == q->scale)) return fail(TCU_EINVAL, "scale is not a number");
+  return TCU_OK;
+}
+
+int check_query_ptrs(const tcu_paged_kv* kv, const tcu_paged_queries* q, int device) {
+  TRY(check_ptr("k", kv->k, device, 16));
+  TRY(check_ptr("v", kv->v, device, 16));
+  TRY(check_ptr("q", q->q, device, 16));
+  TRY(check_ptr("out", q->out, device, 16));
+  TRY(check_ptr("starts", q->starts, device, 4));
+  TRY(check_ptr("lengths", q->lengths, device, 4));
+  if (q->table_width > 0) TRY(check_ptr("tables", q->tables, device, 4));
+  return TCU_OK;
+}
+
+AttendArgs attend_args(const tcu_paged_kv* kv, const tcu_paged_queries* q, const AttendPlan& p, void* workspace) {
+  AttendArgs a{};
+  a.n = q->requests;
+  a.T = q->rows;
+  a.H = q->heads;
+  a.KVH = kv->kv_heads;
+  a.G = q->heads / kv->kv_heads;
+  a.hd = kv->head_dim;
+  a.max_fresh = q->max_fresh;
+  a.q = q->q;
+  a.q_ts = q->q_token_stride;
+  a.q_hs = q->q_head_stride;
+  a.out = q->out;
+  a.o_ts = q->out_token_stride;
+  a.o_hs = q->out_head_stride;
+  a.starts = q->starts;
+  a.lengths = q->lengths;
+  a.tables = q->tables;
+  a.table_stride = q->table_stride;
+  a.width = q->table_width;
+  a.scale = (float)((double)q->scale * 1.4426950408889634);
+  a.kv = view_of(kv);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(w + p.part_o);
+  a.part_ml = reinterpret_cast<float2*>(w + p.part_ml);
+  a.slots = p.slots;
+  a.prefix_slots = p.prefix_slots;
+  a.prefix_chunk = p.prefix_chunk;
+  a.own_chunk = p.own_chunk;
+  return a;
+}
+
+int check_workspace(const AttendPlan& p, void* workspace, uint64_t bytes, int device) {
+  if (bytes < p.bytes) return fail(TCU_EINVAL, "workspace of %llu bytes, %llu needed", (unsigned long long)bytes, (unsigned long long)p.bytes);
+  return check_ptr("workspace", workspace, device, 256);
+}
+
+int check_prefix(const tcu_paged_kv* kv, int32_t prefix_pages, int32_t max_length) {
+  if (prefix_pages < 0 || (int64_t)prefix_pages * kv->page_tokens > 0x7fffffffll) return fail(TCU_EINVAL, "prefix of %d pages", prefix_pages);
+  if (max_length < 0) return fail(TCU_EINVAL, "max_length %d", max_length);
+  return TCU_OK;
+}
+
+// Positions a request can hold: what its table (or the prefix) maps.
+int length_bound(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, int max_length) {
+  const int64_t mapped = (int64_t)std::max(prefix_pages, q->table_width) * kv->page_tokens;
+  return (int)std::min<int64_t>(max_length > 0 ? std::min<int64_t>(max_length, mapped) : mapped, 0x7fffffff);
+}
+
+int check_sparse(const tcu_paged_queries* q, int32_t first, int32_t last, int32_t top) {
+  if (first < 0 || last < 1 || top < 0) return fail(TCU_EINVAL, "first %d and top %d must not be negative, last %d must be at least 1", first, top, last);
+  if ((int64_t)first + last + top > TCU_PAGED_MAX_SELECTED)
+    return fail(TCU_EINVAL, "%lld pages a query, at most %d", (long long)first + last + top, TCU_PAGED_MAX_SELECTED);
+  return TCU_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, const int32_t* fresh, int32_t page_tokens, int32_t* tables,
+                  int32_t table_width, int64_t table_stride, const int32_t* free_pages, int32_t n_free, int32_t capacity, int32_t* starts,
+                  int32_t* lengths, int32_t* positions, int64_t* slots, int32_t* counts) {
+  if (n < 0 || n_free < 0 || capacity < 0 || table_width < 0) return fail(TCU_EINVAL, "negative count");
+  if (page_tokens < 1 || page_tokens > TCU_PAGED_MAX_PAGE_TOKENS)
+    return fail(TCU_EINVAL, "%d positions a page, 1..%d are possible", page_tokens, TCU_PAGED_MAX_PAGE_TOKENS);
+  if (table_stride < table_width) return fail(TCU_EINVAL, "table stride %lld below the width %d", (long long)table_stride, table_width);
+  if (!starts || !counts || (n > 0 && (!held || !fresh || !lengths)) || (capacity > 0 && (!positions || !slots)) ||
+      (n > 0 && table_width > 0 && !tables) || (n_free > 0 && !free_pages))
+    return fail(TCU_EINVAL, "null argument");
+  OnDevice on(device);
+  TRY(on.rc);
+  TRY(check_ptr("starts", starts, device, 4));
+  TRY(check_ptr("counts", counts, device, 4));
+  if (n > 0) {
+    TRY(check_ptr("held", held, device, 4));
+    TRY(check_ptr("fresh", fresh, device, 4));
+    TRY(check_ptr("lengths", lengths, device, 4));
+    if (table_width > 0) TRY(check_ptr("tables", tables, device, 4));
+  }
+  if (n_free > 0) TRY(check_ptr("free_pages", free_pages, device, 4));
+  if (capacity > 0) {
+    TRY(check_ptr("positions", positions, device, 4));
+    TRY(check_ptr("slots", slots, device, 8));
+  }
+  PlanArgs a{};
+  a.n = n;
+  a.P = page_tokens;
+  a.width = table_width;
+  a.n_free = n_free;
+  a.capacity = capacity;
+  a.held = held;
+  a.fresh = fresh;
+  a.tables = tables;
+  a.table_stride = table_stride;
+  a.free_pages = free_pages;
+  a.starts = starts;
+  a.lengths = lengths;
+  a.positions = positions;
+  a.slots = slots;
+  a.counts = counts;
+  a.divP = FastDiv::of((uint32_t)page_tokens);
+  const unsigned grid = (unsigned)std::max<int64_t>(1, ceil_div(capacity, PLAN_TILE));
+  k_plan_step<<<grid, PLAN_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return launched("k_plan_step");
+}
+
+int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t dtype, int32_t rows, int32_t heads, const void* qkv,
+                     int64_t qkv_stride, const int32_t* positions, const int64_t* slots, const tcu_rotary* rotary, const tcu_head_norm* norm,
+                     void* q_out, int64_t q_stride) {
+  TRY(check_kv(kv));
+  TRY(check_pair(dtype, kv->dtype));
+  if (rows < 0 || heads < 1) return fail(TCU_EINVAL, "%d rows of %d heads", rows, heads);
+  const int hd = kv->head_dim;
+  const int64_t width = ((int64_t)heads + 2 * kv->kv_heads) * hd, per16 = 16 / elem_bytes(dtype);
+  if ((int64_t)rows * (heads + 2 * kv->kv_heads) > 0x7fffffffll) return fail(TCU_EINVAL, "too many rows for one call");
+  if (qkv_stride < width || q_stride < (int64_t)heads * hd) return fail(TCU_EINVAL, "a row's stride is below its width");
+  if (qkv_stride % per16 || q_stride % per16) return fail(TCU_EINVAL, "row strides must be multiples of 16 bytes");
+  AppendArgs a{};
+  if (rotary && rotary->pairs > 0) {
+    if (rotary->pairs * 2 > hd) return fail(TCU_EINVAL, "%d rotary pairs in a head of %d", rotary->pairs, hd);
+    if (rotary->max_positions < 1 || !rotary->table) return fail(TCU_EINVAL, "empty rotary table");
+    a.table = reinterpret_cast<const float2*>(rotary->table);
+    a.max_positions = rotary->max_positions;
+    a.pairs = rotary->pairs;
+    a.adjacent = rotary->adjacent != 0;
+  } else if (rotary && rotary->pairs < 0) {
+    return fail(TCU_EINVAL, "%d rotary pairs", rotary->pairs);
+  }
+  if (norm && norm->kind != TCU_NORM_NONE) {
+    if (norm->kind != TCU_NORM_RMS && norm->kind != TCU_NORM_LAYER) return fail(TCU_EINVAL, "unknown norm %d", norm->kind);
+    if (!(norm->eps >= 0) || std::isinf(norm->eps)) return fail(TCU_EINVAL, "norm epsilon %g", norm->eps);
+    if (norm->head_stride != 0 && norm->head_stride != hd) return fail(TCU_EINVAL, "norm weights are shared (stride 0) or per head (stride %d)", hd);
+    a.norm = norm->kind == TCU_NORM_RMS ? NORM_RMS : NORM_LAYER;
+    a.eps = (float)norm->eps;
+    a.qw = norm->q_weight;
+    a.kw = norm->k_weight;
+    a.w_stride = norm->head_stride;
+  }
+  if (rows > 0 && (!qkv || !positions || !slots || !q_out || !kv->k || !kv->v)) return fail(TCU_EINVAL, "null argument");
+  OnDevice on(device);
+  TRY(on.rc);
+  if (rows == 0) return TCU_OK;
+  TRY(check_ptr("k", kv->k, device, 16));
+  TRY(check_ptr("v", kv->v, device, 16));
+  TRY(check_ptr("qkv", qkv, device, 16));
+  TRY(check_ptr("q_out", q_out, device, 16));
+  TRY(check_ptr("positions", positions, device, 4));
+  TRY(check_ptr("slots", slots, device, 8));
+  if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 8));
+  if (a.norm) {
+    TRY(check_ptr("q_weight", a.qw, device, 16));
+    TRY(check_ptr("k_weight", a.kw, device, 16));
+  }
+  a.T = rows;
+  a.H = heads;
+  a.KVH = kv->kv_heads;
+  a.hd = hd;
+  a.qkv = qkv;
+  a.qkv_stride = qkv_stride;
+  a.positions = positions;
+  a.slots = slots;
+  a.q_out = q_out;
+  a.q_stride = q_stride;
+  a.kv = view_of(kv);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == TCU_F32 && kv->dtype == TCU_F32)
+    launch_append<float, float>(a, s);
+  else if (dtype == TCU_F32)
+    launch_append<float, __half>(a, s);
+  else if (dtype == TCU_F16)
+    launch_append<__half, __half>(a, s);
+  else
+    launch_append<bf16, bf16>(a, s);
+  return launched("k_append");
+}
+
+int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t rows, const int64_t* slots, void* means) {
+  TRY(check_kv(kv));
+  if (rows < 0) return fail(TCU_EINVAL, "%d rows", rows);
+  if (rows > 0 && (!slots || !means || !kv->k)) return fail(TCU_EINVAL, "null argument");
+  OnDevice on(device);
+  TRY(on.rc);
+  if (rows == 0) return TCU_OK;
+  TRY(check_ptr("k", kv->k, device, 16));
+  TRY(check_ptr("slots", slots, device, 8));
+  TRY(check_ptr("means", means, device, 16));
+  MeansArgs a{};
+  a.T = rows;
+  a.slots = slots;
+  a.means = means;
+  a.kv = view_of(kv);
+  const dim3 grid((unsigned)ceil_div(rows, 128), kv->kv_heads);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (kv->dtype == TCU_F32)
+    k_page_means<float><<<grid, 128, 0, s>>>(a);
+  else if (kv->dtype == TCU_F16)
+    k_page_means<__half><<<grid, 128, 0, s>>>(a);
+  else
+    k_page_means<bf16><<<grid, 128, 0, s>>>(a);
+  return launched("k_page_means");
+}
+
+int tcu_paged_attend_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* q, int32_t prefix_pages, int32_t max_length, uint64_t* bytes) {
+  if (!bytes) return fail(TCU_EINVAL, "null argument");
+  TRY(check_kv(kv));
+  TRY(check_queries(kv, q));
+  TRY(check_prefix(kv, prefix_pages, max_length));
+  *bytes = plan_attend(kv, q, prefix_pages, length_bound(kv, q, prefix_pages, max_length), 0).bytes;
+  return TCU_OK;
+}
+
+int tcu_paged_attend(int32_t device, void* stream, const tcu_paged_kv* kv, const tcu_paged_queries* q, const int32_t* prefix,
+                     int32_t prefix_pages, int32_t max_length, void* workspace, uint64_t workspace_bytes) {
+  TRY(check_kv(kv));
+  TRY(check_queries(kv, q));
+  TRY(check_prefix(kv, prefix_pages, max_length));
+  if (prefix_pages > 0 && !prefix) return fail(TCU_EINVAL, "prefix is null");
+  OnDevice on(device);
+  TRY(on.rc);
+  if (q->requests == 0 || q->rows == 0) return TCU_OK;
+  TRY(check_query_ptrs(kv, q, device));
+  if (prefix_pages > 0) TRY(check_ptr("prefix", prefix, device, 4));
+  const int bound = length_bound(kv, q, prefix_pages, max_length);
+  const AttendPlan p = plan_attend(kv, q, prefix_pages, bound, 0);
+  TRY(check_workspace(p, workspace, workspace_bytes, device));
+  AttendArgs a = attend_args(kv, q, p, workspace);
+  a.prefix = prefix;
+  a.prefix_pages = prefix_pages;
+  a.max_length = bound;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (q->dtype == TCU_F32 && kv->dtype == TCU_F32) return launch_attend<float, float>(a, p, s);
+  if (q->dtype == TCU_F32) return launch_attend<float, __half>(a, p, s);
+  if (q->dtype == TCU_F16) return launch_attend<__half, __half>(a, p, s);
+  return launch_attend<bf16, bf16>(a, p, s);
+}
+
+int tcu_paged_attend_sparse_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* q, int32_t first, int32_t last, int32_t top, uint64_t* bytes) {
+  if (!bytes) return fail(TCU_EINVAL, "null argument");
+  TRY(check_kv(kv));
+  TRY(check_queries(kv, q));
+  TRY(check_sparse(q, first, last, top));
+  *bytes = plan_attend(kv, q, 0, 0, first + last + top).bytes;
+  return TCU_OK;
+}
+
+int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv, const tcu_paged_queries* q, const void* means, int32_t first,
+                            int32_t last, int32_t top, int32_t* pages, void* workspace, uint64_t workspace_bytes) {
+  TRY(check_kv(kv));
+  TRY(check_queries(kv, q));
+  TRY(check_sparse(q, first, last, top));
+  OnDevice on(device);
+  TRY(on.rc);
+  if (q->requests == 0 || q->rows == 0) return TCU_OK;
+  TRY(check_query_ptrs(kv, q, device));
+  TRY(check_ptr("means", means, device, 16));
+  TRY(check_ptr("pages", pages, device, 4));
+  const AttendPlan p = plan_attend(kv, q, 0, 0, first + last + top);
+  TRY(check_workspace(p, workspace, workspace_bytes, device));
+  AttendArgs a = attend_args(kv, q, p, workspace);
+  a.max_length = (int)std::min<int64_t>((int64_t)q->table_width * kv->page_tokens, 0x7fffffff);
+  a.pages = pages;
+  a.budget = first + last + top;
+  ChooseArgs c{};
+  c.first = first;
+  c.last = last;
+  c.top = top;
+  c.means = means;
+  c.keys = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + p.keys);
+  c.width = q->table_width;
+  c.pages = pages;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (q->dtype == TCU_F32 && kv->dtype == TCU_F32) return launch_sparse<float, float>(a, c, p, s);
+  if (q->dtype == TCU_F32) return launch_sparse<float, __half>(a, c, p, s);
+  if (q->dtype == TCU_F16) return launch_sparse<__half, __half>(a, c, p, s);
+  return launch_sparse<bf16, bf16>(a, c, p, s);
+}
+
+}  // extern "C"

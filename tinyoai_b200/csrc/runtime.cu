@@ -37,6 +37,7 @@
 #include "tp_exchange.cuh"
 #include "gguf.h"
 #include "kv_snapshot.h"
+#include "status.h"
 
 using namespace tcu;
 
@@ -55,6 +56,11 @@ static int fail(int code, const char* fmt, ...) {
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
   g_err = buf;
+  return code;
+}
+
+int tcu::set_error(int code, const char* message) {
+  g_err = message;
   return code;
 }
 
@@ -376,6 +382,29 @@ static int check_device(int device) {
   if (prop.major != 10) return fail(TCU_ENODEV, "device %d is sm_%d%d; this library is built for sm_100a", device, prop.major, prop.minor);
   CK(cudaSetDevice(device));
   return sampling_smem_attrs(device);
+}
+
+// The architecture of each device, checked once (operators that keep no
+// handle call this every time).
+int tcu::require_device(int device) {
+  static std::mutex mu;
+  static bool known[64] = {};
+  if (device >= 0 && device < 64) {
+    std::lock_guard<std::mutex> g(mu);
+    if (known[device]) return TCU_OK;
+  }
+  int n = 0;
+  if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+    cudaGetLastError();
+    return fail(TCU_ENODEV, "no CUDA device available");
+  }
+  if (device < 0 || device >= n || device >= 64) return fail(TCU_ENODEV, "device %d out of range (%d devices)", device, n);
+  int major = 0;
+  CK(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  if (major != 10) return fail(TCU_ENODEV, "device %d is not sm_100; this library is built for sm_100a", device);
+  std::lock_guard<std::mutex> g(mu);
+  known[device] = true;
+  return TCU_OK;
 }
 
 static void init_common(tcu_model* m, const tcu_load_options* o) {
