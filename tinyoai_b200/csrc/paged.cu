@@ -11,6 +11,7 @@
 
 #include "../../include/tinyoai_cuda.h"
 #include "paged.cuh"
+#include "paged_mma.cuh"
 #include "status.h"
 
 using namespace tcu;
@@ -141,46 +142,55 @@ void launch_append(const AppendArgs& a, cudaStream_t s) {
 // Attention
 
 struct AttendPlan {
-  int prefix_chunk = 0, prefix_slots = 0, own_chunk = 0, own_slots = 0, slots = 0;
-  size_t part_o = 0, part_ml = 0, keys = 0, pages = 0, bytes = 0;  // offsets of the workspace regions
+  int prefix_rows = 0, prefix_chunk = 0, prefix_slots = 0, own_rows = 0, own_chunk = 0, own_slots = 0, slots = 0;
+  size_t part_o = 0, part_ml = 0, keys = 0, bytes = 0;  // offsets of the workspace regions, and their size
 };
-
-// Positions per part: enough CTAs for four on each SM, but parts of at least
-// 128 positions, whose own cost (its queries, its partial) a shorter one
-// would not earn back.
-int chunk_of(int64_t positions, int64_t ctas_per_part, int sms) {
-  const int64_t want = std::max<int64_t>(1, 4LL * sms / std::max<int64_t>(1, ctas_per_part));
-  int64_t c = std::max<int64_t>(128, ceil_div(ceil_div(positions, want), 64) * 64);
-  c = std::max<int64_t>(c, ceil_div(ceil_div(positions, 256), 64) * 64);  // at most 256 parts
-  return (int)std::min<int64_t>(c, 1 << 30);
-}
 
 constexpr int SM_COUNT = 148;  // B200
 
+// Positions per part: enough CTAs for four on each SM, but parts of at least
+// 128 positions, whose own cost (its queries, its partial) a shorter one
+// would not earn back, and of at most MM_IDS pages.
+int chunk_of(int64_t positions, int64_t ctas_per_part, int P) {
+  const int64_t want = std::max<int64_t>(1, 4LL * SM_COUNT / std::max<int64_t>(1, ctas_per_part));
+  int64_t c = std::max<int64_t>(128, ceil_div(ceil_div(positions, want), 64) * 64);
+  c = std::min<int64_t>(c, std::max<int64_t>(64, (int64_t)(MM_IDS - 2) * P / 64 * 64));
+  return (int)std::min<int64_t>(c, 1 << 30);
+}
+
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-int rows_per_cta(int hd) { return hd <= 128 ? 4 : 2; }
+// Query rows a CTA takes: CUDA cores 4 (their state lives in registers, hd
+// values each), matrix instructions 8, 16 or 32.
+int rows_per_cta(const tcu_paged_kv* kv, int64_t rows) {
+  if (kv->dtype == TCU_F32) return kv->head_dim <= 128 ? 4 : 2;
+  if (rows <= 8) return 8;
+  return rows <= 16 || kv->head_dim > 128 ? 16 : 32;
+}
 
 AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, int max_length, int budget) {
   AttendPlan p;
-  const int G = q->heads / kv->kv_heads, R = rows_per_cta(kv->head_dim), P = kv->page_tokens;
+  const int G = q->heads / kv->kv_heads, P = kv->page_tokens;
   const int64_t T = q->rows;
   if (budget > 0) {
-    p.own_chunk = chunk_of((int64_t)budget * P, T * kv->kv_heads * ceil_div(G, R), SM_COUNT);
+    p.own_rows = rows_per_cta(kv, G);
+    p.own_chunk = chunk_of((int64_t)budget * P, T * kv->kv_heads * ceil_div(G, p.own_rows), P);
     p.own_slots = (int)ceil_div((int64_t)budget * P, p.own_chunk);
   } else {
     const int64_t shared = (int64_t)prefix_pages * P;
+    p.prefix_rows = rows_per_cta(kv, T * G);
+    p.own_rows = rows_per_cta(kv, (int64_t)q->max_fresh * G);
     if (shared > 0) {
-      p.prefix_chunk = chunk_of(shared, ceil_div(T * G, R) * kv->kv_heads, SM_COUNT);
+      p.prefix_chunk = chunk_of(shared, ceil_div(T * G, p.prefix_rows) * kv->kv_heads, P);
       p.prefix_slots = (int)ceil_div(shared, p.prefix_chunk);
     }
     const int64_t own = std::max<int64_t>(0, (int64_t)max_length - shared);
-    p.own_chunk = chunk_of(own, (int64_t)q->requests * kv->kv_heads * ceil_div((int64_t)q->max_fresh * G, R), SM_COUNT);
+    p.own_chunk = chunk_of(own, (int64_t)q->requests * kv->kv_heads * ceil_div((int64_t)q->max_fresh * G, p.own_rows), P);
     p.own_slots = (int)ceil_div(own, p.own_chunk);
   }
   p.slots = std::max(1, p.prefix_slots + p.own_slots);
   size_t off = 0;
-  const size_t rows = (size_t)T * q->heads;
+  const size_t rows = p.slots > 1 ? (size_t)T * q->heads : 0;
   p.part_o = off;
   off += align256(rows * p.slots * kv->head_dim * sizeof(float));
   p.part_ml = off;
@@ -189,43 +199,81 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
     p.keys = off;
     off += align256((size_t)T * kv->kv_heads * q->table_width * sizeof(unsigned long long));
   }
-  p.bytes = off;
+  p.bytes = std::max<size_t>(off, 256);
   return p;
+}
+
+// x of the grid and row tiles for CTAs of `rows` rows.
+template <int SRC>
+int64_t grid_x(const AttendArgs& a, int rows, int* tiles) {
+  if (SRC == SRC_PREFIX) {
+    *tiles = (int)ceil_div((int64_t)a.T * a.G, rows);
+    return *tiles;
+  }
+  *tiles = (int)ceil_div(SRC == SRC_OWN ? (int64_t)a.max_fresh * a.G : a.G, rows);
+  return (int64_t)a.n * (SRC == SRC_OWN ? 1 : a.max_fresh) * *tiles;
+}
+
+// Raises a kernel's dynamic shared memory limit (it is a property of the
+// kernel on the current device; setting it again changes nothing).
+template <typename K>
+int allow_smem(K kern, size_t bytes) {
+  if (bytes > 48 * 1024) CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  return TCU_OK;
 }
 
 template <typename TQ, typename TK, int NCH, int R, int SRC>
 int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
-  int64_t x;
   int tiles;
-  if (SRC == SRC_PREFIX) {
-    tiles = (int)ceil_div((int64_t)a.T * a.G, R);
-    x = tiles;
-  } else if (SRC == SRC_OWN) {
-    tiles = (int)ceil_div((int64_t)a.max_fresh * a.G, R);
-    x = (int64_t)a.n * tiles;
-  } else {
-    tiles = (int)ceil_div(a.G, R);
-    x = (int64_t)a.n * a.max_fresh * tiles;
-  }
+  const int64_t x = grid_x<SRC>(a, R, &tiles);
   const size_t smem = sizeof(float) * CC_GROUPS * (NCH * 32 + 2);
   k_attend_cc<TQ, TK, NCH, R, SRC><<<dim3((unsigned)x, a.KVH, parts), CC_WARPS * 32, smem, s>>>(a, tiles);
   return launched("k_attend_cc");
 }
 
+template <typename TQ, typename TK, int HD, int NT, int SRC>
+int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
+  int tiles;
+  const int64_t x = grid_x<SRC>(a, 8 * NT, &tiles);
+  constexpr size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>();
+  auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
+  TRY(allow_smem(kern, smem));
+  kern<<<dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s>>>(a, tiles);
+  return launched("k_attend_mma");
+}
+
+template <typename TQ, typename TK, int HD, int SRC>
+int launch_mma(const AttendArgs& a, int rows, int parts, cudaStream_t s) {
+  if (rows == 8) return launch_mma_n<TQ, TK, HD, 1, SRC>(a, parts, s);
+  if (rows == 16) return launch_mma_n<TQ, TK, HD, 2, SRC>(a, parts, s);
+  if constexpr (HD <= 128) return launch_mma_n<TQ, TK, HD, 4, SRC>(a, parts, s);
+  return fail(TCU_EINVAL, "no kernel for %d rows", rows);
+}
+
+// The parts of one source of positions: CUDA cores for float32 caches, matrix
+// instructions for 16-bit ones.
 template <typename TQ, typename TK, int SRC>
-int launch_cc(const AttendArgs& a, int parts, cudaStream_t s) {
+int launch_parts(const AttendArgs& a, int rows, int parts, cudaStream_t s) {
   if (parts == 0) return TCU_OK;
-  const int nch = (a.hd + 31) / 32;
-  if (nch <= 2) return launch_cc_r<TQ, TK, 2, 4, SRC>(a, parts, s);
-  if (nch <= 3) return launch_cc_r<TQ, TK, 3, 4, SRC>(a, parts, s);
-  if (nch <= 4) return launch_cc_r<TQ, TK, 4, 4, SRC>(a, parts, s);
-  return launch_cc_r<TQ, TK, 8, 2, SRC>(a, parts, s);
+  if constexpr (sizeof(TK) == 4) {
+    const int nch = (a.hd + 31) / 32;
+    if (nch <= 2) return launch_cc_r<TQ, TK, 2, 4, SRC>(a, parts, s);
+    if (nch <= 3) return launch_cc_r<TQ, TK, 3, 4, SRC>(a, parts, s);
+    if (nch <= 4) return launch_cc_r<TQ, TK, 4, 4, SRC>(a, parts, s);
+    return launch_cc_r<TQ, TK, 8, 2, SRC>(a, parts, s);
+  } else {
+    if (a.hd <= 64) return launch_mma<TQ, TK, 64, SRC>(a, rows, parts, s);
+    if (a.hd <= 96) return launch_mma<TQ, TK, 96, SRC>(a, rows, parts, s);
+    if (a.hd <= 128) return launch_mma<TQ, TK, 128, SRC>(a, rows, parts, s);
+    return launch_mma<TQ, TK, 256, SRC>(a, rows, parts, s);
+  }
 }
 
 template <typename TQ, typename TK>
 int launch_attend(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
-  TRY((launch_cc<TQ, TK, SRC_PREFIX>(a, p.prefix_slots, s)));
-  TRY((launch_cc<TQ, TK, SRC_OWN>(a, p.own_slots, s)));
+  TRY((launch_parts<TQ, TK, SRC_PREFIX>(a, p.prefix_rows, p.prefix_slots, s)));
+  TRY((launch_parts<TQ, TK, SRC_OWN>(a, p.own_rows, p.own_slots, s)));
+  if (p.prefix_slots + p.own_slots == 1) return TCU_OK;  // the only part wrote the output
   k_attend_join<TQ, 0><<<dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s>>>(a);
   return launched("k_attend_join");
 }
@@ -235,13 +283,14 @@ int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p,
   const unsigned queries = (unsigned)((int64_t)a.n * a.max_fresh);
   if (c.top > 0 && c.width > 0) {
     const size_t smem = sizeof(double) * a.G * a.hd;
-    if (smem > 48 * 1024) CK(cudaFuncSetAttribute(k_page_scores<TQ, TK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    TRY(allow_smem(k_page_scores<TQ, TK>, smem));
     k_page_scores<TQ, TK><<<dim3(queries, a.KVH, (unsigned)ceil_div(c.width, 64)), 128, smem, s>>>(a, c);
     TRY(launched("k_page_scores"));
   }
   k_page_choose<<<dim3(queries, a.KVH), CHOOSE_THREADS, 0, s>>>(a, c);
   TRY(launched("k_page_choose"));
-  TRY((launch_cc<TQ, TK, SRC_LIST>(a, p.own_slots, s)));
+  TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
+  if (p.own_slots == 1) return TCU_OK;  // the only part wrote the output
   k_attend_join<TQ, 1><<<dim3(queries, (a.H + 3) / 4), 128, 0, s>>>(a);
   return launched("k_attend_join");
 }

@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "common.cuh"
 #include "tma.cuh"
 
 namespace tcu {
@@ -490,6 +491,9 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 1 / l, 0 for a row that saw nothing; NaN stays NaN.
+__device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
+
 // CUDA-core parts. A warp holds four groups of eight lanes; a group takes
 // every fourth position of its warp's share and keeps a softmax state of its
 // own for each of R rows, so that nothing is exchanged until the end: dot
@@ -558,7 +562,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     ids = a.pages + ((int64_t)token0 * a.KVH + g) * a.budget;
     table = a.tables + (int64_t)(request / a.max_fresh) * a.table_stride;
   }
-  if (SRC == SRC_OWN && u0 >= u1) return;  // k_attend_join counts the parts by the same rule
+  if (SRC == SRC_OWN && u0 >= u1 && !(part == 0 && a.slots == 1)) return;  // k_attend_join counts the parts by the same rule
 
   float q[R][NCH][4], o[R][NCH][4], m[R], l[R];
 #pragma unroll
@@ -676,13 +680,19 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
       ls = fmaf(sml[2 * i + 1], w[i], ls);
     }
     const int64_t slot = (int64_t)row_out[r] * a.slots + (SRC == SRC_OWN ? a.prefix_slots : 0) + part;
+    const bool direct = a.slots == 1;  // the only part: the output itself
+    const float inv = inverse_sum(ls);
+    TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)(row_out[r] / a.H) * a.o_ts + (int64_t)(row_out[r] % a.H) * a.o_hs;
     for (int d = threadIdx.x; d < hd; d += CC_WARPS * 32) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < CC_GROUPS; i++) s = fmaf(so[i * width + d], w[i], s);
-      a.part_o[slot * hd + d] = s;
+      if (direct)
+        store_as(out + d, s * inv);
+      else
+        a.part_o[slot * hd + d] = s;
     }
-    if (threadIdx.x == 0) a.part_ml[slot] = make_float2(mx, ls);
+    if (threadIdx.x == 0 && !direct) a.part_ml[slot] = make_float2(mx, ls);
   }
 }
 
@@ -714,7 +724,7 @@ __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
   const float ref = mx == -INFINITY ? 0.f : mx;
   float l = 0.f;
   for (int p = 0; p < parts; p++) l = fmaf(ml[p].y, ex2(ml[p].x - ref), l);
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // NaN stays NaN
+  const float inv = inverse_sum(l);
   TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)q.token * a.o_ts + (int64_t)h * a.o_hs;
   const float* po = a.part_o + row * a.slots * a.hd;
   for (int d = lane; d < a.hd; d += 32) {

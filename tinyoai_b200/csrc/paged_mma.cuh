@@ -1,0 +1,403 @@
+// Attention over 16-bit paged caches for few query rows at a time (decode
+// steps, selected pages): the cache streams once from HBM through registers
+// into warp-level matrix instructions.
+//
+// Bytes bound this: a step reads 4 * hd bytes of cache per position and KV
+// head and spends 4 * hd flops per query head on them, far below what a
+// 128-row tcgen05 tile needs to be worth filling (G = H / KVH rows). So a
+// warp takes 16 positions at a time and computes S^T = K Q^T and O^T = V^T P^T
+// with m16n8k16: positions (then features) are the 16 rows, query rows the 8
+// columns. Operands come straight from global memory, with no shared memory
+// and no data exchange in between:
+//  - K (rows = positions, k = features): a lane loads 16 bytes of a position,
+//    eight neighbouring features, and takes them as its k entries of two
+//    steps; Q is read with the same order of features, which a sum over
+//    features does not notice.
+//  - V^T (rows = features, k = positions): a lane loads the same eight
+//    features of four positions and interleaves them pairwise; feature 2j and
+//    2j + 1 of the eight become rows r and r + 8 of product j.
+//  - P^T leaves the first product with positions in rows; one 8 x 8 transpose
+//    within the warp (movmatrix) gives the second product's operand.
+// The softmax statistics are float32, one running maximum per warp and query
+// row; the weights are rounded to the cache's type as operands. Float32
+// queries over a binary16 cache keep 22 bits: q * 2^sx and the weights are
+// each two binary16 values and each product two instructions.
+//
+// A CTA's warps take alternate 16-position tiles of the CTA's part and join
+// their states through shared memory in warp order.
+#pragma once
+#include "paged.cuh"
+
+namespace tcu {
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<bf16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+constexpr int MM_WARPS = 4;
+constexpr int MM_IDS = 1024;  // page ids of a part, copied to shared memory (a part has at most this many pages)
+
+// Shared memory: the queries [PIECES][8 NT columns][HD + 32] 16-bit values (the pad puts
+// the two rows a quarter warp reads on different banks), then, when the loop
+// is over, the warps' outputs [MM_WARPS][8 NT][HD + 4] float32 and their (m, l).
+template <int HD, int NT, int PIECES>
+constexpr size_t mm_smem() {
+  const size_t q = (size_t)PIECES * 8 * NT * (HD + 32) * 2, o = (size_t)MM_WARPS * 8 * NT * (HD + 4 + 2) * 4;
+  return q > o ? q : o;
+}
+
+// grid as k_attend_cc's, with row tiles of 8 * NT rows.
+template <typename TQ, typename TK, int HD, int NT, int SRC>
+__global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT == 4 || HD > 128 ? 2 : 3) k_attend_mma(AttendArgs a, int row_tiles) {
+  constexpr int COLS = 8 * NT, KG = (HD + 31) / 32, VG = (HD + 63) / 64;
+  constexpr int PIECES = sizeof(TQ) == 4 ? 2 : 1;
+  constexpr int QS = HD + 32;
+  extern __shared__ __align__(16) uint8_t mm_mem[];
+  __shared__ int s_limit[COLS], s_row[COLS], s_ids[MM_IDS];
+  __shared__ float s_scale[COLS];
+  TK* qs = reinterpret_cast<TK*>(mm_mem);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, c = lane & 3;
+  const int g = blockIdx.y, part = blockIdx.z, hd = a.hd;
+  const int tile = SRC == SRC_PREFIX ? blockIdx.x : blockIdx.x % row_tiles;
+  const int request = SRC == SRC_PREFIX ? 0 : blockIdx.x / row_tiles;
+  if (tid < COLS) {
+    const int row = tile * COLS + tid;
+    Query q;
+    int hh = row % a.G;
+    if (SRC == SRC_PREFIX) {
+      q = query_of(a, row / a.G);
+    } else if (SRC == SRC_OWN) {
+      q = row / a.G < a.max_fresh ? query_at(a, request, row / a.G) : Query{-1, request, -1};
+    } else {  // "request" counts (request, query) pairs
+      q = query_at(a, request / a.max_fresh, request % a.max_fresh);
+      if (row >= a.G) q.token = -1;
+    }
+    s_limit[tid] = q.token < 0 ? -2 : q.pos;  // -2: no row, -1: a row that sees nothing
+    s_row[tid] = q.token < 0 ? -1 : q.token * a.H + g * a.G + hh;
+  }
+  __syncthreads();
+  int most = -2, least = 0x7fffffff;
+#pragma unroll
+  for (int i = 0; i < COLS; i++) {
+    const int x = s_limit[i];
+    most = max(most, x);
+    if (x > -2) least = min(least, x);
+  }
+  if (most == -2) return;
+  int u0, u1;
+  const int prefix_end = a.prefix_pages * a.kv.P;
+  if (SRC == SRC_PREFIX) {
+    u0 = part * a.prefix_chunk;
+    u1 = min(min(u0 + a.prefix_chunk, prefix_end), most + 1);
+  } else if (SRC == SRC_OWN) {
+    u0 = prefix_end + part * a.own_chunk;
+    u1 = min(u0 + a.own_chunk, most + 1);
+    if (u0 >= u1 && !(part == 0 && a.slots == 1)) return;  // k_attend_join counts the parts by the same rule
+  } else {
+    u0 = part * a.own_chunk;
+    u1 = min(u0 + a.own_chunk, a.budget * a.kv.P);
+  }
+  // The part's page ids (-1: no page) and, for a list, the pages' first positions.
+  const int b0 = (int)a.kv.divP.div(u0);
+  __shared__ int s_first[SRC == SRC_LIST ? MM_IDS : 1];
+  {
+    const int nb = u1 > u0 ? (int)a.kv.divP.div(u1 - 1) - b0 + 1 : 0;
+    if (SRC == SRC_LIST) {
+      const int token = s_row[0] / a.H;
+      const int* list = a.pages + ((int64_t)token * a.KVH + g) * a.budget;
+      const int* table = a.tables + (int64_t)(request / a.max_fresh) * a.table_stride;
+      for (int e = tid; e < nb; e += MM_WARPS * 32) {
+        const int j = list[b0 + e];
+        int id = j >= 0 && j < a.width ? table[j] : -1;
+        if (id >= a.kv.num_pages) id = -1;
+        s_ids[e] = id;
+        s_first[e] = id < 0 ? 0x3fffffff : j * a.kv.P;
+      }
+    } else {
+      const int* ids = SRC == SRC_PREFIX ? a.prefix : a.tables + (int64_t)request * a.table_stride;
+      for (int e = tid; e < nb; e += MM_WARPS * 32) {
+        int id = SRC == SRC_PREFIX || b0 + e < a.width ? ids[b0 + e] : -1;
+        if (id >= a.kv.num_pages) id = -1;
+        s_ids[e] = id;
+      }
+    }
+  }
+  // Queries into shared memory; float32 ones as pairs of binary16 values of q * 2^sx.
+  if (PIECES == 1) {
+    constexpr int CH = HD / 8;
+    for (int e = tid; e < COLS * CH; e += MM_WARPS * 32) {
+      const int col = e / CH, d = (e % CH) * 8, row = s_row[col];
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row >= 0 && d < hd)
+        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const TQ*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
+      *reinterpret_cast<uint4*>(qs + col * QS + d) = x;
+    }
+    if (tid < COLS) s_scale[tid] = a.scale;
+  } else {
+    for (int col = warp; col < COLS; col += MM_WARPS) {
+      const int row = s_row[col];
+      float x[(HD + 31) / 32], mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < (HD + 31) / 32; i++) {
+        const int d = lane + 32 * i;
+        x[i] = row >= 0 && d < hd ? (float)(reinterpret_cast<const TQ*>(a.q)[(int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d]) : 0.f;
+        mx = fmaxf(mx, fabsf(x[i]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // 2^sx brings the largest value into [2^13, 2^14). Infinite or NaN rows stay as they are.
+      int ex = 0;
+      if (mx > 0.f && mx < INFINITY) frexpf(mx, &ex);
+      const int sx = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+      const float up = __int_as_float((127 + sx) << 23);
+#pragma unroll
+      for (int i = 0; i < (HD + 31) / 32; i++) {
+        const int d = lane + 32 * i;
+        if (d < HD) {
+          const float y = x[i] * up;
+          const __half h = __float2half_rn(y);
+          const float rest = y - __half2float(h);
+          reinterpret_cast<__half*>(qs)[col * QS + d] = h;
+          reinterpret_cast<__half*>(qs)[COLS * QS + col * QS + d] = __float2half_rn(rest == rest ? rest : 0.f);
+        }
+      }
+      if (lane == 0) s_scale[col] = a.scale * __int_as_float((127 - sx) << 23);
+    }
+  }
+  __syncthreads();
+  float o[VG][4][NT][4], m[NT][2], l[NT][2], sc[NT][2];
+  int lim[NT][2];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      m[t][e] = -INFINITY;
+      l[t][e] = 0.f;
+      sc[t][e] = s_scale[t * 8 + 2 * c + e];
+      lim[t][e] = s_limit[t * 8 + 2 * c + e];
+#pragma unroll
+      for (int v = 0; v < VG; v++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          o[v][j][t][e] = 0.f;
+          o[v][j][t][2 + e] = 0.f;
+        }
+    }
+  const TK* kb = reinterpret_cast<const TK*>(a.kv.k) + (int64_t)g * a.kv.sh;
+  const TK* vb = reinterpret_cast<const TK*>(a.kv.v) + (int64_t)g * a.kv.sh;
+  const bool aligned = (a.kv.P & 15) == 0;  // a 16-position tile lies in one page
+  for (int ub = u0 + warp * 16; ub < u1; ub += MM_WARPS * 16) {
+    // Cache rows: positions r and r + 8 of the tile for K, 2c, 2c + 1, 2c + 8 and 2c + 9 for V.
+    int64_t ko[2], vo[4];
+    int tk[2], tv[4];
+    if (aligned) {
+      const int b = (int)a.kv.divP.div(ub), row0 = ub - b * a.kv.P, id = s_ids[b - b0];
+      const int64_t base = (int64_t)id * a.kv.sp + (int64_t)row0 * a.kv.st;
+      const int t0 = id < 0 ? 0x3fffffff : SRC == SRC_LIST ? s_first[b - b0] + row0 : ub;
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        ko[i] = base + (int64_t)(r + 8 * i) * a.kv.st;
+        tk[i] = t0 + r + 8 * i;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int x = 2 * c + (i & 1) + (i >> 1) * 8;
+        vo[i] = base + (int64_t)x * a.kv.st;
+        tv[i] = t0 + x;
+      }
+    } else {
+      auto at = [&](int u, int64_t& off, int& t) {
+        off = 0;
+        t = 0x3fffffff;
+        if (u >= u1) return;
+        const int b = (int)a.kv.divP.div(u), row = u - b * a.kv.P, id = s_ids[b - b0];
+        if (id < 0) return;
+        off = (int64_t)id * a.kv.sp + (int64_t)row * a.kv.st;
+        t = SRC == SRC_LIST ? s_first[b - b0] + row : u;
+      };
+#pragma unroll
+      for (int i = 0; i < 2; i++) at(ub + r + 8 * i, ko[i], tk[i]);
+#pragma unroll
+      for (int i = 0; i < 4; i++) at(ub + 2 * c + (i & 1) + (i >> 1) * 8, vo[i], tv[i]);
+    }
+    // Positions no row sees are not read: whatever lies there stays out of the products.
+    uint4 kx[2][KG], vx[VG][4];
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int q = 0; q < KG; q++) {
+        const int d = q * 32 + c * 8;
+        kx[i][q] = tk[i] <= most && d < hd ? ld_stream16(kb + ko[i] + d) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+    for (int v = 0; v < VG; v++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int d = v * 64 + r * 8;
+        vx[v][i] = tv[i] <= most && d < hd ? ld_stream16(vb + vo[i] + d) : make_uint4(0, 0, 0, 0);
+      }
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+#pragma unroll
+    for (int q = 0; q < KG; q++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+          const uint4 y = *reinterpret_cast<const uint4*>(qs + (p * COLS + t * 8 + r) * QS + q * 32 + c * 8);
+          mma16816<TK>(s[t], kx[0][q].x, kx[1][q].x, kx[0][q].y, kx[1][q].y, y.x, y.y);
+          mma16816<TK>(s[t], kx[0][q].z, kx[1][q].z, kx[0][q].w, kx[1][q].w, y.z, y.w);
+        }
+    // Scores in units of log2; rows: positions r (entries 0, 1) and r + 8 (2, 3).
+    float alpha[NT][2];
+    uint32_t ph[NT][2], pl[NT][2];
+    const bool masked = tk[1] > least || tk[0] > least;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        s[t][e] *= sc[t][e];
+        s[t][2 + e] *= sc[t][e];
+        if (masked) {
+          if (tk[0] > lim[t][e]) s[t][e] = -INFINITY;
+          if (tk[1] > lim[t][e]) s[t][2 + e] = -INFINITY;
+        }
+        float mx = fmaxf(s[t][e], s[t][2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        mx = fmaxf(mx, m[t][e]);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        alpha[t][e] = ex2(m[t][e] - ref);
+        m[t][e] = mx;
+        s[t][e] = ex2(s[t][e] - ref);
+        s[t][2 + e] = ex2(s[t][2 + e] - ref);
+        l[t][e] = fmaf(l[t][e], alpha[t][e], s[t][e] + s[t][2 + e]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        const uint32_t h = pack2<TK>(s[t][2 * i], s[t][2 * i + 1]);
+        ph[t][i] = transpose8x8(h);
+        if (PIECES == 2) {
+          const float2 hf = __half22float2(*reinterpret_cast<const __half2*>(&h));
+          pl[t][i] = transpose8x8(pack2<TK>(s[t][2 * i] - hf.x, s[t][2 * i + 1] - hf.y));
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VG; v++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const uint32_t x0 = j == 0 ? vx[v][0].x : j == 1 ? vx[v][0].y : j == 2 ? vx[v][0].z : vx[v][0].w;
+        const uint32_t x1 = j == 0 ? vx[v][1].x : j == 1 ? vx[v][1].y : j == 2 ? vx[v][1].z : vx[v][1].w;
+        const uint32_t x2 = j == 0 ? vx[v][2].x : j == 1 ? vx[v][2].y : j == 2 ? vx[v][2].z : vx[v][2].w;
+        const uint32_t x3 = j == 0 ? vx[v][3].x : j == 1 ? vx[v][3].y : j == 2 ? vx[v][3].z : vx[v][3].w;
+        const uint32_t a0 = __byte_perm(x0, x1, 0x5410), a1 = __byte_perm(x0, x1, 0x7632);
+        const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            o[v][j][t][e] *= alpha[t][e];
+            o[v][j][t][2 + e] *= alpha[t][e];
+          }
+          mma16816<TK>(o[v][j][t], a0, a1, a2, a3, ph[t][0], ph[t][1]);
+          if (PIECES == 2) mma16816<TK>(o[v][j][t], a0, a1, a2, a3, pl[t][0], pl[t][1]);
+        }
+      }
+  }
+  // Each lane's sums cover its own positions.
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 4);
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 8);
+      l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], 16);
+    }
+  __syncthreads();  // the queries are read
+  constexpr int OS = HD + 4;
+  float* so = reinterpret_cast<float*>(mm_mem);
+  float2* sml = reinterpret_cast<float2*>(so + MM_WARPS * COLS * OS);
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int col = t * 8 + 2 * c + e;
+      float* dst = so + (warp * COLS + col) * OS;
+#pragma unroll
+      for (int v = 0; v < VG; v++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int d = v * 64 + r * 8 + 2 * j;
+          if (d < HD) *reinterpret_cast<float2*>(dst + d) = make_float2(o[v][j][t][e], o[v][j][t][2 + e]);
+        }
+      if (r == 0) sml[warp * COLS + col] = make_float2(m[t][e], l[t][e]);
+    }
+  __syncthreads();
+  const bool direct = a.slots == 1;  // the only part: the output itself
+  for (int e = tid; e < COLS * (HD / 4); e += MM_WARPS * 32) {
+    const int col = e / (HD / 4), d = (e % (HD / 4)) * 4, row = s_row[col];
+    if (row < 0 || d >= hd) continue;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < MM_WARPS; w++) mx = fmaxf(mx, sml[w * COLS + col].x);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float ls = 0.f;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < MM_WARPS; w++) {
+      const float2 ml = sml[w * COLS + col];
+      const float f = ex2(ml.x - ref);
+      const float4 y = *reinterpret_cast<const float4*>(so + (w * COLS + col) * OS + d);
+      ls = fmaf(ml.y, f, ls);
+      x.x = fmaf(y.x, f, x.x);
+      x.y = fmaf(y.y, f, x.y);
+      x.z = fmaf(y.z, f, x.z);
+      x.w = fmaf(y.w, f, x.w);
+    }
+    if (direct) {
+      const float inv = inverse_sum(ls);
+      TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)(row / a.H) * a.o_ts + (int64_t)(row % a.H) * a.o_hs + d;
+      store4(out, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    } else {
+      const int64_t slot = (int64_t)row * a.slots + (SRC == SRC_OWN ? a.prefix_slots : 0) + part;
+      *reinterpret_cast<float4*>(a.part_o + slot * hd + d) = x;
+      if (d == 0) a.part_ml[slot] = make_float2(mx, ls);
+    }
+  }
+}
+
+}  // namespace tcu
