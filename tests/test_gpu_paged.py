@@ -412,6 +412,55 @@ def test_attend(qt, kt, case):
     assert bool((out[s["T"]:] == 5).all())  # rows behind the last request
 
 
+SHARED = [
+    # requests, fresh, H, KVH, hd, P, prefix pages, own positions, order: row tiles of the tensor cores
+    (40, 1, 4, 4, 80, 32, 17, 40, "heads"),          # one tile, the streams take alternate blocks, a part block at the end
+    (33, 1, 2, 1, 64, 8, 64, 9, "positions"),        # pages of 8, one 64-feature operand
+    (128, 1, 8, 8, 128, 16, 40, 33, "heads"),        # a full tile
+    (129, 1, 4, 4, 128, 64, 9, 70, "both"),          # two tiles, the second almost empty
+    (70, 3, 16, 2, 128, 32, 33, 5, "heads"),         # three tokens each, groups of 8
+    (100, 1, 28, 4, 112, 128, 5, 20, "heads"),       # groups of 7, pages of 128
+    (20, 2, 64, 1, 96, 256, 3, 300, "positions"),    # a group of 64, pages of 256
+    (300, 1, 4, 2, 72, 32, 24, 64, "heads"),         # 72 features
+    (64, 1, 2, 2, 64, 32, 150, 0, "heads"),          # nothing but the prefix
+]
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("case", range(len(SHARED)))
+def test_attend_shared_prefix_tiles(t, case):
+    n, fresh, H, KVH, hd, P, prefix, own, order = SHARED[case]
+    dt = TYPES[t]
+    lens = [prefix * P + (own * (i * 7 % 11)) // 10 for i in range(n)]
+    f = [1 + i % fresh for i in range(n)]
+    if case % 2:
+        lens[3], lens[5] = prefix * P // 2, 0  # shorter than the prefix, and empty
+        f[4] = 0
+    s = attention_state(lens, f, H, KVH, hd, P, dt, dt, seed=70 + case, prefix=prefix, order=order)
+    for scale in (1 / math.sqrt(hd), -0.7 / math.sqrt(hd), 0.0)[: 3 if case < 2 else 1]:
+        out = torch.full((s["T"] + 2, H, hd), 5.0, dtype=dt, device=DEV)
+        paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], max(f), prefix=s["prefix"], scale=scale,
+                                           max_length=s["lim"], out=out)
+        want, tol = expected(s, lens, f, H, KVH, hd, P, scale, prefix)
+        near(out[:s["T"]], want, tol)
+        assert bool((out[s["T"]:] == 5).all())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [48, 200])
+def test_attend_prefix_with_missing_pages(t, n):
+    """Ids outside the pool among the prefix's pages; a growing score, so that rows move their reference again and again."""
+    dt, P, prefix, hd = TYPES[t], 32, 40, 64
+    lens = [prefix * P + 1 + i % 40 for i in range(n)]
+    s = attention_state(lens, [1] * n, 2, 2, hd, P, dt, dt, seed=5, prefix=prefix)
+    for j in range(prefix):
+        s["k"][s["prefix"][j].long()] *= 0.2 + j / 4
+    s["prefix"][3], s["prefix"][4], s["prefix"][17], s["prefix"][39] = -1, 10 ** 6, -7, len(s["k"])
+    out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"])
+    want, tol = expected(s, lens, [1] * n, 2, 2, hd, P, 1 / math.sqrt(hd), prefix)
+    near(out[:n], want, tol)
+
+
 @pytest.mark.parametrize("qt, kt", PAIRS)
 def test_attend_ignores_missing_pages_and_stale_values(qt, kt):
     """Page ids outside the pool are no pages; the values behind a request's

@@ -55,6 +55,7 @@
 #include <cuda_bf16.h>
 #include "common.cuh"
 #include "gemv.cuh"
+#include "tcgen05.cuh"
 #include "tma.cuh"
 
 namespace tcu {
@@ -116,38 +117,11 @@ struct TcArgs {
 // 2^e exactly, for e in [-126, 127].
 __device__ __forceinline__ float tc_pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-__device__ __forceinline__ uint64_t tc_smem_desc(uint32_t saddr) {
-  // K-major operand, 128-byte swizzle: 8-row groups 1024 bytes apart (SBO),
-  // LBO unused (1), descriptor version 1, layout type 2 (SWIZZLE_128B).
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
 // Instruction descriptor: float32 accumulator, A and B both binary16 (or
 // both bfloat16), both K-major, N = n, M = 128.
 __device__ __forceinline__ uint32_t tc_idesc(int n, bool bf16) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TC_BM >> 4) << 24);
 }
-
-__device__ __forceinline__ void tc_mma(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(tmem_d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
-      : "memory");
-}
-
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, float (&v)[16]) {
   uint32_t r[16];

@@ -8,11 +8,14 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "../../include/tinyoai_cuda.h"
 #include "paged.cuh"
 #include "paged_mma.cuh"
+#include "paged_tc.cuh"
 #include "status.h"
+#include "tma_host.h"
 
 using namespace tcu;
 
@@ -143,6 +146,9 @@ void launch_append(const AppendArgs& a, cudaStream_t s) {
 
 struct AttendPlan {
   int prefix_rows = 0, prefix_chunk = 0, prefix_slots = 0, own_rows = 0, own_chunk = 0, own_slots = 0, slots = 0;
+  bool tc = false;  // the prefix on tcgen05
+  PagedTcArgs tc_args{};
+  int tc_tiles = 0, tc_parts = 0;
   size_t part_o = 0, part_ml = 0, keys = 0, bytes = 0;  // offsets of the workspace regions, and their size
 };
 
@@ -168,6 +174,50 @@ int rows_per_cta(const tcu_paged_kv* kv, int64_t rows) {
   return rows <= 16 || kv->head_dim > 128 ? 16 : 32;
 }
 
+// Whether the prefix goes to k_attend_prefix_tc, and how it is cut. The kernel
+// takes 16-bit rows and caches of one type, head sizes 64..128, pages that
+// tile 128 positions (or that 128 positions tile), strides TMA can describe,
+// and is worth its set-up from TC_MIN_ROWS rows and TC_MIN_BLOCKS blocks on.
+constexpr int TC_MIN_ROWS = 33, TC_MIN_BLOCKS = 4;
+
+void plan_tc(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, AttendPlan* p) {
+  const int P = kv->page_tokens, hd = kv->head_dim;
+  const int64_t rows = (int64_t)q->rows * (q->heads / kv->kv_heads), shared = (int64_t)prefix_pages * P;
+  const int64_t blocks = ceil_div(shared, PT_KEYS);
+  if (kv->dtype == TCU_F32 || q->dtype != kv->dtype || hd < 64 || hd > 128 || P % 8 || (P <= PT_KEYS ? PT_KEYS % P : P % PT_KEYS)) return;
+  if (rows < TC_MIN_ROWS || blocks < TC_MIN_BLOCKS) return;
+  const int64_t strides[3] = {kv->token_stride, kv->head_stride, kv->page_stride};
+  const int64_t dims[3] = {P, kv->kv_heads, kv->num_pages};
+  for (int i = 0; i < 3; i++)
+    if (strides[i] * 2 >= (1LL << 40) || (dims[i] > 1 && strides[i] == 0)) return;
+  p->tc = true;
+  const int split = rows <= PT_ROWS;
+  p->tc_tiles = (int)ceil_div(rows, split ? PT_ROWS : 2 * PT_ROWS);
+  const int64_t units = (int64_t)p->tc_tiles * kv->kv_heads;
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)(PT_IDS - 2) * P / PT_KEYS));
+  // Blocks per part: waves of one CTA per SM, each block about 1.3 us (half
+  // of that where the streams share the blocks), three blocks' worth of
+  // set-up, and the join's traffic of every part.
+  double best = 1e30;
+  const double join = 1e-6 * q->rows * q->heads * hd * 8 / 4.0 * (split ? 2 : 1);  // us a part at 4 TB/s
+  for (int64_t parts = ceil_div(blocks, most); parts <= std::min<int64_t>(blocks, ceil_div(blocks, most) + 64); parts++) {
+    const int64_t per = ceil_div(blocks, parts), real = ceil_div(blocks, per);
+    const double us = (double)ceil_div(units * real, SM_COUNT) * (1.3 * (split ? ceil_div(per, 2) : per) + 4.0) + join * real;
+    if (us < best) {
+      best = us;
+      p->tc_args.per = (int)per;
+      p->tc_parts = (int)real;
+    }
+  }
+  const int sub = hd > 64 ? 2 : 1;
+  p->tc_args.blocks = (int)blocks;
+  p->tc_args.split_keys = split;
+  p->tc_args.stages = sub == 2 ? 2 : 4;
+  p->tc_args.box = std::min(P, PT_KEYS);
+  p->tc_args.hdp = (hd + 15) / 16 * 16;
+  p->prefix_slots = p->tc_parts * (split ? 2 : 1);
+}
+
 AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, int max_length, int budget) {
   AttendPlan p;
   const int G = q->heads / kv->kv_heads, P = kv->page_tokens;
@@ -180,7 +230,8 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
     const int64_t shared = (int64_t)prefix_pages * P;
     p.prefix_rows = rows_per_cta(kv, T * G);
     p.own_rows = rows_per_cta(kv, (int64_t)q->max_fresh * G);
-    if (shared > 0) {
+    plan_tc(kv, q, prefix_pages, &p);
+    if (shared > 0 && !p.tc) {
       p.prefix_chunk = chunk_of(shared, ceil_div(T * G, p.prefix_rows) * kv->kv_heads, P);
       p.prefix_slots = (int)ceil_div(shared, p.prefix_chunk);
     }
@@ -190,7 +241,7 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
   }
   p.slots = std::max(1, p.prefix_slots + p.own_slots);
   size_t off = 0;
-  const size_t rows = p.slots > 1 ? (size_t)T * q->heads : 0;
+  const size_t rows = p.slots > 1 || p.tc ? (size_t)T * q->heads : 0;
   p.part_o = off;
   off += align256(rows * p.slots * kv->head_dim * sizeof(float));
   p.part_ml = off;
@@ -269,11 +320,46 @@ int launch_parts(const AttendArgs& a, int rows, int parts, cudaStream_t s) {
   }
 }
 
+// The cache as a tensor of [features, positions, heads, pages] and 64 x box x 1 x 1 boxes.
+int cache_map(CUtensorMap* map, const AttendArgs& a, void* base, int box, bool is_bf16) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return fail(TCU_ECUDA, "cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[4] = {(cuuint64_t)a.hd, (cuuint64_t)a.kv.P, (cuuint64_t)a.kv.kvh, (cuuint64_t)a.kv.num_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)a.kv.st * 2, (cuuint64_t)a.kv.sh * 2, (cuuint64_t)a.kv.sp * 2};
+  for (int i = 0; i < 3; i++)
+    if (dims[i + 1] == 1 && strides[i] == 0) strides[i] = 16;  // a dimension of one has no step
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = encode(map, is_bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, base, dims, strides, boxes, ones,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(TCU_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return TCU_OK;
+}
+
+template <typename T>
+int launch_prefix_tc(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
+  CUtensorMap km, vm;
+  const bool is_bf16 = std::is_same<T, bf16>::value;
+  TRY(cache_map(&km, a, a.kv.k, p.tc_args.box, is_bf16));
+  TRY(cache_map(&vm, a, a.kv.v, p.tc_args.box, is_bf16));
+  const int sub = a.hd > 64 ? 2 : 1;
+  const size_t smem = pt_smem(sub, p.tc_args.split_keys, p.tc_args.stages);
+  const dim3 grid(p.tc_tiles, a.KVH, p.tc_parts);
+  auto kern = sub == 2 ? k_attend_prefix_tc<T, 2> : k_attend_prefix_tc<T, 1>;
+  TRY(allow_smem(kern, smem));
+  kern<<<grid, PT_THREADS, smem, s>>>(a, p.tc_args, km, vm);
+  return launched("k_attend_prefix_tc");
+}
+
 template <typename TQ, typename TK>
 int launch_attend(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
-  TRY((launch_parts<TQ, TK, SRC_PREFIX>(a, p.prefix_rows, p.prefix_slots, s)));
+  if (p.tc) {
+    if constexpr (std::is_same<TQ, TK>::value && sizeof(TK) == 2) TRY(launch_prefix_tc<TK>(a, p, s));
+  } else {
+    TRY((launch_parts<TQ, TK, SRC_PREFIX>(a, p.prefix_rows, p.prefix_slots, s)));
+  }
   TRY((launch_parts<TQ, TK, SRC_OWN>(a, p.own_rows, p.own_slots, s)));
-  if (p.prefix_slots + p.own_slots == 1) return TCU_OK;  // the only part wrote the output
+  if (!p.tc && p.prefix_slots + p.own_slots == 1) return TCU_OK;  // the only part wrote the output
   k_attend_join<TQ, 0><<<dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s>>>(a);
   return launched("k_attend_join");
 }

@@ -1,0 +1,366 @@
+// Attention of many query rows to the prefix they share (16-bit caches) on
+// the 5th-generation tensor cores.
+//
+// All rows of a step (queries x the G query heads of a KV head) read the same
+// keys, so they fill 128-row tcgen05 tiles, and each 128-position block of
+// keys and values is fetched by TMA once per CTA:
+//   S = Q K^T   M = 128 rows, N = 128 positions, K = head size; Q and K in
+//               shared memory (128-byte swizzle), S in TMEM;
+//   P = 2^(S scale - m)  one thread per row, packed to 16 bits over S's own
+//               TMEM columns;
+//   O += P V    A = P from TMEM, B = V as stored (features contiguous), O in
+//               TMEM.
+// Two streams of this run against each other so that one stream's softmax
+// covers the other's products: two tiles of rows over the same blocks
+// (more than 128 rows) or one tile of rows over alternate blocks, each
+// stream then leaving a partial result of its own. Warps 0-3 and 4-7 are the
+// streams' softmax, warp 8 issues the TMA loads, warp 9 the products.
+//
+// A row's reference m moves only when a block's maximum passes it by more
+// than 2^8 (weights up to 256 fit both types), which spares the
+// multiplication of O in TMEM for almost every block; the sums stay exact in
+// float32 since the same m enters numerator and denominator. A stream's
+// product S(i + 1) overwrites the columns of P(i): the tensor core runs a
+// CTA's products in the order they are issued, P(i) V before S(i + 1).
+//
+// Copies read this GPU's own memory into this CTA's shared memory; page ids
+// that name no page become a coordinate behind the last page, which TMA fills
+// with zeros, and their positions are masked. Every wait is bounded; one that
+// runs out ends the CTA with NaN results.
+#pragma once
+#include <cuda.h>
+
+#include "paged.cuh"
+#include "paged_mma.cuh"
+#include "tcgen05.cuh"
+
+namespace tcu {
+
+constexpr int PT_ROWS = 128, PT_KEYS = 128;
+constexpr int PT_THREADS = 320;
+constexpr int PT_IDS = 1024;      // page ids of a part
+constexpr int PT_SUB = 16384;     // bytes of 128 rows of 64 values
+constexpr int PT_MAX_STAGES = 4;
+
+struct PagedTcArgs {
+  int per;         // blocks of a part
+  int blocks;      // blocks of the prefix
+  int split_keys;  // 1: both streams have the same rows and take alternate blocks
+  int stages;      // of the K ring, and of the V ring
+  int box;         // rows of one TMA box: min(page, 128)
+  int hdp;         // head size rounded up to 16
+};
+
+struct PtShared {
+  uint64_t k_full[PT_MAX_STAGES], k_empty[PT_MAX_STAGES], v_full[PT_MAX_STAGES], v_empty[PT_MAX_STAGES];
+  uint64_t s_full[2], p_full[2], o_done[2];
+  uint32_t tmem;
+  int err, bad;
+  int row[2 * PT_ROWS], limit[2 * PT_ROWS];
+  int ids[PT_IDS];
+};
+
+__host__ __device__ constexpr size_t pt_smem(int sub, int split_keys, int stages) {
+  return (size_t)sub * PT_SUB * ((split_keys ? 1 : 2) + 2 * stages) + 1024 + sizeof(PtShared);
+}
+
+// One box of a [features, positions, heads, pages] tensor.
+__device__ __forceinline__ void pt_load(void* dst, const CUtensorMap* map, int x, int row, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(row), "r"(head), "r"(page), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// After a failed wait: the phase's copies or products must have landed
+// before the CTA leaves (bounded as well).
+__device__ __forceinline__ void pt_drain(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = global_ns();
+  while (!mbar_try_wait(bar, parity))
+    if (global_ns() - t0 > TCU_WAIT_NS) return;
+}
+
+template <typename T, int SUB>
+__global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a, PagedTcArgs p, const __grid_constant__ CUtensorMap kmap,
+                                                                     const __grid_constant__ CUtensorMap vmap) {
+  extern __shared__ uint8_t pt_mem[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_mem) + 1023) & ~(uintptr_t)1023);
+  uint8_t* qs = base;
+  uint8_t* ks = qs + (size_t)(p.split_keys ? 1 : 2) * SUB * PT_SUB;
+  uint8_t* vs = ks + (size_t)p.stages * SUB * PT_SUB;
+  PtShared& sh = *reinterpret_cast<PtShared*>(vs + (size_t)p.stages * SUB * PT_SUB);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = blockIdx.y, part = blockIdx.z;
+  const int blk0 = part * p.per, nblk = min(p.per, p.blocks - blk0);
+  const int prefix_end = a.prefix_pages * a.kv.P;
+  const int tiles = p.split_keys ? 1 : 2;
+
+  // The rows, the page ids, the barriers.
+  int valid = 0;
+  if (tid < tiles * PT_ROWS) {
+    const int row = blockIdx.x * tiles * PT_ROWS + tid;
+    const Query q = query_of(a, row / a.G);
+    sh.row[tid] = q.token < 0 ? -1 : q.token * a.H + g * a.G + row % a.G;
+    sh.limit[tid] = q.token < 0 ? -1 : q.pos;
+    valid = q.token >= 0;
+  }
+  if (tid == 0) {
+    sh.err = 0;
+    sh.bad = 0;
+  }
+  if (!__syncthreads_or(valid)) return;  // padding rows only
+  {
+    const int first = (int)a.kv.divP.div(blk0 * PT_KEYS);
+    const int last = (int)a.kv.divP.div(min(prefix_end, (blk0 + nblk) * PT_KEYS) - 1);
+    for (int e = tid; e <= last - first; e += PT_THREADS) {
+      int id = a.prefix[first + e];
+      if (id < 0 || id >= a.kv.num_pages) {
+        id = -1;
+        sh.bad = 1;
+      }
+      sh.ids[e] = id;
+    }
+  }
+  if (tid == 0) {
+    for (int i = 0; i < p.stages; i++) {
+      mbar_init(&sh.k_full[i], 1);
+      mbar_init(&sh.k_empty[i], 1);
+      mbar_init(&sh.v_full[i], 1);
+      mbar_init(&sh.v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; t++) {
+      mbar_init(&sh.s_full[t], 1);
+      mbar_init(&sh.p_full[t], 4);
+      mbar_init(&sh.o_done[t], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // Queries, swizzled as the descriptors read them; a negative scale is taken
+  // into their sign, so that the largest score is the largest S.
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+  for (int e = tid; e < tiles * PT_ROWS * SUB * 8; e += PT_THREADS) {
+    const int rr = e / (SUB * 8), ch = e % (SUB * 8), row = sh.row[rr], d = ch * 8;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (row >= 0 && d < a.hd)
+      x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
+    x.x ^= flip;
+    x.y ^= flip;
+    x.z ^= flip;
+    x.w ^= flip;
+    const int t = rr / PT_ROWS, r = rr % PT_ROWS;
+    *reinterpret_cast<uint4*>(qs + (size_t)(t * SUB + (ch >> 3)) * PT_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  // TMEM columns: S (and P) of stream t at t * 128, O of stream t at 256 + t * 128.
+  const int count[2] = {p.split_keys ? (nblk + 1) / 2 : nblk, p.split_keys ? nblk / 2 : nblk};
+
+  if (warp == 8) {
+    if (lane == 0) {
+      const uint32_t bytes = (uint32_t)SUB * PT_SUB;
+      const int boxes = PT_KEYS / p.box;
+      int b = 0;
+      for (; b < nblk; b++) {
+        const int st = b % p.stages, round = b / p.stages;
+        const int key0 = (blk0 + b) * PT_KEYS;
+        bool ok = true;
+#pragma unroll 1
+        for (int kv = 0; kv < 2 && ok; kv++) {
+          uint64_t* full = kv ? &sh.v_full[st] : &sh.k_full[st];
+          if (round > 0) ok = mbar_wait(kv ? &sh.v_empty[st] : &sh.k_empty[st], (round - 1) & 1, &sh.err);
+          if (!ok) break;
+          mbar_expect_tx(full, bytes);
+          uint8_t* dst = (kv ? vs : ks) + (size_t)st * SUB * PT_SUB;
+          for (int x = 0; x < boxes; x++) {
+            const int key = key0 + x * p.box;
+            const int pg = (int)a.kv.divP.div(key), row0 = key - pg * a.kv.P;
+            int id = key < prefix_end ? sh.ids[pg - (int)a.kv.divP.div(blk0 * PT_KEYS)] : -1;
+            if (id < 0) id = a.kv.num_pages;  // behind the pool: zeros
+            for (int s = 0; s < SUB; s++) pt_load(dst + (size_t)s * PT_SUB + x * p.box * 128, kv ? &vmap : &kmap, s * 64, row0, g, id, full);
+          }
+        }
+        if (!ok) break;
+      }
+      if (b < nblk)  // gave up: the copies of the last rounds must have landed
+        for (int i = 0; i < p.stages; i++) {
+          const int last = b - 1 - i;
+          if (last >= 0) {
+            pt_drain(&sh.k_full[last % p.stages], (last / p.stages) & 1);
+            pt_drain(&sh.v_full[last % p.stages], (last / p.stages) & 1);
+          }
+        }
+    }
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint32_t type = sizeof(T) == 2 && __is_same(T, bf16) ? (1u << 7) | (1u << 10) : 0u;
+      const uint32_t id_s = (1u << 4) | type | ((uint32_t)(PT_KEYS >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
+      const uint32_t id_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(p.hdp >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
+      const int ksteps = p.hdp / 16;
+      bool ok = true;
+      auto scores = [&](int t, int i) {
+        const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
+        ok = ok && mbar_wait(&sh.k_full[st], (b / p.stages) & 1, &sh.err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t qb = smem_u32(qs) + (p.split_keys ? 0 : t) * SUB * PT_SUB, kb = smem_u32(ks) + st * SUB * PT_SUB;
+        for (int kk = 0; kk < ksteps; kk++) {
+          const uint32_t off = (kk >> 2) * PT_SUB + (kk & 3) * 32;
+          tc_mma(tmem + t * 128, tc_smem_desc(qb + off), tc_smem_desc(kb + off), id_s, kk > 0 ? 1u : 0u);
+        }
+        tc_commit(&sh.s_full[t]);
+        if (p.split_keys || t == 1) tc_commit(&sh.k_empty[st]);
+      };
+      auto values = [&](int t, int i) {
+        const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
+        ok = ok && mbar_wait(&sh.v_full[st], (b / p.stages) & 1, &sh.err);
+        ok = ok && mbar_wait(&sh.p_full[t], i & 1, &sh.err);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t vb = smem_u32(vs) + st * SUB * PT_SUB;
+        for (int kk = 0; kk < PT_KEYS / 16; kk++)
+          tc_mma_ta(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, tc_smem_desc_mn(vb + kk * 2048, PT_SUB), id_o, i > 0 || kk > 0 ? 1u : 0u);
+        if (p.split_keys || t == 1) tc_commit(&sh.v_empty[st]);
+        if (i == count[t] - 1) tc_commit(&sh.o_done[t]);
+      };
+      for (int t = 0; t < 2; t++)
+        if (count[t] > 0) scores(t, 0);
+      for (int i = 0; i < count[0]; i++)
+        for (int t = 0; t < 2; t++)
+          if (i < count[t]) {
+            values(t, i);
+            if (i + 1 < count[t]) scores(t, i + 1);
+          }
+      if (!ok) {  // products in flight read shared memory: let them finish
+        tc_commit(&sh.o_done[0]);
+        pt_drain(&sh.o_done[0], 0);
+      }
+    }
+  } else {
+    const int t = warp >> 2, r = tid & 127;
+    const int at = p.split_keys ? r : tid;  // this thread's row
+    const int row = sh.row[at], limit = sh.limit[at];
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
+    // Not zero, so that a masked score times it stays -inf.
+    const float scale = fmaxf(fabsf(a.scale), 1.17549435e-38f);
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < count[t]; i++) {
+      const int key0 = (blk0 + (p.split_keys ? 2 * i + t : i)) * PT_KEYS;
+      ok = mbar_wait(&sh.s_full[t], i & 1, &sh.err);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[PT_KEYS];
+#pragma unroll
+      for (int q = 0; q < PT_KEYS / 32; q++) tc_ld32(ts + q * 32, s + q * 32);
+      tc_wait_ld();
+      const int seen = min(limit, prefix_end - 1) - key0;  // columns up to here are this row's
+      if (__any_sync(0xffffffffu, seen < PT_KEYS - 1)) {
+#pragma unroll
+        for (int q = 0; q < PT_KEYS; q++)
+          if (q > seen) s[q] = 0xff800000u;
+      }
+      if (sh.bad) {  // some page of this part is none: a bit per position
+        const int first = (int)a.kv.divP.div(blk0 * PT_KEYS);
+#pragma unroll
+        for (int w = 0; w < PT_KEYS / 32; w++) {
+          const int key = key0 + w * 32 + lane;
+          const uint32_t there = __ballot_sync(0xffffffffu, key < prefix_end && sh.ids[min((int)a.kv.divP.div(key) - first, PT_IDS - 1)] >= 0);
+#pragma unroll
+          for (int q = 0; q < 32; q++)
+            if (!(there >> q & 1)) s[w * 32 + q] = 0xff800000u;
+        }
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < PT_KEYS; q++) mx = fmaxf(mx, __uint_as_float(s[q]));
+      mx *= scale;
+      const bool move = mx > m + 8.f;  // from -inf as well
+      if (__any_sync(0xffffffffu, move)) {
+        const float alpha = move ? (m == -INFINITY ? 0.f : ex2(m - mx)) : 1.f;
+        if (move) m = mx;
+        l *= alpha;
+        if (i > 0) {  // S(i) is complete, so P(i - 1) V is, which was issued before it
+          for (int q = 0; q < p.hdp; q += 16) {
+            uint32_t x[16];
+            asm volatile(
+                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]),
+                  "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+                : "r"(to + q));
+            tc_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(to + q),
+                "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]),
+                "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+                : "memory");
+          }
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int q = 0; q < PT_KEYS; q += 4) {
+        float e[4];
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+          e[z] = ex2(fmaf(__uint_as_float(s[q + z]), scale, -ref));
+          sum[z] += e[z];
+        }
+        s[q / 2] = pack2<T>(e[0], e[1]);
+        s[q / 2 + 1] = pack2<T>(e[2], e[3]);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tc_st32(ts, s);
+      tc_st32(ts + 32, s + 32);
+      tc_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.p_full[t]);
+    }
+    if (ok && count[t] > 0) ok = mbar_wait(&sh.o_done[t], 0, &sh.err);
+    ok = __all_sync(0xffffffffu, ok);
+    tc_fence_after();
+    const int64_t slot = (int64_t)(row < 0 ? 0 : row) * a.slots + (p.split_keys ? 2 * part + t : part);
+    for (int q = 0; q < p.hdp; q += 16) {
+      uint32_t x[16];
+      if (count[t] > 0) {
+        asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+              "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+            : "r"(to + q));
+        tc_wait_ld();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[e] = 0;
+      }
+      if (row >= 0) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          if (q + e < a.hd) *reinterpret_cast<uint4*>(a.part_o + slot * a.hd + q + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+      }
+    }
+    if (row >= 0) a.part_ml[slot] = ok ? make_float2(m, l) : make_float2(NAN, NAN);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+  }
+}
+
+}  // namespace tcu

@@ -38,6 +38,7 @@
 #include "gguf.h"
 #include "kv_snapshot.h"
 #include "status.h"
+#include "tma_host.h"
 
 using namespace tcu;
 
@@ -1354,7 +1355,7 @@ static std::once_flag g_encode_once;
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link
 // against the driver library); nullptr if unavailable.
-static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+PFN_cuTensorMapEncodeTiled_v12000 tcu::tensor_map_encoder() {
   std::call_once(g_encode_once, [] {
     cudaDriverEntryPointQueryResult q;
     void* f = nullptr;
