@@ -244,6 +244,25 @@ def test_append(qt, kt, T, H, KVH, hd, P, norm, pairs, adjacent, order):
     assert torch.equal(k[at // P, :, at % P], k0[at // P, :, at % P]) and torch.equal(v[at // P, :, at % P], v0[at // P, :, at % P])
 
 
+def test_norm_weights_of_a_single_key_head():
+    """Weights per head where one of the two kinds has a single head."""
+    g = gen(8)
+    for H, KVH in ((4, 1), (1, 1)):
+        k, v = make_cache(2, KVH, 8, 64, torch.bfloat16, g)
+        qw, kw = normal((H, 64), g), normal((KVH, 64), g)
+        x = normal((5, (H + 2 * KVH) * 64), g, torch.bfloat16)
+        slots = torch.arange(5, device=DEV) + 3
+        c = paged.Cache(k, v)
+        q = c.append(x, H, i32([0] * 5), slots, norm=paged.HeadNorm("layer", qw, kw, 1e-5))
+        qr, kr, _ = append_ref(x.reshape(5, -1, 64), H, KVH, "layer", 1e-5, qw, kw, None, None, False)
+        for got, want in ((q, qr), (k[slots // 8, :, slots % 8], kr)):
+            near(got, want, 64 * 2.0 ** -24 * want.abs().amax(-1, keepdim=True) + 2.0 ** -8 * want.abs())
+    with pytest.raises(BackendError):  # one row for several heads beside rows per head
+        k, v = make_cache(2, 2, 8, 64, torch.bfloat16, g)
+        paged.Cache(k, v).append(normal((5, 8 * 64), g, torch.bfloat16), 4, i32([0] * 5), slots,
+                                 norm=paged.HeadNorm("layer", normal((1, 64), g), normal((2, 64), g), 1e-5))
+
+
 def test_append_keeps_values_it_only_moves():
     """Without norm and rotation keys, values and queries are copies: infinities, NaN and the type's extremes among them."""
     g = gen(5)

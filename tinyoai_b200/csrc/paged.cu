@@ -123,22 +123,44 @@ int launched(const char* name) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+constexpr int SM_COUNT = 148;  // B200
+
 // ---------------------------------------------------------------------------
 // Append
 
 template <typename TQ, typename TK>
 void launch_append(const AppendArgs& a, cudaStream_t s) {
-  const int chunks = (a.hd + 3) / 4;
-  const int64_t items = (int64_t)a.T * (a.H + 2 * a.KVH);
-  auto go = [&](auto kern, int lph) { kern<<<(unsigned)ceil_div(items, APPEND_THREADS / lph), APPEND_THREADS, 0, s>>>(a); };
-  if (chunks <= 8)
-    go(k_append<TQ, TK, 8, 1>, 8);
-  else if (chunks <= 16)
-    go(k_append<TQ, TK, 16, 1>, 16);
-  else if (chunks <= 32)
-    go(k_append<TQ, TK, 32, 1>, 32);
+  const int heads = a.H + 2 * a.KVH;
+  auto go = [&](auto kern, int lph) {
+    // A CTA takes all heads of a token when there are tokens enough to fill
+    // the GPU twice over, otherwise as many as its groups of lanes hold at once.
+    const int groups = APPEND_THREADS / lph;
+    const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(ceil_div(heads, groups), ceil_div(8 * SM_COUNT, a.T)));
+    const int per = (int)(ceil_div(ceil_div(heads, shares), groups) * groups);
+    kern<<<dim3((unsigned)a.T, (unsigned)ceil_div(heads, per)), APPEND_THREADS, 0, s>>>(a, per);
+  };
+  auto pick = [&](auto turn) {
+    constexpr int TURN = decltype(turn)::value;
+    if (a.hd <= 64)
+      go(k_append<TQ, TK, 8, TURN>, 8);
+    else if (a.hd <= 128)
+      go(k_append<TQ, TK, 16, TURN>, 16);
+    else
+      go(k_append<TQ, TK, 32, TURN>, 32);
+  };
+  if (a.pairs == 0)
+    pick(std::integral_constant<int, TURN_NONE>());
+  else if (a.adjacent)
+    pick(std::integral_constant<int, TURN_OWN>());
+  else if (a.pairs % 8 == 0)
+    pick(std::integral_constant<int, TURN_LANES>());
   else
-    go(k_append<TQ, TK, 32, 2>, 32);
+    pick(std::integral_constant<int, TURN_SHARED>());
+}
+
+template <typename TK>
+void launch_means(const MeansArgs& a, cudaStream_t s) {
+  k_page_means<TK><<<dim3((unsigned)ceil_div(a.T, 128), a.kv.kvh), 128, 0, s>>>(a);
 }
 
 // ---------------------------------------------------------------------------
@@ -149,10 +171,9 @@ struct AttendPlan {
   bool tc = false;  // the prefix on tcgen05
   PagedTcArgs tc_args{};
   int tc_tiles = 0, tc_parts = 0;
-  size_t part_o = 0, part_ml = 0, keys = 0, bytes = 0;  // offsets of the workspace regions, and their size
+  size_t part_o = 0, part_ml = 0, keys = 0, scores = 0, eps = 0, bytes = 0;  // offsets of the workspace regions, and their size
 };
 
-constexpr int SM_COUNT = 148;  // B200
 
 // Positions per part: enough CTAs for four on each SM, but parts of at least
 // 128 positions, whose own cost (its queries, its partial) a shorter one
@@ -248,7 +269,12 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
   off += align256(rows * p.slots * sizeof(float2));
   if (budget > 0) {
     p.keys = off;
-    off += align256((size_t)T * kv->kv_heads * q->table_width * sizeof(unsigned long long));
+    const size_t lists = (size_t)T * kv->kv_heads;
+    off += align256(lists * q->table_width * sizeof(unsigned long long));
+    p.scores = off;
+    off += align256(lists * q->table_width * sizeof(float));
+    p.eps = off;
+    off += align256(lists * ceil_div(q->table_width, SCORE_PAGES) * sizeof(float));
   }
   p.bytes = std::max<size_t>(off, 256);
   return p;
@@ -367,13 +393,23 @@ int launch_attend(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
 template <typename TQ, typename TK>
 int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p, cudaStream_t s) {
   const unsigned queries = (unsigned)((int64_t)a.n * a.max_fresh);
-  if (c.top > 0 && c.width > 0) {
-    const size_t smem = sizeof(double) * a.G * a.hd;
-    TRY(allow_smem(k_page_scores<TQ, TK>, smem));
-    k_page_scores<TQ, TK><<<dim3(queries, a.KVH, (unsigned)ceil_div(c.width, 64)), 128, smem, s>>>(a, c);
+  // No query has more than width pages: with room for all, none is scored.
+  if (c.top > 0 && c.width - c.first - c.last > c.top) {
+    const dim3 grid(queries, a.KVH, c.tiles);
+    if constexpr (sizeof(TK) == 4) {
+      const size_t smem = sizeof(float) * a.G * a.hd;
+      TRY(allow_smem(k_page_scores_cc<TQ, TK>, smem));
+      k_page_scores_cc<TQ, TK><<<grid, 128, smem, s>>>(a, c);
+    } else {
+      const int hd = a.hd <= 64 ? 64 : a.hd <= 96 ? 96 : a.hd <= 128 ? 128 : 256;
+      auto kern = hd == 64 ? k_page_scores_mma<TQ, TK, 64> : hd == 96 ? k_page_scores_mma<TQ, TK, 96> : hd == 128 ? k_page_scores_mma<TQ, TK, 128> : k_page_scores_mma<TQ, TK, 256>;
+      const size_t smem = (size_t)(sizeof(TQ) == 4 ? 2 : 1) * ((a.G + 7) / 8 * 8) * (hd + 32) * 2;
+      TRY(allow_smem(kern, smem));
+      kern<<<grid, MM_WARPS * 32, smem, s>>>(a, c);
+    }
     TRY(launched("k_page_scores"));
   }
-  k_page_choose<<<dim3(queries, a.KVH), CHOOSE_THREADS, 0, s>>>(a, c);
+  k_page_choose<TQ, TK><<<dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s>>>(a, c);
   TRY(launched("k_page_choose"));
   TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
   if (p.own_slots == 1) return TCU_OK;  // the only part wrote the output
@@ -515,7 +551,10 @@ int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, 
   a.counts = counts;
   a.divP = FastDiv::of((uint32_t)page_tokens);
   const unsigned grid = (unsigned)std::max<int64_t>(1, ceil_div(capacity, PLAN_TILE));
-  k_plan_step<<<grid, PLAN_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  if (n <= 256)
+    k_plan_step<256><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  else
+    k_plan_step<1024><<<grid, 1024, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launched("k_plan_step");
 }
 
@@ -604,14 +643,13 @@ int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_
   a.slots = slots;
   a.means = means;
   a.kv = view_of(kv);
-  const dim3 grid((unsigned)ceil_div(rows, 128), kv->kv_heads);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (kv->dtype == TCU_F32)
-    k_page_means<float><<<grid, 128, 0, s>>>(a);
+    launch_means<float>(a, s);
   else if (kv->dtype == TCU_F16)
-    k_page_means<__half><<<grid, 128, 0, s>>>(a);
+    launch_means<__half>(a, s);
   else
-    k_page_means<bf16><<<grid, 128, 0, s>>>(a);
+    launch_means<bf16>(a, s);
   return launched("k_page_means");
 }
 
@@ -681,7 +719,10 @@ int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv
   c.top = top;
   c.means = means;
   c.keys = reinterpret_cast<unsigned long long*>(static_cast<uint8_t*>(workspace) + p.keys);
+  c.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.scores);
+  c.eps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.eps);
   c.width = q->table_width;
+  c.tiles = (int)ceil_div(q->table_width, SCORE_PAGES);
   c.pages = pages;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (q->dtype == TCU_F32 && kv->dtype == TCU_F32) return launch_sparse<float, float>(a, c, p, s);

@@ -61,6 +61,28 @@ __device__ __forceinline__ float4 load4(const bf16* p) {
   return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
 }
 
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = load4(p), b = load4(p + 4);
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void unpack2(__half, uint32_t r, float& lo, float& hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+  lo = f.x;
+  hi = f.y;
+}
+__device__ __forceinline__ void unpack2(bf16, uint32_t r, float& lo, float& hi) {
+  lo = __uint_as_float(r << 16);
+  hi = __uint_as_float(r & 0xffff0000u);
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
+  const uint4 r = *reinterpret_cast<const uint4*>(p);
+  unpack2(T(), r.x, x[0], x[1]);
+  unpack2(T(), r.y, x[2], x[3]);
+  unpack2(T(), r.z, x[4], x[5]);
+  unpack2(T(), r.w, x[6], x[7]);
+}
+
 // One rounding (to nearest even) to the stored type.
 __device__ __forceinline__ void store_as(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
@@ -73,6 +95,26 @@ __device__ __forceinline__ void store4(__half* p, float4 v) {
 __device__ __forceinline__ void store4(bf16* p, float4 v) {
   const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
   *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  store4(p, make_float4(x[0], x[1], x[2], x[3]));
+  store4(p + 4, make_float4(x[4], x[5], x[6], x[7]));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
 }
 
 // ---------------------------------------------------------------------------
@@ -100,13 +142,15 @@ struct PlanArgs {
   FastDiv divP;
 };
 
-constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_TILE = 1024;  // tokens a CTA fills
 
 struct PlanSum {
   long long tok, pg;
 };
 
+// PLAN_THREADS: 256, or 1024 so that up to 1,024 requests are one tile (a
+// tile's chain of loads, barriers and searches takes about 3 us).
+template <int PLAN_THREADS>
 __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
   __shared__ PlanSum wsum[PLAN_THREADS / 32];
   __shared__ int s_start[PLAN_THREADS + 1], s_page[PLAN_THREADS], s_held[PLAN_THREADS];
@@ -228,9 +272,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
 //          a' = a c - b s, b' = b c + a s
 //   split halves: a = y[i], b = y[i + pairs]; adjacent: a = y[2i], b = y[2i + 1].
 //
-// Float32 throughout, rounded once when stored. LPH lanes share one head of
-// one token, four values a lane and chunk; the partner of a rotary pair comes
-// from shared memory. Bytes bound it: each value is read and written once.
+// Float32 throughout, rounded once when stored. Bytes bound it: each value is
+// read and written once. A CTA takes one token and a share of its heads; LPH
+// lanes hold a head, eight values each, and all heads of a group of lanes
+// that the CTA has (three at a time, two of float32) are loaded before the
+// token's position and slot are known. A lane has the same features of every
+// head, so it keeps their cosines and sines in registers; the partner of a
+// rotary pair comes from another lane (through shared memory where pairs do
+// not fall on whole lanes).
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
 struct AppendArgs {
@@ -252,111 +301,155 @@ struct AppendArgs {
 
 constexpr int APPEND_THREADS = 256;
 
-template <typename TQ, typename TK, int LPH, int CH>
-__global__ void __launch_bounds__(APPEND_THREADS) k_append(AppendArgs a) {
+// Eight stored values, as loaded.
+template <typename T>
+struct Raw8 {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    unpack2(T(), v.x, x[0], x[1]);
+    unpack2(T(), v.y, x[2], x[3]);
+    unpack2(T(), v.z, x[4], x[5]);
+    unpack2(T(), v.w, x[6], x[7]);
+  }
+};
+template <>
+struct Raw8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = load4(p);
+    b = load4(p + 4);
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+  }
+};
+
+// How a rotary pair's other value is found.
+enum { TURN_NONE = 0, TURN_LANES = 1, TURN_OWN = 2, TURN_SHARED = 3 };
+
+// grid: x = token, y = share of the heads (heads_per_cta of them).
+template <typename TQ, typename TK, int LPH, int TURN>
+__global__ void __launch_bounds__(APPEND_THREADS, 4) k_append(AppendArgs a, int heads_per_cta) {
   constexpr int GROUPS = APPEND_THREADS / LPH;
-  __shared__ __align__(16) float stage[GROUPS][LPH * CH * 4 + 4];
+  constexpr int APPEND_HEADS = sizeof(TQ) == 4 ? 2 : 3;  // heads of a group of lanes in flight (64 registers)
+  __shared__ __align__(16) float stage[TURN == TURN_SHARED ? GROUPS : 1][LPH * 8 + 4];
   const int grp = threadIdx.x / LPH, lane = threadIdx.x % LPH;
-  const int heads = a.H + 2 * a.KVH;
-  const int64_t item = (int64_t)blockIdx.x * GROUPS + grp;
-  const int t = (int)(item / heads), h = (int)(item % heads);
-  int pos = -1;
-  int64_t slot = -1;
-  if (t < a.T) {
-    pos = a.positions[t];
-    slot = a.slots[t];
-  }
-  // Padding, and positions or slots outside the table and the pool: nothing is written.
-  const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (a.pairs == 0 || pos < a.max_positions);
-  const bool rot = h < a.H + a.KVH;
-  float x[CH][4];
+  const int t = blockIdx.x, heads = a.H + 2 * a.KVH;
+  const int h0 = blockIdx.y * heads_per_cta, h1 = min(heads, h0 + heads_per_cta);
+  const int d = lane * 8;
+  const bool in = d < a.hd;
+  const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + d;
+  Raw8<TQ> raw[APPEND_HEADS];
+  auto fetch = [&](int hb) {
 #pragma unroll
-  for (int c = 0; c < CH; c++) {
-    const int d = (c * LPH + lane) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (live && d < a.hd) v = load4(reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + (int64_t)h * a.hd + d);
-    x[c][0] = v.x;
-    x[c][1] = v.y;
-    x[c][2] = v.z;
-    x[c][3] = v.w;
-  }
-  if (a.norm != NORM_NONE) {
-    const float inv = 1.f / (float)a.hd;
-    float mean = 0.f;
-    if (a.norm == NORM_LAYER) {
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < CH; c++) s += (x[c][0] + x[c][1]) + (x[c][2] + x[c][3]);
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      mean = s * inv;
+    for (int i = 0; i < APPEND_HEADS; i++) {
+      const int h = hb + i * GROUPS + grp;
+      if (in && h < h1) raw[i].load(src + (int64_t)h * a.hd); else raw[i].zero();
     }
-    float s = 0.f;
+  };
+  fetch(h0);
+  const int pos = a.positions[t];
+  const int64_t slot = a.slots[t];
+  // Padding, and positions or slots outside the table and the pool: nothing is written.
+  const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (TURN == TURN_NONE || pos < a.max_positions);
+  if (!live) return;
+  // x' = x cs + other sn for this lane's features (cs = 1, sn = 0 past the rotary ones).
+  float cs[8], sn[8];
+  if (TURN != TURN_NONE) {
+    const float2* tab = a.table + (int64_t)pos * a.pairs;
 #pragma unroll
-    for (int c = 0; c < CH; c++)
+    for (int e = 0; e < 8; e++) {
+      const int f = d + e;
+      const bool turned = f < 2 * a.pairs, second = TURN == TURN_OWN ? f & 1 : f >= a.pairs;
+      const int i = TURN == TURN_OWN ? f >> 1 : second ? f - a.pairs : f;
+      const float2 v = turned ? tab[i] : make_float2(1.f, 0.f);
+      cs[e] = v.x;
+      sn[e] = second ? v.y : -v.y;
+    }
+  }
+  const int64_t page = slot / a.kv.P, row = slot - page * a.kv.P;
+  const int64_t kv_off = page * a.kv.sp + row * a.kv.st + d;
+  TQ* q_out = reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride + d;
+  const float inv = 1.f / (float)a.hd;
+  // Every group runs as often, so that its warp's shuffles see all lanes.
+  for (int hb = h0; hb < h1; hb += GROUPS * APPEND_HEADS) {
+    if (hb > h0) fetch(hb);
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if ((c * LPH + lane) * 4 + j < a.hd) s = fmaf(x[c][j] - mean, x[c][j] - mean, s);
+    for (int i = 0; i < APPEND_HEADS; i++) {
+      const int h = hb + i * GROUPS + grp;
+      const bool rot = h < a.H + a.KVH;
+      float x[8];
+      raw[i].get(x);
+      if (a.norm != NORM_NONE) {
+        float mean = 0.f;
+        if (a.norm == NORM_LAYER) {
+          float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (rot) {
-      const float r = rsqrtf(fmaf(s, inv, a.eps));
-      const float* w = h < a.H ? a.qw + h * a.w_stride : a.kw + (h - a.H) * a.w_stride;
+          for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          mean = s * inv;
+        }
+        float s = 0.f;
+        if (in)
 #pragma unroll
-      for (int c = 0; c < CH; c++) {
-        const int d = (c * LPH + lane) * 4;
-        if (d < a.hd) {
-          const float4 wv = *reinterpret_cast<const float4*>(w + d);
-          x[c][0] = (x[c][0] - mean) * r * wv.x;
-          x[c][1] = (x[c][1] - mean) * r * wv.y;
-          x[c][2] = (x[c][2] - mean) * r * wv.z;
-          x[c][3] = (x[c][3] - mean) * r * wv.w;
+          for (int e = 0; e < 8; e++) s = fmaf(x[e] - mean, x[e] - mean, s);
+#pragma unroll
+        for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (rot && h < h1 && in) {
+          const float r = rsqrtf(fmaf(s, inv, a.eps));
+          float w[8];
+          load8((h < a.H ? a.qw + h * a.w_stride : a.kw + (h - a.H) * a.w_stride) + d, w);
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = (x[e] - mean) * r * w[e];
         }
       }
-    }
-  }
-  if (a.pairs > 0) {
-    float* st = stage[grp];
+      if (TURN == TURN_OWN) {
+        if (rot)
 #pragma unroll
-    for (int c = 0; c < CH; c++) *reinterpret_cast<float4*>(st + (c * LPH + lane) * 4) = make_float4(x[c][0], x[c][1], x[c][2], x[c][3]);
-    __syncwarp();
-    if (live && rot) {
-      const float2* tab = a.table + (int64_t)pos * a.pairs;
-#pragma unroll
-      for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int d = (c * LPH + lane) * 4 + j;
-          if (d < 2 * a.pairs) {
-            const bool second = a.adjacent ? (d & 1) : d >= a.pairs;
-            const int i = a.adjacent ? d >> 1 : (second ? d - a.pairs : d);
-            const float2 cs = tab[i];
-            const float other = st[a.adjacent ? d ^ 1 : (second ? d - a.pairs : d + a.pairs)];
-            x[c][j] = second ? fmaf(x[c][j], cs.x, other * cs.y) : fmaf(x[c][j], cs.x, -(other * cs.y));
+          for (int e = 0; e < 8; e += 2) {
+            if (d + e >= 2 * a.pairs) continue;
+            const float u = x[e], v = x[e + 1];
+            x[e] = fmaf(u, cs[e], v * sn[e]);
+            x[e + 1] = fmaf(v, cs[e + 1], u * sn[e + 1]);
           }
-        }
-    }
-  }
-  if (!live) return;
-  const int64_t page = slot / a.kv.P, row = slot - page * a.kv.P;
-  const int g = h < a.H + a.KVH ? h - a.H : h - a.H - a.KVH;
-  const int64_t off = page * a.kv.sp + (int64_t)g * a.kv.sh + row * a.kv.st;
+      } else if (TURN == TURN_LANES) {
+        const int step = a.pairs / 8, from = lane < step ? lane + step : lane < 2 * step ? lane - step : lane;
 #pragma unroll
-  for (int c = 0; c < CH; c++) {
-    const int d = (c * LPH + lane) * 4;
-    if (d >= a.hd) continue;
-    const float4 v = make_float4(x[c][0], x[c][1], x[c][2], x[c][3]);
-    if (h < a.H)
-      store4(reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride + (int64_t)h * a.hd + d, v);
-    else
-      store4(reinterpret_cast<TK*>(rot ? a.kv.k : a.kv.v) + off + d, v);
+        for (int e = 0; e < 8; e++) {
+          const float other = __shfl_sync(0xffffffffu, x[e], from, LPH);
+          if (rot && lane < 2 * step) x[e] = fmaf(x[e], cs[e], other * sn[e]);
+        }
+      } else if (TURN == TURN_SHARED) {
+        float* st = stage[grp];
+        __syncwarp();
+        *reinterpret_cast<float4*>(st + d) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(st + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        __syncwarp();
+        if (rot)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int f = d + e;
+            if (f < 2 * a.pairs) x[e] = fmaf(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs] * sn[e]);
+          }
+      }
+      if (h < h1 && in) {
+        if (h < a.H)
+          store8(q_out + (int64_t)h * a.hd, x);
+        else
+          store8(reinterpret_cast<TK*>(rot ? a.kv.k : a.kv.v) + kv_off + (int64_t)(rot ? h - a.H : h - a.H - a.KVH) * a.kv.sh, x);
+      }
+    }
   }
 }
 
 // ---------------------------------------------------------------------------
 // Page means: for every slot that is the last of its page, the mean key of
-// the page for each KV head (float32 sum in position order of each lane's
-// rows, rounded once). One warp takes 32 slots and one KV head.
+// the page for each KV head, float32 sums rounded once. One warp takes 32
+// slots and one KV head. hd / 8 lanes hold a position's features, eight each;
+// as many positions as the warp has lanes for are read side by side, eight
+// loads in flight a lane. The lanes' sums are added in a fixed order.
 struct MeansArgs {
   int T;
   const int64_t* slots;
@@ -366,32 +459,48 @@ struct MeansArgs {
 
 template <typename TK>
 __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
-  const int warp = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int g = blockIdx.y, P = a.kv.P;
+  __shared__ __align__(16) float sums[4][32][8];
+  const int wid = threadIdx.x >> 5, warp = blockIdx.x * 4 + wid, lane = threadIdx.x & 31;
+  const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, rows = 32 / lpr;
   const int64_t t = (int64_t)warp * 32 + lane;
   int64_t slot = t < a.T ? a.slots[t] : -1;
   if (slot >= (int64_t)a.kv.num_pages * P) slot = -1;
-  const int64_t my_page = slot < 0 ? -1 : slot / P;
-  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - my_page * P == P - 1);
+  const int my_page = slot < 0 ? -1 : (int)(slot / P);
+  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - (int64_t)my_page * P == P - 1);
+  const int r0 = lane / lpr, d = (lane - r0 * lpr) * 8;
+  constexpr int U = 8;
   while (todo) {
     const int src = __ffs(todo) - 1;
     todo &= todo - 1;
     const int64_t page = __shfl_sync(0xffffffffu, my_page, src);
-    const TK* base = reinterpret_cast<const TK*>(a.kv.k) + page * a.kv.sp + (int64_t)g * a.kv.sh;
-    TK* out = reinterpret_cast<TK*>(a.means) + (page * a.kv.kvh + g) * a.kv.hd;
-    for (int d0 = 0; d0 < a.kv.hd; d0 += 128) {
-      const int d = d0 + lane * 4;
-      if (d >= a.kv.hd) continue;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < P; r++) {
-        const float4 v = load4(base + (int64_t)r * a.kv.st + d);
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+    const TK* base = reinterpret_cast<const TK*>(a.kv.k) + page * a.kv.sp + (int64_t)g * a.kv.sh + d;
+    float s[8] = {};
+    if (r0 < rows) {
+      for (int r = r0; r < P; r += U * rows) {
+        Raw8<TK> x[U];
+#pragma unroll
+        for (int i = 0; i < U; i++)
+          if (r + i * rows < P) x[i].load(base + (int64_t)(r + i * rows) * a.kv.st); else x[i].zero();
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+          float y[8];
+          x[i].get(y);
+#pragma unroll
+          for (int e = 0; e < 8; e++) s[e] += y[e];
+        }
       }
+    }
+    __syncwarp();
+    store8(&sums[wid][lane][0], s);
+    __syncwarp();
+    if (lane < lpr) {
+      for (int i = 1; i < rows; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) s[e] += sums[wid][lane + i * lpr][e];
       const float n = (float)P;
-      store4(out + d, make_float4(s.x / n, s.y / n, s.z / n, s.w / n));
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[e] = s[e] / n;
+      store8(reinterpret_cast<TK*>(a.means) + (page * a.kv.kvh + g) * a.kv.hd + d, s);
     }
   }
 }
@@ -703,9 +812,8 @@ __device__ __forceinline__ int own_parts(const AttendArgs& a, int pos) {
 }
 
 // Adds up the parts of one row (warp per row): out = sum_j w_j o_j / sum_j w_j
-// l_j with w_j = 2^(m_j - max m), in part order. grid: x = request * max_fresh
-// + query, y = heads / 4. Positions of one request may use different numbers
-// of parts; the request's largest position decides which were written.
+// l_j with w_j = 2^(m_j - max m), in part order; a part without weight is not
+// read. grid: x = request * max_fresh + query, y = heads / 4.
 template <typename TQ, int LIST>
 __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
   const int i = blockIdx.x / a.max_fresh, j = blockIdx.x % a.max_fresh;
@@ -713,167 +821,356 @@ __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
   if (h >= a.H) return;
   const Query q = query_at(a, i, j);
   if (q.token < 0) return;
-  const int np = a.prefix_slots, no = LIST ? a.slots : own_parts(a, q.pos);
+  const int parts = LIST ? a.slots : a.prefix_slots + own_parts(a, q.pos);
   const int64_t row = (int64_t)q.token * a.H + h;
   const float2* ml = a.part_ml + row * a.slots;
-  const int parts = LIST ? no : np + no;
   float mx = -INFINITY;
   for (int p = lane; p < parts; p += 32) mx = fmaxf(mx, ml[p].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float ref = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f;
-  for (int p = 0; p < parts; p++) l = fmaf(ml[p].y, ex2(ml[p].x - ref), l);
-  const float inv = inverse_sum(l);
-  TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)q.token * a.o_ts + (int64_t)h * a.o_hs;
   const float* po = a.part_o + row * a.slots * a.hd;
-  for (int d = lane; d < a.hd; d += 32) {
-    float s = 0.f;
-    for (int p = 0; p < parts; p++) s = fmaf(po[(int64_t)p * a.hd + d], ex2(ml[p].x - ref), s);
-    store_as(out + d, s * inv);
+  TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)q.token * a.o_ts + (int64_t)h * a.o_hs;
+  for (int d0 = 0; d0 < a.hd; d0 += 128) {
+    const int d = d0 + lane * 4;
+    float l = 0.f;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < parts; p0 += 32) {
+      const float2 mine = p0 + lane < parts ? ml[p0 + lane] : make_float2(-INFINITY, 0.f);
+      const float w = ex2(mine.x - ref);
+      const int n = min(32, parts - p0);
+      for (int p1 = 0; p1 < n; p1 += 8) {
+        float wp[8];
+        float4 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          wp[e] = __shfl_sync(0xffffffffu, w, (p1 + e) & 31);
+          l = fmaf(__shfl_sync(0xffffffffu, mine.y, (p1 + e) & 31), wp[e], l);
+          if (p1 + e >= n) wp[e] = 0.f;
+          x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (wp[e] != 0.f && d < a.hd) x[e] = *reinterpret_cast<const float4*>(po + (int64_t)(p0 + p1 + e) * a.hd + d);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          s.x = fmaf(x[e].x, wp[e], s.x);
+          s.y = fmaf(x[e].y, wp[e], s.y);
+          s.z = fmaf(x[e].z, wp[e], s.z);
+          s.w = fmaf(x[e].w, wp[e], s.w);
+        }
+      }
+    }
+    const float inv = inverse_sum(l);
+    if (d < a.hd) store4(out + d, make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv));
   }
 }
 
 // ---------------------------------------------------------------------------
 // Page choice of sparse attention.
 //
-// score(b) = max over the KV head's query heads h of q_h . mean_b, in float64:
+// score(b) = max over the KV head's query heads h of q_h . mean_b, of which
+// the order is wanted in float64. The scores are first taken in float32 with
+// a bound on their error, eps = c sum_d |q_d| |mean_d| (the largest over
+// heads and pages; c counts every rounding of the products and sums). With s
+// the top-th largest float32 score, pages above s + 2 eps are certainly among
+// the best and pages below s - 2 eps certainly not; only those between, seldom
+// more than the page at the border itself, are scored again in float64, where
 // products of the stored types are exact and the sum is good to 2^-52 of its
-// terms, so the order of pages does not depend on how the sum was taken.
-// Candidates: first <= b < npages - last; a key orders them (NaN lowest).
+// terms. A bound that is not finite (infinite or NaN means) sends every page
+// to float64.
 struct ChooseArgs {
   int first, last, top;
-  const void* means;       // [num_pages][KVH][hd]
-  unsigned long long* keys;  // [T][KVH][width]
-  int width;
-  int* pages;              // [T][KVH][budget]
+  const void* means;         // [num_pages][KVH][hd]
+  float* scores;             // [T][KVH][width]; NaN: no page, or a NaN score
+  float* eps;                // [T][KVH][tiles]
+  unsigned long long* keys;  // [T][KVH][width], of the pages scored again
+  int width, tiles;
+  int* pages;                // [T][KVH][budget]
 };
 
-__device__ __forceinline__ unsigned long long score_key(double s) {
-  if (!(s == s)) return 1ull;
-  s += 0.0;  // -0 and +0 are one value
-  const unsigned long long u = (unsigned long long)__double_as_longlong(s);
-  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+constexpr int SCORE_PAGES = 128;  // pages of a scoring CTA
+
+// c above: (2 hd + 32) steps of 2^-23 cover hd products and additions (the
+// tensor core's may truncate) and the 22-bit split of float32 queries.
+__host__ __device__ inline float score_slack(int hd) { return (float)(2 * hd + 32) * 1.1920929e-7f; }
+
+// Candidate pages [lo, hi) of a query.
+struct Candidates {
+  int npages, lo, hi;
+};
+__device__ __forceinline__ Candidates candidates_of(const AttendArgs& a, const ChooseArgs& c, int pos) {
+  Candidates x;
+  x.npages = pos < 0 ? 0 : min((int)a.kv.divP.div(pos) + 1, c.width);
+  x.lo = min(c.first, x.npages);
+  x.hi = max(x.lo, x.npages - c.last);
+  return x;
 }
 
-// grid: x = request * max_fresh + query, y = KV head, z = 64-page tile; eight
-// lanes a page.
+// Float32 scores on CUDA cores (float32 caches), eight lanes a page.
+// grid: x = request * max_fresh + query, y = KV head, z = page tile.
 template <typename TQ, typename TK>
-__global__ void __launch_bounds__(128) k_page_scores(AttendArgs a, ChooseArgs c) {
-  extern __shared__ double qs[];  // [G][hd]
+__global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs c) {
+  extern __shared__ __align__(16) float cq[];  // [G][hd]
+  __shared__ float s_eps[4];
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
-  if (q.token < 0 || q.pos < 0) return;
+  if (q.token < 0) return;
   const int g = blockIdx.y, hd = a.hd;
-  const int npages = q.pos / a.kv.P + 1;
-  const int lo = max(c.first, (int)blockIdx.z * 64), hi = min(min(npages - c.last, c.width), (int)blockIdx.z * 64 + 64);
-  if (lo >= hi) return;
-  for (int e = threadIdx.x; e < a.G * hd; e += 128) {
-    const int h = e / hd, d = e % hd;
-    qs[e] = (double)(float)(reinterpret_cast<const TQ*>(a.q)[(int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs + d]);
+  const Candidates cand = candidates_of(a, c, q.pos);
+  const int lo = max(cand.lo, (int)blockIdx.z * SCORE_PAGES), hi = min(cand.hi, (int)blockIdx.z * SCORE_PAGES + SCORE_PAGES);
+  if (lo >= hi || cand.hi - cand.lo <= c.top) return;  // nothing to choose here
+  for (int e = threadIdx.x * 4; e < a.G * hd; e += 128 * 4) {
+    const int h = e / hd, d = e - h * hd;
+    *reinterpret_cast<float4*>(cq + e) = load4(reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs + d);
   }
   __syncthreads();
   const int* table = a.tables + (int64_t)q.request * a.table_stride;
   const int l8 = threadIdx.x & 7;
-  for (int b0 = blockIdx.z * 64; b0 < (int)blockIdx.z * 64 + 64; b0 += 16) {
+  float most = 0.f;
+  for (int b0 = blockIdx.z * SCORE_PAGES; b0 < hi; b0 += 16) {
     const int b = b0 + (threadIdx.x >> 3);
     const int id = b >= lo && b < hi ? table[b] : -1;
     const bool on = id >= 0 && id < a.kv.num_pages;
     const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)(on ? id : 0) * a.KVH + g) * hd;
-    double best = 0.0;
+    float best = -INFINITY;
+    bool nan = false;
     for (int h = 0; h < a.G; h++) {
-      double s = 0.0;
+      float s = 0.f, z = 0.f;
       for (int d = l8 * 4; d < hd; d += 32) {
         const float4 v = on ? load4(mp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const double* x = qs + h * hd + d;
-        s = fma(x[0], (double)v.x, s);
-        s = fma(x[1], (double)v.y, s);
-        s = fma(x[2], (double)v.z, s);
-        s = fma(x[3], (double)v.w, s);
+        const float4 x = *reinterpret_cast<const float4*>(cq + h * hd + d);
+        s = fmaf(x.x, v.x, fmaf(x.y, v.y, fmaf(x.z, v.z, fmaf(x.w, v.w, s))));
+        z = fmaf(fabsf(x.x), fabsf(v.x), fmaf(fabsf(x.y), fabsf(v.y), fmaf(fabsf(x.z), fabsf(v.z), fmaf(fabsf(x.w), fabsf(v.w), z))));
       }
-      s += __shfl_xor_sync(0xffffffffu, s, 4);
-      s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s += __shfl_xor_sync(0xffffffffu, s, 1);
-      // The largest of the heads; a NaN makes the page NaN.
-      best = h == 0 || s > best || !(s == s) ? (h > 0 && !(best == best) ? best : s) : best;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        s += __shfl_xor_sync(0xffffffffu, s, o);
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+      }
+      nan |= !(s == s);
+      best = fmaxf(best, s);
+      most = z > most || !(z == z) ? z : most;
     }
-    if (l8 == 0 && b >= lo && b < hi) c.keys[((int64_t)q.token * a.KVH + g) * c.width + b] = on ? score_key(best) : 0ull;
+    if (l8 == 0 && b >= lo && b < hi) c.scores[((int64_t)q.token * a.KVH + g) * c.width + b] = on && !nan ? best : NAN;
+  }
+  // NaN outlives the maximum: it has the largest bits of the positive floats.
+  const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+  if ((threadIdx.x & 31) == 0) s_eps[threadIdx.x >> 5] = __uint_as_float(w);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t x = 0;
+    for (int i = 0; i < 4; i++) x = max(x, __float_as_uint(s_eps[i]));
+    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = __uint_as_float(x) * score_slack(hd);
   }
 }
 
-// One CTA per (query, KV head): the key of the top-th candidate by radix
-// selection (eight bits a pass, histograms in shared memory), then the chosen
-// pages in ascending order; candidates equal to that key are taken from the
-// lowest page on. grid: x = request * max_fresh + query, y = KV head.
-constexpr int CHOOSE_THREADS = 256;
+// Order-preserving keys; NaN is 1, below every number, and no page 0.
+__device__ __forceinline__ uint32_t score_key32(float s) {
+  if (!(s == s)) return 1u;
+  return float_order_key(s + 0.f);  // -0 and +0 are one value
+}
+__device__ __forceinline__ unsigned long long score_key(double s) {
+  if (!(s == s)) return 1ull;
+  s += 0.0;
+  const unsigned long long u = (unsigned long long)__double_as_longlong(s);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
 
+constexpr int CHOOSE_THREADS = 256;
+constexpr int CHOOSE_CACHE = 8192;  // scores a CTA keeps in shared memory; others are read again from L2
+
+// The digit d whose bins above it hold fewer than `want` entries and with it
+// at least `want`, from a histogram of 256 bins (one per thread), and how many
+// are still wanted within it. Every thread returns the same.
+__device__ __forceinline__ void pick_digit(int count, int want, int* warp_sums, int* result, int& digit, int& left) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // Sums of the bins from this one up.
+  int up = count;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_down_sync(0xffffffffu, up, o);
+    if (lane + o < 32) up += x;
+  }
+  if (lane == 0) warp_sums[warp] = up;
+  __syncthreads();
+  for (int w = warp + 1; w < 8; w++) up += warp_sums[w];
+  if (up >= want && up - count < want) {  // one thread
+    result[0] = tid;
+    result[1] = want - (up - count);
+  }
+  __syncthreads();
+  digit = result[0];
+  left = result[1];
+}
+
+// One CTA per (query, KV head): the top-th key by radix selection, then the
+// chosen pages in ascending order. grid: x = request * max_fresh + query, y = KV head.
+template <typename TQ, typename TK>
 __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, ChooseArgs c) {
   __shared__ int hist[256];
-  __shared__ int wsum[CHOOSE_THREADS / 32], wtie[CHOOSE_THREADS / 32];
-  __shared__ unsigned long long s_prefix;
-  __shared__ int s_want;
+  __shared__ int sums[CHOOSE_THREADS / 32], result[2], ties_of[CHOOSE_THREADS / 32];
+  __shared__ int s_sure, s_open;
+  __shared__ uint32_t s_eps;
+  extern __shared__ float cache[];  // min(width, CHOOSE_CACHE)
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
   if (q.token < 0) return;
   const int g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int* out = c.pages + ((int64_t)q.token * a.KVH + g) * a.budget;
-  const int npages = q.pos < 0 ? 0 : min(q.pos / a.kv.P + 1, c.width);
-  const int lo = min(c.first, npages), hi = max(lo, npages - c.last);
-  const unsigned long long* keys = c.keys + ((int64_t)q.token * a.KVH + g) * c.width;
-  unsigned long long thr = 0;  // every candidate with a larger key is taken
-  int ties = 0;                // and this many with this key
-  if (hi - lo <= c.top) {
-    ties = hi - lo;  // all: the keys do not matter
-  } else if (c.top > 0) {
-    unsigned long long prefix = 0;
+  const int64_t at = (int64_t)q.token * a.KVH + g;
+  int* out = c.pages + at * a.budget;
+  const Candidates cand = candidates_of(a, c, q.pos);
+  const int npages = cand.npages, lo = cand.lo, hi = cand.hi;
+  const bool all = hi - lo <= c.top, choose = !all && c.top > 0;
+  const float* scores = c.scores + at * c.width;
+  unsigned long long* keys = c.keys + at * c.width;
+  const int kept = min(hi, min(c.width, CHOOSE_CACHE));
+  auto score = [&](int b) { return b < kept ? cache[b] : scores[b]; };
+  float in_above = INFINITY, out_below = INFINITY;  // certain: score > in_above; not certain: >= out_below (and NaN, when eps is not finite)
+  bool every = false;                               // all candidates are open
+  unsigned long long thr = 0;                       // open pages with a larger key are taken,
+  int ties = 0;                                     // and this many with this one
+  if (choose) {
+    if (tid == 0) {
+      s_eps = 0;
+      s_sure = s_open = 0;
+    }
+    for (int b = lo + tid; b < kept; b += CHOOSE_THREADS) cache[b] = scores[b];
+    __syncthreads();
+    uint32_t e = 0;
+    for (int i = lo / SCORE_PAGES + tid; i <= (hi - 1) / SCORE_PAGES; i += CHOOSE_THREADS) e = max(e, __float_as_uint(c.eps[at * c.tiles + i]) & 0x7fffffffu);
+    e = __reduce_max_sync(0xffffffffu, e);
+    if (lane == 0 && e) atomicMax(&s_eps, e);
+    // The top-th largest float32 score.
+    uint32_t prefix = 0;
     int want = c.top;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      for (int e = tid; e < 256; e += CHOOSE_THREADS) hist[e] = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      hist[tid] = 0;
       __syncthreads();
       for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
-        const unsigned long long k = keys[b];
-        if (shift == 56 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        const uint32_t k = score_key32(score(b));
+        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
       }
       __syncthreads();
-      if (tid == 0) {
-        int d = 255, left = want;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        s_prefix = prefix | ((unsigned long long)d << shift);
-        s_want = left;
-      }
-      __syncthreads();
-      prefix = s_prefix;
-      want = s_want;
+      int digit, left;
+      pick_digit(hist[tid], want, sums, result, digit, left);
+      prefix |= (uint32_t)digit << shift;
+      want = left;
     }
-    thr = prefix;
-    ties = want;
+    const float eps = __uint_as_float(s_eps);
+    const float edge = float_from_order_key(prefix);
+    every = !(eps < INFINITY) || prefix <= 1u || !(fabsf(edge) < INFINITY);
+    if (!every) {
+      // Rounded outwards by the additions' own half steps.
+      const float r = 2.f * eps + 2e-7f * fabsf(edge);
+      in_above = edge + r;
+      out_below = edge - r;
+    }
+    // Pages certainly in, and pages that float64 has to order.
+    int sure = 0, open = 0;
+    for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
+      const float x = score(b);
+      if (!every && x > in_above)
+        sure++;
+      else if (every || x >= out_below)
+        open++;
+    }
+    sure = __reduce_add_sync(0xffffffffu, sure);
+    open = __reduce_add_sync(0xffffffffu, open);
+    if (lane == 0) {
+      atomicAdd(&s_sure, sure);
+      atomicAdd(&s_open, open);
+    }
+    __syncthreads();
+    want = c.top - s_sure;
+    if (s_open == want) {
+      ties = want;
+      thr = ~0ull;  // all open pages: see `taken`
+    } else {
+      // Float64 keys of the open pages, a warp each.
+      const int* table = a.tables + (int64_t)q.request * a.table_stride;
+      for (int b0 = lo + warp * 32; b0 < hi; b0 += CHOOSE_THREADS) {
+        const int mine = b0 + lane;
+        const float x = mine < hi ? score(mine) : 0.f;
+        uint32_t todo = __ballot_sync(0xffffffffu, mine < hi && (every || (x <= in_above && x >= out_below)));
+        while (todo) {
+          const int b = b0 + __ffs(todo) - 1;
+          todo &= todo - 1;
+          const int id = table[b];
+          unsigned long long key = 0;
+          if (id >= 0 && id < a.kv.num_pages) {
+            const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)id * a.KVH + g) * a.hd;
+            double best = 0.0;
+            for (int h = 0; h < a.G; h++) {
+              const TQ* qp = reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs;
+              double s = 0.0;
+              for (int d = lane * 4; d < a.hd; d += 128) {
+                const float4 u = load4(qp + d), v = load4(mp + d);
+                s = fma((double)u.x, (double)v.x, s);
+                s = fma((double)u.y, (double)v.y, s);
+                s = fma((double)u.z, (double)v.z, s);
+                s = fma((double)u.w, (double)v.w, s);
+              }
+#pragma unroll
+              for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+              // The largest of the heads; a NaN makes the page NaN.
+              if (h == 0 || (best == best && (s > best || !(s == s)))) best = s;
+            }
+            key = score_key(best);
+          }
+          if (lane == 0) keys[b] = key;
+        }
+      }
+      __syncthreads();
+      for (int shift = 56; shift >= 0; shift -= 8) {
+        hist[tid] = 0;
+        __syncthreads();
+        for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
+          const float x = score(b);
+          if (!(every || (x <= in_above && x >= out_below))) continue;
+          const unsigned long long k = keys[b];
+          if (shift == 56 || (k >> (shift + 8)) == (thr >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        }
+        __syncthreads();
+        int digit, left;
+        pick_digit(hist[tid], want, sums, result, digit, left);
+        thr |= (unsigned long long)digit << shift;
+        want = left;
+      }
+      ties = want;
+    }
   }
-  const bool all = hi - lo <= c.top;
+  const bool keyed = choose && thr != ~0ull;
   int done = 0, tied = 0;  // pages written, ties seen
   for (int b0 = 0; b0 < npages; b0 += CHOOSE_THREADS) {
     const int b = b0 + tid;
     const bool inside = b >= lo && b < hi;
-    const unsigned long long k = inside && !all ? keys[b] : 0;
-    const bool tie = inside && !all && c.top > 0 && k == thr;
-    const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) wtie[warp] = __popc(tb);
-    __syncthreads();
-    int before = tied + __popc(tb & ((1u << lane) - 1));
-    int tie_total = 0;
-    for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-      if (w < warp) before += wtie[w];
-      tie_total += wtie[w];
+    bool take = b < npages && (!inside || all), tie = false;
+    if (inside && choose) {
+      const float x = score(b);
+      const bool open = every || (x <= in_above && x >= out_below);
+      const unsigned long long k = open && keyed ? keys[b] : 0;
+      take = open ? !keyed || k > thr : x > in_above;
+      tie = open && keyed && k == thr;
     }
-    const bool take = b < npages && (!inside || all || (c.top > 0 && k > thr) || (tie && before < ties));
+    int before = tied;
+    if (keyed) {  // ties go to the lower pages
+      const uint32_t tb = __ballot_sync(0xffffffffu, tie);
+      if (lane == 0) ties_of[warp] = __popc(tb);
+      __syncthreads();
+      before += __popc(tb & ((1u << lane) - 1));
+      for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
+        if (w < warp) before += ties_of[w];
+        tied += ties_of[w];
+      }
+    }
+    take = take || (tie && before < ties);
     const uint32_t kb = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) wsum[warp] = __popc(kb);
+    if (lane == 0) sums[warp] = __popc(kb);
     __syncthreads();
-    int at = done + __popc(kb & ((1u << lane) - 1)), total = 0;
+    int to = done + __popc(kb & ((1u << lane) - 1)), total = 0;
     for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-      if (w < warp) at += wsum[w];
-      total += wsum[w];
+      if (w < warp) to += sums[w];
+      total += sums[w];
     }
-    if (take && at < a.budget) out[at] = b;
+    if (take && to < a.budget) out[to] = b;
     done += total;
-    tied += tie_total;
     __syncthreads();
   }
   for (int e = done + tid; e < a.budget; e += CHOOSE_THREADS) out[e] = -1;

@@ -26,6 +26,7 @@
 // A CTA's warps take alternate 16-position tiles of the CTA's part and join
 // their states through shared memory in warp order.
 #pragma once
+#include "../../include/tinyoai_cuda.h"
 #include "paged.cuh"
 
 namespace tcu {
@@ -51,19 +52,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
 constexpr int MM_WARPS = 4;
 constexpr int MM_IDS = 1024;  // page ids of a part, copied to shared memory (a part has at most this many pages)
 
@@ -74,6 +62,55 @@ template <int HD, int NT, int PIECES>
 constexpr size_t mm_smem() {
   const size_t q = (size_t)PIECES * 8 * NT * (HD + 32) * 2, o = (size_t)MM_WARPS * 8 * NT * (HD + 4 + 2) * 4;
   return q > o ? q : o;
+}
+
+// Query rows col -> (token * H + head, -1: none) into shared memory [PIECES][cols][HD + 32],
+// float32 ones as pairs of binary16 values of q * 2^sx. scale[col] = s * 2^-sx.
+template <typename TQ, typename TK, int HD, int PIECES>
+__device__ __forceinline__ void mm_load_queries(const AttendArgs& a, TK* qs, const int* rows, float* scale, int cols, float s) {
+  constexpr int QS = HD + 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.hd;
+  if (PIECES == 1) {
+    constexpr int CH = HD / 8;
+    for (int e = tid; e < cols * CH; e += MM_WARPS * 32) {
+      const int col = e / CH, d = (e % CH) * 8, row = rows[col];
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row >= 0 && d < hd)
+        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const TQ*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
+      *reinterpret_cast<uint4*>(qs + col * QS + d) = x;
+    }
+    for (int col = tid; col < cols; col += MM_WARPS * 32) scale[col] = s;
+  } else {
+    for (int col = warp; col < cols; col += MM_WARPS) {
+      const int row = rows[col];
+      float x[(HD + 31) / 32], mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < (HD + 31) / 32; i++) {
+        const int d = lane + 32 * i;
+        x[i] = row >= 0 && d < hd ? (float)(reinterpret_cast<const TQ*>(a.q)[(int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d]) : 0.f;
+        mx = fmaxf(mx, fabsf(x[i]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // 2^sx brings the largest value into [2^13, 2^14). Infinite or NaN rows stay as they are.
+      int ex = 0;
+      if (mx > 0.f && mx < INFINITY) frexpf(mx, &ex);
+      const int sx = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
+      const float up = __int_as_float((127 + sx) << 23);
+#pragma unroll
+      for (int i = 0; i < (HD + 31) / 32; i++) {
+        const int d = lane + 32 * i;
+        if (d < HD) {
+          const float y = x[i] * up;
+          const __half h = __float2half_rn(y);
+          const float rest = y - __half2float(h);
+          reinterpret_cast<__half*>(qs)[col * QS + d] = h;
+          reinterpret_cast<__half*>(qs)[cols * QS + col * QS + d] = __float2half_rn(rest == rest ? rest : 0.f);
+        }
+      }
+      if (lane == 0) scale[col] = s * __int_as_float((127 - sx) << 23);
+    }
+  }
 }
 
 // grid as k_attend_cc's, with row tiles of 8 * NT rows.
@@ -153,48 +190,7 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
       }
     }
   }
-  // Queries into shared memory; float32 ones as pairs of binary16 values of q * 2^sx.
-  if (PIECES == 1) {
-    constexpr int CH = HD / 8;
-    for (int e = tid; e < COLS * CH; e += MM_WARPS * 32) {
-      const int col = e / CH, d = (e % CH) * 8, row = s_row[col];
-      uint4 x = make_uint4(0, 0, 0, 0);
-      if (row >= 0 && d < hd)
-        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const TQ*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
-      *reinterpret_cast<uint4*>(qs + col * QS + d) = x;
-    }
-    if (tid < COLS) s_scale[tid] = a.scale;
-  } else {
-    for (int col = warp; col < COLS; col += MM_WARPS) {
-      const int row = s_row[col];
-      float x[(HD + 31) / 32], mx = 0.f;
-#pragma unroll
-      for (int i = 0; i < (HD + 31) / 32; i++) {
-        const int d = lane + 32 * i;
-        x[i] = row >= 0 && d < hd ? (float)(reinterpret_cast<const TQ*>(a.q)[(int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d]) : 0.f;
-        mx = fmaxf(mx, fabsf(x[i]));
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      // 2^sx brings the largest value into [2^13, 2^14). Infinite or NaN rows stay as they are.
-      int ex = 0;
-      if (mx > 0.f && mx < INFINITY) frexpf(mx, &ex);
-      const int sx = mx > 0.f && mx < INFINITY ? min(max(14 - ex, -126), 126) : 0;
-      const float up = __int_as_float((127 + sx) << 23);
-#pragma unroll
-      for (int i = 0; i < (HD + 31) / 32; i++) {
-        const int d = lane + 32 * i;
-        if (d < HD) {
-          const float y = x[i] * up;
-          const __half h = __float2half_rn(y);
-          const float rest = y - __half2float(h);
-          reinterpret_cast<__half*>(qs)[col * QS + d] = h;
-          reinterpret_cast<__half*>(qs)[COLS * QS + col * QS + d] = __float2half_rn(rest == rest ? rest : 0.f);
-        }
-      }
-      if (lane == 0) s_scale[col] = a.scale * __int_as_float((127 - sx) << 23);
-    }
-  }
+  mm_load_queries<TQ, TK, HD, PIECES>(a, qs, s_row, s_scale, COLS, a.scale);
   __syncthreads();
   float o[VG][4][NT][4], m[NT][2], l[NT][2], sc[NT][2];
   int lim[NT][2];
@@ -397,6 +393,100 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
       *reinterpret_cast<float4*>(a.part_o + slot * hd + d) = x;
       if (d == 0) a.part_ml[slot] = make_float2(mx, ls);
     }
+  }
+}
+
+// Float32 scores of pages (16-bit caches): the first product of the attention
+// with mean keys in the place of keys, and the same product of magnitudes for
+// the error bound; both cost nothing beside the means' bytes.
+// grid: x = request * max_fresh + query, y = KV head, z = page tile.
+template <typename TQ, typename TK, int HD>
+__global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a, ChooseArgs c) {
+  constexpr int PIECES = sizeof(TQ) == 4 ? 2 : 1;
+  constexpr int KG = (HD + 31) / 32, QS = HD + 32;
+  extern __shared__ __align__(16) uint8_t mm_mem[];  // [PIECES][groups of 8][HD + 32]
+  __shared__ int s_row[TCU_PAGED_MAX_GROUP];
+  __shared__ float s_scale[TCU_PAGED_MAX_GROUP];
+  __shared__ uint32_t s_eps[MM_WARPS];
+  TK* qs = reinterpret_cast<TK*>(mm_mem);
+  const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
+  if (q.token < 0) return;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cc = lane & 3;
+  const int g = blockIdx.y, hd = a.hd, groups = (a.G + 7) / 8;
+  const Candidates cand = candidates_of(a, c, q.pos);
+  const int lo = max(cand.lo, (int)blockIdx.z * SCORE_PAGES), hi = min(cand.hi, (int)blockIdx.z * SCORE_PAGES + SCORE_PAGES);
+  if (lo >= hi || cand.hi - cand.lo <= c.top) return;  // nothing to choose here
+  // The means of this warp's pages, both tiles' loads in flight while the queries come.
+  constexpr int TILES = SCORE_PAGES / (16 * MM_WARPS);
+  uint4 kx[TILES][2][KG];
+  bool on[TILES][2];
+  const int* table = a.tables + (int64_t)q.request * a.table_stride;
+#pragma unroll
+  for (int t = 0; t < TILES; t++)
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int b = blockIdx.z * SCORE_PAGES + (t * MM_WARPS + warp) * 16 + r + 8 * i;
+      const int id = b >= lo && b < hi ? table[b] : -1;
+      on[t][i] = id >= 0 && id < a.kv.num_pages;
+      const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)(on[t][i] ? id : 0) * a.KVH + g) * hd;
+#pragma unroll
+      for (int k = 0; k < KG; k++) {
+        const int d = k * 32 + cc * 8;
+        kx[t][i][k] = on[t][i] && d < hd ? ld_stream16(mp + d) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  if (tid < groups * 8) s_row[tid] = tid < a.G ? q.token * a.H + g * a.G + tid : -1;
+  __syncthreads();
+  mm_load_queries<TQ, TK, HD, PIECES>(a, qs, s_row, s_scale, groups * 8, 1.f);
+  __syncthreads();
+  float most = 0.f;
+#pragma unroll
+  for (int t = 0; t < TILES; t++) {
+    float best[2] = {-INFINITY, -INFINITY};
+    uint32_t nan = 0;
+    for (int n = 0; n < groups; n++) {
+      float s[4] = {}, z[4] = {};
+#pragma unroll
+      for (int k = 0; k < KG; k++)
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+          const uint4 y = *reinterpret_cast<const uint4*>(qs + (p * groups * 8 + n * 8 + r) * QS + k * 32 + cc * 8);
+          const uint4 u = kx[t][0][k], v = kx[t][1][k];
+          constexpr uint32_t M = 0x7fff7fffu;
+          mma16816<TK>(s, u.x, v.x, u.y, v.y, y.x, y.y);
+          mma16816<TK>(s, u.z, v.z, u.w, v.w, y.z, y.w);
+          mma16816<TK>(z, u.x & M, v.x & M, u.y & M, v.y & M, y.x & M, y.y & M);
+          mma16816<TK>(z, u.z & M, v.z & M, u.w & M, v.w & M, y.z & M, y.w & M);
+        }
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int col = n * 8 + 2 * cc + (e & 1);
+        if (col < a.G) {
+          const float x = s[e] * s_scale[col], w = z[e] * s_scale[col];
+          if (!(x == x)) nan |= 1u << (e >> 1);
+          best[e >> 1] = fmaxf(best[e >> 1], x);
+          most = w > most || !(w == w) ? w : most;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
+        nan |= __shfl_xor_sync(0xffffffffu, nan, o);
+      }
+      const int b = blockIdx.z * SCORE_PAGES + (t * MM_WARPS + warp) * 16 + r + 8 * i;
+      if (cc == 0 && b >= lo && b < hi) c.scores[((int64_t)q.token * a.KVH + g) * c.width + b] = on[t][i] && !(nan >> i & 1) ? best[i] : NAN;
+    }
+  }
+  const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
+  if (lane == 0) s_eps[warp] = w;
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t x = 0;
+    for (int i = 0; i < MM_WARPS; i++) x = max(x, s_eps[i]);
+    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = __uint_as_float(x) * score_slack(hd);
   }
 }
 

@@ -80,6 +80,65 @@ __device__ __forceinline__ void pt_drain(uint64_t* bar, uint32_t parity) {
     if (global_ns() - t0 > TCU_WAIT_NS) return;
 }
 
+// a * b + c and a + b on two floats at once.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+
+// Masks 64 scores of positions key0 ..: past column `seen`, and of pages that are none.
+__device__ __noinline__ void pt_mask_bits(const AttendArgs& a, const PtShared& sh, int key0, int seen, int prefix_end, int blk0, uint32_t* bits) {
+  const int lane = threadIdx.x & 31, first = (int)a.kv.divP.div(blk0 * PT_KEYS);
+#pragma unroll
+  for (int w = 0; w < 2; w++) {
+    const int key = key0 + w * 32 + lane;
+    const uint32_t there = __ballot_sync(0xffffffffu, key < prefix_end && sh.ids[min((int)a.kv.divP.div(min(key, prefix_end - 1)) - first, PT_IDS - 1)] >= 0);
+    const int n = min(max(seen + 1 - 32 * w, 0), 32);
+    bits[w] = there & (n == 32 ? 0xffffffffu : (1u << n) - 1);
+  }
+}
+__device__ __forceinline__ void pt_mask(const AttendArgs& a, const PtShared& sh, uint32_t (&s)[PT_KEYS / 2], int key0, int seen, int prefix_end, int blk0) {
+  uint32_t bits[2];
+  pt_mask_bits(a, sh, key0, seen, prefix_end, blk0, bits);
+#pragma unroll
+  for (int q = 0; q < PT_KEYS / 2; q++)
+    if (!(bits[q >> 5] >> (q & 31) & 1)) s[q] = 0xff800000u;
+}
+
+__device__ __forceinline__ void pt_ld16(uint32_t taddr, uint32_t (&x)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+        "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+      : "r"(taddr));
+  tc_wait_ld();
+}
+
+// This lane's first n columns from taddr on, times f.
+__device__ __noinline__ void pt_scale_rows(uint32_t taddr, int n, float f) {
+  for (int q = 0; q < n; q += 16) {
+    uint32_t x[16];
+    pt_ld16(taddr + q, x);
+#pragma unroll
+    for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr + q), "r"(x[0]),
+        "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
+        "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+        : "memory");
+  }
+}
+
 template <typename T, int SUB>
 __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a, PagedTcArgs p, const __grid_constant__ CUtensorMap kmap,
                                                                      const __grid_constant__ CUtensorMap vmap) {
@@ -159,7 +218,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
-  // TMEM columns: S (and P) of stream t at t * 128, O of stream t at 256 + t * 128.
+  // TMEM columns: S of stream t at t * 128, P over its second half, O of stream t at 256 + t * 128.
   const int count[2] = {p.split_keys ? (nblk + 1) / 2 : nblk, p.split_keys ? nblk / 2 : nblk};
 
   if (warp == 8) {
@@ -225,7 +284,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a
         tc_fence_after();
         const uint32_t vb = smem_u32(vs) + st * SUB * PT_SUB;
         for (int kk = 0; kk < PT_KEYS / 16; kk++)
-          tc_mma_ta(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, tc_smem_desc_mn(vb + kk * 2048, PT_SUB), id_o, i > 0 || kk > 0 ? 1u : 0u);
+          tc_mma_ta(tmem + 256 + t * 128, tmem + t * 128 + PT_KEYS / 2 + kk * 8, tc_smem_desc_mn(vb + kk * 2048, PT_SUB), id_o, i > 0 || kk > 0 ? 1u : 0u);
         if (p.split_keys || t == 1) tc_commit(&sh.v_empty[st]);
         if (i == count[t] - 1) tc_commit(&sh.o_done[t]);
       };
@@ -260,71 +319,56 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a
         break;
       }
       tc_fence_after();
-      uint32_t s[PT_KEYS];
-#pragma unroll
-      for (int q = 0; q < PT_KEYS / 32; q++) tc_ld32(ts + q * 32, s + q * 32);
-      tc_wait_ld();
+      // First the row's maximum, 64 columns at a time (all 128 would not stay
+      // in registers); the second half is still there for its weights.
+      constexpr int HALF = PT_KEYS / 2;
+      uint32_t s[HALF];
       const int seen = min(limit, prefix_end - 1) - key0;  // columns up to here are this row's
-      if (__any_sync(0xffffffffu, seen < PT_KEYS - 1)) {
-#pragma unroll
-        for (int q = 0; q < PT_KEYS; q++)
-          if (q > seen) s[q] = 0xff800000u;
-      }
-      if (sh.bad) {  // some page of this part is none: a bit per position
-        const int first = (int)a.kv.divP.div(blk0 * PT_KEYS);
-#pragma unroll
-        for (int w = 0; w < PT_KEYS / 32; w++) {
-          const int key = key0 + w * 32 + lane;
-          const uint32_t there = __ballot_sync(0xffffffffu, key < prefix_end && sh.ids[min((int)a.kv.divP.div(key) - first, PT_IDS - 1)] >= 0);
-#pragma unroll
-          for (int q = 0; q < 32; q++)
-            if (!(there >> q & 1)) s[w * 32 + q] = 0xff800000u;
-        }
-      }
+      const bool special = sh.bad || __any_sync(0xffffffffu, seen < PT_KEYS - 1);
+      auto load = [&](int half) {
+        tc_ld32(ts + half * HALF, s);
+        tc_ld32(ts + half * HALF + 32, s + 32);
+        tc_wait_ld();
+        if (special) pt_mask(a, sh, s, key0 + half * HALF, seen - half * HALF, prefix_end, blk0);
+      };
       float mx = -INFINITY;
 #pragma unroll
-      for (int q = 0; q < PT_KEYS; q++) mx = fmaxf(mx, __uint_as_float(s[q]));
+      for (int half = 0; half < 2; half++) {
+        load(half);
+        float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int q = 0; q < HALF; q += 8)
+#pragma unroll
+          for (int z = 0; z < 4; z++) x[z] = fmaxf(x[z], fmaxf(__uint_as_float(s[q + z]), __uint_as_float(s[q + 4 + z])));
+        mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+      }
       mx *= scale;
       const bool move = mx > m + 8.f;  // from -inf as well
       if (__any_sync(0xffffffffu, move)) {
         const float alpha = move ? (m == -INFINITY ? 0.f : ex2(m - mx)) : 1.f;
         if (move) m = mx;
         l *= alpha;
-        if (i > 0) {  // S(i) is complete, so P(i - 1) V is, which was issued before it
-          for (int q = 0; q < p.hdp; q += 16) {
-            uint32_t x[16];
-            asm volatile(
-                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]),
-                  "=r"(x[9]), "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
-                : "r"(to + q));
-            tc_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * alpha);
-            asm volatile(
-                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(to + q),
-                "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]),
-                "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
-                : "memory");
-          }
-        }
+        // S(i) is complete, so P(i - 1) V is, which was issued before it.
+        if (i > 0) pt_scale_rows(to, p.hdp, alpha);
       }
       const float ref = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // Weights of the second half, then of the first, packed into the
+      // second half of S's columns, which is read by then.
 #pragma unroll
-      for (int q = 0; q < PT_KEYS; q += 4) {
-        float e[4];
+      for (int half = 1; half >= 0; half--) {
+        if (half == 0) load(0);
+        uint32_t w[HALF / 2];
 #pragma unroll
-        for (int z = 0; z < 4; z++) {
-          e[z] = ex2(fmaf(__uint_as_float(s[q + z]), scale, -ref));
-          sum[z] += e[z];
+        for (int q = 0; q < HALF; q += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), make_float2(scale, scale), make_float2(-ref, -ref));
+          const float2 e = make_float2(ex2(x.x), ex2(x.y));
+          sum[(q / 2) & 1] = add2(sum[(q / 2) & 1], e);
+          w[q / 2] = pack2<T>(e.x, e.y);
         }
-        s[q / 2] = pack2<T>(e[0], e[1]);
-        s[q / 2 + 1] = pack2<T>(e[2], e[3]);
+        tc_st32(ts + HALF + half * (HALF / 2), w);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tc_st32(ts, s);
-      tc_st32(ts + 32, s + 32);
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -335,18 +379,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a
     tc_fence_after();
     const int64_t slot = (int64_t)(row < 0 ? 0 : row) * a.slots + (p.split_keys ? 2 * part + t : part);
     for (int q = 0; q < p.hdp; q += 16) {
-      uint32_t x[16];
-      if (count[t] > 0) {
-        asm volatile(
-            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-            : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
-              "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
-            : "r"(to + q));
-        tc_wait_ld();
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[e] = 0;
-      }
+      uint32_t x[16] = {};
+      if (count[t] > 0) pt_ld16(to + q, x);
       if (row >= 0) {
 #pragma unroll
         for (int e = 0; e < 16; e += 4)

@@ -87,10 +87,10 @@ class HeadNorm:
             _on_gpu(name, w)
             if w.dim() != 2 or w.dtype != torch.float32 or not w.is_contiguous() or w.device != q_weight.device:
                 raise _bad(f"{name} is a contiguous float32 tensor [heads or 1, head size]")
-        if (q_weight.shape[0] == 1) != (k_weight.shape[0] == 1) or q_weight.shape[1] != k_weight.shape[1]:
-            raise _bad("query and key weights are both shared or both per head, of one head size")
+        if q_weight.shape[1] != k_weight.shape[1]:
+            raise _bad("query and key weights are of one head size")
         self.q_weight, self.k_weight = q_weight, k_weight
-        # One head of each has one row either way; the stride does not matter then.
+        # One row of each is every head's; otherwise append checks that there is a row for each head.
         self.shared = q_weight.shape[0] == 1 and k_weight.shape[0] == 1
         self.struct = _lib.HeadNorm(_NORMS[kind], float(eps), q_weight.data_ptr(), k_weight.data_ptr(), 0 if self.shared else q_weight.shape[1])
 
