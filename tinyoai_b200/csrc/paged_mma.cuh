@@ -263,6 +263,8 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
         const int d = v * 64 + r * 8;
         vx[v][i] = tv[i] <= most && d < hd ? ld_stream16(vb + vo[i] + d) : make_uint4(0, 0, 0, 0);
       }
+    // The instruction's additions truncate. Float32 results want better than
+    // a chain of them: there each product starts from zero and is added here.
     float s[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; t++) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
@@ -273,8 +275,16 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
           const uint4 y = *reinterpret_cast<const uint4*>(qs + (p * COLS + t * 8 + r) * QS + q * 32 + c * 8);
-          mma16816<TK>(s[t], kx[0][q].x, kx[1][q].x, kx[0][q].y, kx[1][q].y, y.x, y.y);
-          mma16816<TK>(s[t], kx[0][q].z, kx[1][q].z, kx[0][q].w, kx[1][q].w, y.z, y.w);
+          if (PIECES == 1) {
+            mma16816<TK>(s[t], kx[0][q].x, kx[1][q].x, kx[0][q].y, kx[1][q].y, y.x, y.y);
+            mma16816<TK>(s[t], kx[0][q].z, kx[1][q].z, kx[0][q].w, kx[1][q].w, y.z, y.w);
+          } else {
+            float u[4] = {}, w[4] = {};
+            mma16816<TK>(u, kx[0][q].x, kx[1][q].x, kx[0][q].y, kx[1][q].y, y.x, y.y);
+            mma16816<TK>(w, kx[0][q].z, kx[1][q].z, kx[0][q].w, kx[1][q].w, y.z, y.w);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[t][e] += u[e] + w[e];
+          }
         }
     // Scores in units of log2; rows: positions r (entries 0, 1) and r + 8 (2, 3).
     float alpha[NT][2];
@@ -324,13 +334,23 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
         const uint32_t a2 = __byte_perm(x2, x3, 0x5410), a3 = __byte_perm(x2, x3, 0x7632);
 #pragma unroll
         for (int t = 0; t < NT; t++) {
+          if (PIECES == 1) {
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            o[v][j][t][e] *= alpha[t][e];
-            o[v][j][t][2 + e] *= alpha[t][e];
+            for (int e = 0; e < 2; e++) {
+              o[v][j][t][e] *= alpha[t][e];
+              o[v][j][t][2 + e] *= alpha[t][e];
+            }
+            mma16816<TK>(o[v][j][t], a0, a1, a2, a3, ph[t][0], ph[t][1]);
+          } else {
+            float u[4] = {};
+            mma16816<TK>(u, a0, a1, a2, a3, pl[t][0], pl[t][1]);
+            mma16816<TK>(u, a0, a1, a2, a3, ph[t][0], ph[t][1]);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+              o[v][j][t][e] = fmaf(o[v][j][t][e], alpha[t][e], u[e]);
+              o[v][j][t][2 + e] = fmaf(o[v][j][t][2 + e], alpha[t][e], u[2 + e]);
+            }
           }
-          mma16816<TK>(o[v][j][t], a0, a1, a2, a3, ph[t][0], ph[t][1]);
-          if (PIECES == 2) mma16816<TK>(o[v][j][t], a0, a1, a2, a3, pl[t][0], pl[t][1]);
         }
       }
   }

@@ -257,50 +257,66 @@ __global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a
         }
     }
   } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t type = sizeof(T) == 2 && __is_same(T, bf16) ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t id_s = (1u << 4) | type | ((uint32_t)(PT_KEYS >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
-      const uint32_t id_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(p.hdp >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
-      const int ksteps = p.hdp / 16;
-      bool ok = true;
-      auto scores = [&](int t, int i) {
-        const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
-        ok = ok && mbar_wait(&sh.k_full[st], (b / p.stages) & 1, &sh.err);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t qb = smem_u32(qs) + (p.split_keys ? 0 : t) * SUB * PT_SUB, kb = smem_u32(ks) + st * SUB * PT_SUB;
-        for (int kk = 0; kk < ksteps; kk++) {
-          const uint32_t off = (kk >> 2) * PT_SUB + (kk & 3) * 32;
-          tc_mma(tmem + t * 128, tc_smem_desc(qb + off), tc_smem_desc(kb + off), id_s, kk > 0 ? 1u : 0u);
+    // The whole warp runs the schedule, so that descriptors stay in uniform
+    // registers; its elected lane issues the products and their commits.
+    const uint32_t type = __is_same(T, bf16) ? (1u << 7) | (1u << 10) : 0u;
+    const uint32_t id_s = (1u << 4) | type | ((uint32_t)(PT_KEYS >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
+    const uint32_t id_o = (1u << 4) | type | (1u << 16) | ((uint32_t)(p.hdp >> 3) << 17) | ((uint32_t)(PT_ROWS >> 4) << 24);
+    const int ksteps = p.hdp / 16;
+    // Descriptors of the first tile of each operand; steps add to the address field (16-byte units).
+    const uint64_t q_desc = tc_smem_desc(smem_u32(qs)), k_desc = tc_smem_desc(smem_u32(ks)), v_desc = tc_smem_desc_mn(smem_u32(vs), PT_SUB);
+    const bool leader = tc_elect();
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) { ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, &sh.err)); };
+    auto scores = [&](int t, int i) {
+      const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
+      wait(&sh.k_full[st], (b / p.stages) & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t qd = q_desc + (uint64_t)((p.split_keys ? 0 : t) * (SUB * PT_SUB >> 4)), kd = k_desc + (uint64_t)(st * (SUB * PT_SUB >> 4));
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < SUB * 4; kk++) {
+          const uint64_t off = (kk >> 2) * (PT_SUB >> 4) + (kk & 3) * 2;
+          if (kk < ksteps) tc_mma(tmem + t * 128, qd + off, kd + off, id_s, kk > 0 ? 1u : 0u);
         }
         tc_commit(&sh.s_full[t]);
-        if (p.split_keys || t == 1) tc_commit(&sh.k_empty[st]);
-      };
-      auto values = [&](int t, int i) {
-        const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
-        ok = ok && mbar_wait(&sh.v_full[st], (b / p.stages) & 1, &sh.err);
-        ok = ok && mbar_wait(&sh.p_full[t], i & 1, &sh.err);
-        if (!ok) return;
-        tc_fence_after();
-        const uint32_t vb = smem_u32(vs) + st * SUB * PT_SUB;
-        for (int kk = 0; kk < PT_KEYS / 16; kk++)
-          tc_mma_ta(tmem + 256 + t * 128, tmem + t * 128 + PT_KEYS / 2 + kk * 8, tc_smem_desc_mn(vb + kk * 2048, PT_SUB), id_o, i > 0 || kk > 0 ? 1u : 0u);
-        if (p.split_keys || t == 1) tc_commit(&sh.v_empty[st]);
-        if (i == count[t] - 1) tc_commit(&sh.o_done[t]);
-      };
-      for (int t = 0; t < 2; t++)
-        if (count[t] > 0) scores(t, 0);
-      for (int i = 0; i < count[0]; i++)
-        for (int t = 0; t < 2; t++)
-          if (i < count[t]) {
-            values(t, i);
-            if (i + 1 < count[t]) scores(t, i + 1);
-          }
-      if (!ok) {  // products in flight read shared memory: let them finish
-        tc_commit(&sh.o_done[0]);
-        pt_drain(&sh.o_done[0], 0);
+        if ((p.split_keys || t == 1) && b + p.stages < nblk) tc_commit(&sh.k_empty[st]);
       }
+      __syncwarp();
+    };
+    auto values = [&](int t, int i) {
+      const int b = p.split_keys ? 2 * i + t : i, st = b % p.stages;
+      wait(&sh.v_full[st], (b / p.stages) & 1);
+      wait(&sh.p_full[t], i & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t vd = v_desc + (uint64_t)(st * (SUB * PT_SUB >> 4));
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < PT_KEYS / 16; kk++)
+          tc_mma_ta(tmem + 256 + t * 128, tmem + t * 128 + PT_KEYS / 2 + kk * 8, vd + (uint64_t)(kk * (2048 >> 4)), id_o, i > 0 || kk > 0 ? 1u : 0u);
+        if ((p.split_keys || t == 1) && b + p.stages < nblk) tc_commit(&sh.v_empty[st]);
+        if (i == count[t] - 1) tc_commit(&sh.o_done[t]);
+      }
+      __syncwarp();
+    };
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+      if (count[t] > 0) scores(t, 0);
+    for (int i = 0; i < count[0]; i++) {
+#pragma unroll
+      for (int t = 0; t < 2; t++)
+        if (i < count[t]) {
+          values(t, i);
+          if (i + 1 < count[t]) scores(t, i + 1);
+        }
     }
+    if (!ok && leader) {  // products in flight read shared memory: let them finish
+      tc_commit(&sh.o_done[0]);
+      pt_drain(&sh.o_done[0], 0);
+    }
+    __syncwarp();
   } else {
     const int t = warp >> 2, r = tid & 127;
     const int at = p.split_keys ? r : tid;  // this thread's row

@@ -57,6 +57,13 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
+// True on one lane of a converged warp, always the same one.
+__device__ __forceinline__ bool tc_elect() {
+  uint32_t leads;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(leads));
+  return leads != 0;
+}
+
 // Thirty-two columns of this thread's TMEM lane. The load is complete after
 // tc_wait_ld, the store visible to later tcgen05 work after tc_wait_st.
 __device__ __forceinline__ void tc_ld32(uint32_t taddr, uint32_t* r) {
