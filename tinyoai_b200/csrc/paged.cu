@@ -115,9 +115,25 @@ PagedView view_of(const tcu_paged_kv* kv) {
   return v;
 }
 
-int launched(const char* name) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(TCU_ECUDA, "%s: %s", name, cudaGetErrorString(e));
+// Queues a kernel that may start while the one before it on the stream
+// drains; every kernel here waits for that one before it reads (paged.cuh).
+template <typename... P, typename... A>
+int launch(const char* name, void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(TCU_ECUDA, "%s: %s", name, cudaGetErrorString(e));
+  }
   return TCU_OK;
 }
 
@@ -129,7 +145,7 @@ constexpr int SM_COUNT = 148;  // B200
 // Append
 
 template <typename TQ, typename TK>
-void launch_append(const AppendArgs& a, cudaStream_t s) {
+int launch_append(const AppendArgs& a, cudaStream_t s) {
   const int heads = a.H + 2 * a.KVH;
   auto go = [&](auto kern, int lph) {
     // A CTA takes all heads of a token when there are tokens enough to fill
@@ -137,30 +153,23 @@ void launch_append(const AppendArgs& a, cudaStream_t s) {
     const int groups = APPEND_THREADS / lph;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(ceil_div(heads, groups), ceil_div(8 * SM_COUNT, a.T)));
     const int per = (int)(ceil_div(ceil_div(heads, shares), groups) * groups);
-    kern<<<dim3((unsigned)a.T, (unsigned)ceil_div(heads, per)), APPEND_THREADS, 0, s>>>(a, per);
+    return launch("k_append", kern, dim3((unsigned)a.T, (unsigned)ceil_div(heads, per)), APPEND_THREADS, 0, s, a, per);
   };
   auto pick = [&](auto turn) {
     constexpr int TURN = decltype(turn)::value;
-    if (a.hd <= 64)
-      go(k_append<TQ, TK, 8, TURN>, 8);
-    else if (a.hd <= 128)
-      go(k_append<TQ, TK, 16, TURN>, 16);
-    else
-      go(k_append<TQ, TK, 32, TURN>, 32);
+    if (a.hd <= 64) return go(k_append<TQ, TK, 8, TURN>, 8);
+    if (a.hd <= 128) return go(k_append<TQ, TK, 16, TURN>, 16);
+    return go(k_append<TQ, TK, 32, TURN>, 32);
   };
-  if (a.pairs == 0)
-    pick(std::integral_constant<int, TURN_NONE>());
-  else if (a.adjacent)
-    pick(std::integral_constant<int, TURN_OWN>());
-  else if (a.pairs % 8 == 0)
-    pick(std::integral_constant<int, TURN_LANES>());
-  else
-    pick(std::integral_constant<int, TURN_SHARED>());
+  if (a.pairs == 0) return pick(std::integral_constant<int, TURN_NONE>());
+  if (a.adjacent) return pick(std::integral_constant<int, TURN_OWN>());
+  if (a.pairs % 8 == 0) return pick(std::integral_constant<int, TURN_LANES>());
+  return pick(std::integral_constant<int, TURN_SHARED>());
 }
 
 template <typename TK>
-void launch_means(const MeansArgs& a, cudaStream_t s) {
-  k_page_means<TK><<<dim3((unsigned)ceil_div(a.T, 128), a.kv.kvh), 128, 0, s>>>(a);
+int launch_means(const MeansArgs& a, cudaStream_t s) {
+  return launch("k_page_means", k_page_means<TK>, dim3((unsigned)ceil_div(a.T, 128), a.kv.kvh), 128, 0, s, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -304,8 +313,7 @@ int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, R, &tiles);
   const size_t smem = sizeof(float) * CC_GROUPS * (NCH * 32 + 2);
-  k_attend_cc<TQ, TK, NCH, R, SRC><<<dim3((unsigned)x, a.KVH, parts), CC_WARPS * 32, smem, s>>>(a, tiles);
-  return launched("k_attend_cc");
+  return launch("k_attend_cc", k_attend_cc<TQ, TK, NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), CC_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int NT, int SRC>
@@ -315,8 +323,7 @@ int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   constexpr size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>();
   auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
   TRY(allow_smem(kern, smem));
-  kern<<<dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s>>>(a, tiles);
-  return launched("k_attend_mma");
+  return launch("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int SRC>
@@ -373,21 +380,20 @@ int launch_prefix_tc(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
   const dim3 grid(p.tc_tiles, a.KVH, p.tc_parts);
   auto kern = sub == 2 ? k_attend_prefix_tc<T, 2> : k_attend_prefix_tc<T, 1>;
   TRY(allow_smem(kern, smem));
-  kern<<<grid, PT_THREADS, smem, s>>>(a, p.tc_args, km, vm);
-  return launched("k_attend_prefix_tc");
+  return launch("k_attend_prefix_tc", kern, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
 }
 
 template <typename TQ, typename TK>
-int launch_attend(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
+int launch_attend(AttendArgs a, const AttendPlan& p, cudaStream_t s) {
   if (p.tc) {
     if constexpr (std::is_same<TQ, TK>::value && sizeof(TK) == 2) TRY(launch_prefix_tc<TK>(a, p, s));
   } else {
     TRY((launch_parts<TQ, TK, SRC_PREFIX>(a, p.prefix_rows, p.prefix_slots, s)));
   }
+  a.overlap = p.tc;
   TRY((launch_parts<TQ, TK, SRC_OWN>(a, p.own_rows, p.own_slots, s)));
   if (!p.tc && p.prefix_slots + p.own_slots == 1) return TCU_OK;  // the only part wrote the output
-  k_attend_join<TQ, 0><<<dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s>>>(a);
-  return launched("k_attend_join");
+  return launch("k_attend_join", k_attend_join<TQ, 0>, dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s, a);
 }
 
 template <typename TQ, typename TK>
@@ -399,22 +405,19 @@ int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p,
     if constexpr (sizeof(TK) == 4) {
       const size_t smem = sizeof(float) * a.G * a.hd;
       TRY(allow_smem(k_page_scores_cc<TQ, TK>, smem));
-      k_page_scores_cc<TQ, TK><<<grid, 128, smem, s>>>(a, c);
+      TRY(launch("k_page_scores_cc", k_page_scores_cc<TQ, TK>, grid, 128, smem, s, a, c));
     } else {
       const int hd = a.hd <= 64 ? 64 : a.hd <= 96 ? 96 : a.hd <= 128 ? 128 : 256;
       auto kern = hd == 64 ? k_page_scores_mma<TQ, TK, 64> : hd == 96 ? k_page_scores_mma<TQ, TK, 96> : hd == 128 ? k_page_scores_mma<TQ, TK, 128> : k_page_scores_mma<TQ, TK, 256>;
       const size_t smem = (size_t)(sizeof(TQ) == 4 ? 2 : 1) * ((a.G + 7) / 8 * 8) * (hd + 32) * 2;
       TRY(allow_smem(kern, smem));
-      kern<<<grid, MM_WARPS * 32, smem, s>>>(a, c);
+      TRY(launch("k_page_scores_mma", kern, grid, MM_WARPS * 32, smem, s, a, c));
     }
-    TRY(launched("k_page_scores"));
   }
-  k_page_choose<TQ, TK><<<dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s>>>(a, c);
-  TRY(launched("k_page_choose"));
+  TRY(launch("k_page_choose", k_page_choose<TQ, TK>, dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s, a, c));
   TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
   if (p.own_slots == 1) return TCU_OK;  // the only part wrote the output
-  k_attend_join<TQ, 1><<<dim3(queries, (a.H + 3) / 4), 128, 0, s>>>(a);
-  return launched("k_attend_join");
+  return launch("k_attend_join", k_attend_join<TQ, 1>, dim3(queries, (a.H + 3) / 4), 128, 0, s, a);
 }
 
 int check_queries(const tcu_paged_kv* kv, const tcu_paged_queries* q) {
@@ -551,11 +554,8 @@ int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, 
   a.counts = counts;
   a.divP = FastDiv::of((uint32_t)page_tokens);
   const unsigned grid = (unsigned)std::max<int64_t>(1, ceil_div(capacity, PLAN_TILE));
-  if (n <= 256)
-    k_plan_step<256><<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  else
-    k_plan_step<1024><<<grid, 1024, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return launched("k_plan_step");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return n <= 256 ? launch("k_plan_step", k_plan_step<256>, dim3(grid), 256, 0, s, a) : launch("k_plan_step", k_plan_step<1024>, dim3(grid), 1024, 0, s, a);
 }
 
 int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t dtype, int32_t rows, int32_t heads, const void* qkv,
@@ -617,15 +617,10 @@ int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32
   a.q_stride = q_stride;
   a.kv = view_of(kv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == TCU_F32 && kv->dtype == TCU_F32)
-    launch_append<float, float>(a, s);
-  else if (dtype == TCU_F32)
-    launch_append<float, __half>(a, s);
-  else if (dtype == TCU_F16)
-    launch_append<__half, __half>(a, s);
-  else
-    launch_append<bf16, bf16>(a, s);
-  return launched("k_append");
+  if (dtype == TCU_F32 && kv->dtype == TCU_F32) return launch_append<float, float>(a, s);
+  if (dtype == TCU_F32) return launch_append<float, __half>(a, s);
+  if (dtype == TCU_F16) return launch_append<__half, __half>(a, s);
+  return launch_append<bf16, bf16>(a, s);
 }
 
 int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t rows, const int64_t* slots, void* means) {
@@ -644,13 +639,9 @@ int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_
   a.means = means;
   a.kv = view_of(kv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (kv->dtype == TCU_F32)
-    launch_means<float>(a, s);
-  else if (kv->dtype == TCU_F16)
-    launch_means<__half>(a, s);
-  else
-    launch_means<bf16>(a, s);
-  return launched("k_page_means");
+  if (kv->dtype == TCU_F32) return launch_means<float>(a, s);
+  if (kv->dtype == TCU_F16) return launch_means<__half>(a, s);
+  return launch_means<bf16>(a, s);
 }
 
 int tcu_paged_attend_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* q, int32_t prefix_pages, int32_t max_length, uint64_t* bytes) {

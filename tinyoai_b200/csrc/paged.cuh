@@ -152,6 +152,7 @@ struct PlanSum {
 // tile's chain of loads, barriers and searches takes about 3 us).
 template <int PLAN_THREADS>
 __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
+  pdl_wait();
   __shared__ PlanSum wsum[PLAN_THREADS / 32];
   __shared__ int s_start[PLAN_THREADS + 1], s_page[PLAN_THREADS], s_held[PLAN_THREADS];
   __shared__ int s_bad;
@@ -342,6 +343,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) k_append(AppendArgs a, int 
   const int d = lane * 8;
   const bool in = d < a.hd;
   const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + d;
+  pdl_wait();
   Raw8<TQ> raw[APPEND_HEADS];
   auto fetch = [&](int hb) {
 #pragma unroll
@@ -463,6 +465,7 @@ __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
   const int wid = threadIdx.x >> 5, warp = blockIdx.x * 4 + wid, lane = threadIdx.x & 31;
   const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, rows = 32 / lpr;
   const int64_t t = (int64_t)warp * 32 + lane;
+  pdl_wait();
   int64_t slot = t < a.T ? a.slots[t] : -1;
   if (slot >= (int64_t)a.kv.num_pages * P) slot = -1;
   const int my_page = slot < 0 ? -1 : (int)(slot / P);
@@ -538,7 +541,23 @@ struct AttendArgs {
   // Sparse: the pages each (query, KV head) reads (ascending, -1 behind them).
   const int* pages;  // [T][KVH][budget]
   int budget;
+  // 1: launched behind the prefix's kernel to run beside it (see overlap_begin).
+  int overlap;
 };
+
+// Kernels here are launched so that they may start while the one before them
+// on the stream drains (programmatic dependent launch), and wait for it
+// before they read anything. The kernel of the requests' own positions reads
+// nothing the prefix's kernel writes and is bound by other parts of the GPU:
+// it starts as soon as every CTA of that one has (which had waited for all
+// earlier work), runs beside it, and its last CTA ends after it, so that what
+// follows finds both complete.
+__device__ __forceinline__ void overlap_begin(const AttendArgs& a) {
+  if (!a.overlap) pdl_wait();
+}
+__device__ __forceinline__ void overlap_end(const AttendArgs& a) {
+  if (a.overlap && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) pdl_wait();
+}
 
 struct Query {
   int token;     // row of q, -1: none
@@ -617,6 +636,7 @@ constexpr int CC_GROUPS = CC_WARPS * 4;
 
 template <typename TQ, typename TK, int NCH, int R, int SRC>
 __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int row_tiles) {
+  pdl_wait();
   extern __shared__ __align__(16) float cc_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int grp = lane >> 3, l8 = lane & 7;
@@ -816,6 +836,7 @@ __device__ __forceinline__ int own_parts(const AttendArgs& a, int pos) {
 // read. grid: x = request * max_fresh + query, y = heads / 4.
 template <typename TQ, int LIST>
 __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
+  pdl_wait();
   const int i = blockIdx.x / a.max_fresh, j = blockIdx.x % a.max_fresh;
   const int h = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (h >= a.H) return;
@@ -911,6 +932,7 @@ template <typename TQ, typename TK>
 __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs c) {
   extern __shared__ __align__(16) float cq[];  // [G][hd]
   __shared__ float s_eps[4];
+  pdl_wait();
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
   if (q.token < 0) return;
   const int g = blockIdx.y, hd = a.hd;
@@ -1010,6 +1032,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
   __shared__ int s_sure, s_open;
   __shared__ uint32_t s_eps;
   extern __shared__ float cache[];  // min(width, CHOOSE_CACHE)
+  pdl_wait();
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
   if (q.token < 0) return;
   const int g = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;

@@ -115,7 +115,7 @@ __device__ __forceinline__ void mm_load_queries(const AttendArgs& a, TK* qs, con
 
 // grid as k_attend_cc's, with row tiles of 8 * NT rows.
 template <typename TQ, typename TK, int HD, int NT, int SRC>
-__global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT == 4 || HD > 128 ? 2 : 3) k_attend_mma(AttendArgs a, int row_tiles) {
+__device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
   constexpr int COLS = 8 * NT, KG = (HD + 31) / 32, VG = (HD + 63) / 64;
   constexpr int PIECES = sizeof(TQ) == 4 ? 2 : 1;
   constexpr int QS = HD + 32;
@@ -416,6 +416,13 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
   }
 }
 
+template <typename TQ, typename TK, int HD, int NT, int SRC>
+__global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT == 4 || HD > 128 ? 2 : 3) k_attend_mma(const __grid_constant__ AttendArgs a, int row_tiles) {
+  overlap_begin(a);
+  mm_part<TQ, TK, HD, NT, SRC>(a, row_tiles);
+  overlap_end(a);
+}
+
 // Float32 scores of pages (16-bit caches): the first product of the attention
 // with mean keys in the place of keys, and the same product of magnitudes for
 // the error bound; both cost nothing beside the means' bytes.
@@ -429,6 +436,7 @@ __global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a,
   __shared__ float s_scale[TCU_PAGED_MAX_GROUP];
   __shared__ uint32_t s_eps[MM_WARPS];
   TK* qs = reinterpret_cast<TK*>(mm_mem);
+  pdl_wait();
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
   if (q.token < 0) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cc = lane & 3;

@@ -38,6 +38,9 @@ namespace tcu {
 
 constexpr int PT_ROWS = 128, PT_KEYS = 128;
 constexpr int PT_THREADS = 320;
+// Registers a thread: leaves an SM 16,896 of them and 23 KB of shared memory,
+// one CTA of k_attend_mma beside this kernel's.
+#define PT_REGS 152
 constexpr int PT_IDS = 1024;      // page ids of a part
 constexpr int PT_SUB = 16384;     // bytes of 128 rows of 64 values
 constexpr int PT_MAX_STAGES = 4;
@@ -140,9 +143,11 @@ __device__ __noinline__ void pt_scale_rows(uint32_t taddr, int n, float f) {
 }
 
 template <typename T, int SUB>
-__global__ void __launch_bounds__(PT_THREADS, 1) k_attend_prefix_tc(AttendArgs a, PagedTcArgs p, const __grid_constant__ CUtensorMap kmap,
+__global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ AttendArgs a, const __grid_constant__ PagedTcArgs p, const __grid_constant__ CUtensorMap kmap,
                                                                      const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ uint8_t pt_mem[];
+  pdl_wait();
+  pdl_launch_dependents();  // the requests' own positions
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pt_mem) + 1023) & ~(uintptr_t)1023);
   uint8_t* qs = base;
   uint8_t* ks = qs + (size_t)(p.split_keys ? 1 : 2) * SUB * PT_SUB;
