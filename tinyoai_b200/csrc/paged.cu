@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -300,11 +301,17 @@ int64_t grid_x(const AttendArgs& a, int rows, int* tiles) {
   return (int64_t)a.n * (SRC == SRC_OWN ? 1 : a.max_fresh) * *tiles;
 }
 
-// Raises a kernel's dynamic shared memory limit (it is a property of the
-// kernel on the current device; setting it again changes nothing).
-template <typename K>
-int allow_smem(K kern, size_t bytes) {
-  if (bytes > 48 * 1024) CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+// Once per kernel and device: lets the kernel have up to `most` bytes of
+// dynamic shared memory.
+template <auto Kern>
+int prepare_kernel(size_t most) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  CK(cudaGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_acquire) & bit) return TCU_OK;
+  CK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  done.fetch_or(bit, std::memory_order_release);
   return TCU_OK;
 }
 
@@ -321,8 +328,8 @@ int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, 8 * NT, &tiles);
   constexpr size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>();
-  auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
-  TRY(allow_smem(kern, smem));
+  constexpr auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
+  TRY((prepare_kernel<kern>(smem)));
   return launch("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s, a, tiles);
 }
 
@@ -378,9 +385,12 @@ int launch_prefix_tc(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
   const int sub = a.hd > 64 ? 2 : 1;
   const size_t smem = pt_smem(sub, p.tc_args.split_keys, p.tc_args.stages);
   const dim3 grid(p.tc_tiles, a.KVH, p.tc_parts);
-  auto kern = sub == 2 ? k_attend_prefix_tc<T, 2> : k_attend_prefix_tc<T, 1>;
-  TRY(allow_smem(kern, smem));
-  return launch("k_attend_prefix_tc", kern, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
+  if (sub == 2) {
+    TRY((prepare_kernel<k_attend_prefix_tc<T, 2>>(PT_MAX_SMEM)));
+    return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 2>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
+  }
+  TRY((prepare_kernel<k_attend_prefix_tc<T, 1>>(PT_MAX_SMEM)));
+  return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 1>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
 }
 
 template <typename TQ, typename TK>
@@ -396,23 +406,34 @@ int launch_attend(AttendArgs a, const AttendPlan& p, cudaStream_t s) {
   return launch("k_attend_join", k_attend_join<TQ, 0>, dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s, a);
 }
 
+template <typename T>
+int launch_scores_cc(const AttendArgs& a, const ChooseArgs& c, unsigned queries, cudaStream_t s) {
+  TRY((prepare_kernel<k_page_scores_cc<T, T>>(sizeof(float) * TCU_PAGED_MAX_GROUP * TCU_PAGED_MAX_HEAD_DIM)));
+  return launch("k_page_scores_cc", k_page_scores_cc<T, T>, dim3(queries, a.KVH, c.tiles), 128, sizeof(float) * a.G * a.hd, s, a, c);
+}
+
+template <typename TQ, typename TK, int HD>
+int launch_scores(const AttendArgs& a, const ChooseArgs& c, unsigned queries, cudaStream_t s) {
+  constexpr size_t row = (sizeof(TQ) == 4 ? 2 : 1) * (HD + 32) * 2;
+  TRY((prepare_kernel<k_page_scores_mma<TQ, TK, HD>>(row * TCU_PAGED_MAX_GROUP)));
+  return launch("k_page_scores_mma", k_page_scores_mma<TQ, TK, HD>, dim3(queries, a.KVH, c.tiles), MM_WARPS * 32, row * ((a.G + 7) / 8 * 8), s, a, c);
+}
+
 template <typename TQ, typename TK>
 int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p, cudaStream_t s) {
   const unsigned queries = (unsigned)((int64_t)a.n * a.max_fresh);
   // No query has more than width pages: with room for all, none is scored.
   if (c.top > 0 && c.width - c.first - c.last > c.top) {
-    const dim3 grid(queries, a.KVH, c.tiles);
-    if constexpr (sizeof(TK) == 4) {
-      const size_t smem = sizeof(float) * a.G * a.hd;
-      TRY(allow_smem(k_page_scores_cc<TQ, TK>, smem));
-      TRY(launch("k_page_scores_cc", k_page_scores_cc<TQ, TK>, grid, 128, smem, s, a, c));
-    } else {
-      const int hd = a.hd <= 64 ? 64 : a.hd <= 96 ? 96 : a.hd <= 128 ? 128 : 256;
-      auto kern = hd == 64 ? k_page_scores_mma<TQ, TK, 64> : hd == 96 ? k_page_scores_mma<TQ, TK, 96> : hd == 128 ? k_page_scores_mma<TQ, TK, 128> : k_page_scores_mma<TQ, TK, 256>;
-      const size_t smem = (size_t)(sizeof(TQ) == 4 ? 2 : 1) * ((a.G + 7) / 8 * 8) * (hd + 32) * 2;
-      TRY(allow_smem(kern, smem));
-      TRY(launch("k_page_scores_mma", kern, grid, MM_WARPS * 32, smem, s, a, c));
-    }
+    if constexpr (sizeof(TK) == 4)
+      TRY(launch_scores_cc<TQ>(a, c, queries, s));
+    else if (a.hd <= 64)
+      TRY((launch_scores<TQ, TK, 64>(a, c, queries, s)));
+    else if (a.hd <= 96)
+      TRY((launch_scores<TQ, TK, 96>(a, c, queries, s)));
+    else if (a.hd <= 128)
+      TRY((launch_scores<TQ, TK, 128>(a, c, queries, s)));
+    else
+      TRY((launch_scores<TQ, TK, 256>(a, c, queries, s)));
   }
   TRY(launch("k_page_choose", k_page_choose<TQ, TK>, dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s, a, c));
   TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
