@@ -302,15 +302,17 @@ int64_t grid_x(const AttendArgs& a, int rows, int* tiles) {
 }
 
 // Once per kernel and device: lets the kernel have up to `most` bytes of
-// dynamic shared memory.
+// dynamic shared memory, and states the share of an SM's cache it wants as
+// shared memory (percent, -1: left to the driver).
 template <auto Kern>
-int prepare_kernel(size_t most) {
+int prepare_kernel(size_t most, int carveout = -1) {
   static std::atomic<uint64_t> done{0};
   int device = 0;
   CK(cudaGetDevice(&device));
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_acquire) & bit) return TCU_OK;
   CK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  if (carveout >= 0) CK(cudaFuncSetAttribute(Kern, cudaFuncAttributePreferredSharedMemoryCarveout, carveout));
   done.fetch_or(bit, std::memory_order_release);
   return TCU_OK;
 }
@@ -329,7 +331,10 @@ int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   const int64_t x = grid_x<SRC>(a, 8 * NT, &tiles);
   constexpr size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>();
   constexpr auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
-  TRY((prepare_kernel<kern>(smem)));
+  // Beside the prefix's kernel: with half of the cache as shared memory, which
+  // its own four CTAs fill, 256 requests over 32,768 shared positions take 241 us,
+  // with the driver's choice 271, with all of it (no cache left for its loads) 282.
+  TRY((prepare_kernel<kern>(smem, SRC == SRC_OWN ? 50 : -1)));
   return launch("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s, a, tiles);
 }
 
@@ -386,10 +391,10 @@ int launch_prefix_tc(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
   const size_t smem = pt_smem(sub, p.tc_args.split_keys, p.tc_args.stages);
   const dim3 grid(p.tc_tiles, a.KVH, p.tc_parts);
   if (sub == 2) {
-    TRY((prepare_kernel<k_attend_prefix_tc<T, 2>>(PT_MAX_SMEM)));
+    TRY((prepare_kernel<k_attend_prefix_tc<T, 2>>(PT_MAX_SMEM, 50)));
     return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 2>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
   }
-  TRY((prepare_kernel<k_attend_prefix_tc<T, 1>>(PT_MAX_SMEM)));
+  TRY((prepare_kernel<k_attend_prefix_tc<T, 1>>(PT_MAX_SMEM, 50)));
   return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 1>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
 }
 

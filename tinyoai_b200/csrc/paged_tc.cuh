@@ -38,10 +38,9 @@ namespace tcu {
 
 constexpr int PT_ROWS = 128, PT_KEYS = 128;
 constexpr int PT_THREADS = 320;
-// Registers a thread: an SM sub-partition with three of this kernel's ten
-// warps keeps the 4,096 registers of one k_attend_mma warp, and the SM 23 KB
-// of shared memory: one CTA of that kernel runs beside this one's.
-#define PT_REGS 128
+// Registers a thread: leaves an SM 16,896 of them and 23 KB of shared memory,
+// one CTA of k_attend_mma beside this kernel's.
+#define PT_REGS 152
 constexpr int PT_IDS = 1024;      // page ids of a part
 constexpr int PT_SUB = 16384;     // bytes of 128 rows of 64 values
 constexpr int PT_MAX_STAGES = 4;
@@ -103,19 +102,23 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return d;
 }
 
-// Masks 32 scores of positions key0 ..: past column `seen`, and of pages that are none.
-__device__ __forceinline__ uint32_t pt_mask_bits(const AttendArgs& a, const PtShared& sh, int key0, int seen, int prefix_end, int blk0) {
-  const int first = (int)a.kv.divP.div(blk0 * PT_KEYS), key = key0 + (threadIdx.x & 31);
-  const bool there = key < prefix_end && sh.ids[min((int)a.kv.divP.div(min(key, prefix_end - 1)) - first, PT_IDS - 1)] >= 0;
-  const uint32_t bits = __ballot_sync(0xffffffffu, there);
-  const int n = min(max(seen + 1, 0), 32);
-  return bits & (n == 32 ? 0xffffffffu : (1u << n) - 1);
-}
-__device__ __forceinline__ void pt_mask(const AttendArgs& a, const PtShared& sh, uint32_t (&s)[32], int key0, int seen, int prefix_end, int blk0) {
-  const uint32_t bits = pt_mask_bits(a, sh, key0, seen, prefix_end, blk0);
+// Masks 64 scores of positions key0 ..: past column `seen`, and of pages that are none.
+__device__ __forceinline__ void pt_mask_bits(const AttendArgs& a, const PtShared& sh, int key0, int seen, int prefix_end, int blk0, uint32_t* bits) {
+  const int lane = threadIdx.x & 31, first = (int)a.kv.divP.div(blk0 * PT_KEYS);
 #pragma unroll
-  for (int q = 0; q < 32; q++)
-    if (!(bits >> q & 1)) s[q] = 0xff800000u;
+  for (int w = 0; w < 2; w++) {
+    const int key = key0 + w * 32 + lane;
+    const uint32_t there = __ballot_sync(0xffffffffu, key < prefix_end && sh.ids[min((int)a.kv.divP.div(min(key, prefix_end - 1)) - first, PT_IDS - 1)] >= 0);
+    const int n = min(max(seen + 1 - 32 * w, 0), 32);
+    bits[w] = there & (n == 32 ? 0xffffffffu : (1u << n) - 1);
+  }
+}
+__device__ __forceinline__ void pt_mask(const AttendArgs& a, const PtShared& sh, uint32_t (&s)[PT_KEYS / 2], int key0, int seen, int prefix_end, int blk0) {
+  uint32_t bits[2];
+  pt_mask_bits(a, sh, key0, seen, prefix_end, blk0, bits);
+#pragma unroll
+  for (int q = 0; q < PT_KEYS / 2; q++)
+    if (!(bits[q >> 5] >> (q & 31) & 1)) s[q] = 0xff800000u;
 }
 
 __device__ __forceinline__ void pt_ld16(uint32_t taddr, uint32_t (&x)[16]) {
@@ -127,14 +130,6 @@ __device__ __forceinline__ void pt_ld16(uint32_t taddr, uint32_t (&x)[16]) {
   tc_wait_ld();
 }
 
-__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&x)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(x[0]),
-      "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
-      "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
-      : "memory");
-}
-
 // This lane's first n columns from taddr on, times f.
 __device__ __forceinline__ void pt_scale_rows(uint32_t taddr, int n, float f) {
   for (int q = 0; q < n; q += 16) {
@@ -142,7 +137,11 @@ __device__ __forceinline__ void pt_scale_rows(uint32_t taddr, int n, float f) {
     pt_ld16(taddr + q, x);
 #pragma unroll
     for (int e = 0; e < 16; e++) x[e] = __float_as_uint(__uint_as_float(x[e]) * f);
-    tc_st16(taddr + q, x);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr + q), "r"(x[0]),
+        "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
+        "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+        : "memory");
   }
 }
 
@@ -344,30 +343,29 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
         break;
       }
       tc_fence_after();
-      // First the row's maximum, then the weights, 32 columns at a time with
-      // the next 32 on their way (a row of 128 would not stay in registers).
-      // The weights are taken from the last columns on and packed into the
-      // second half of S's columns: 16 columns that were read before.
-      constexpr int CH = 32, N = PT_KEYS / CH;
-      uint32_t s[2][CH];
+      // First the row's maximum, 64 columns at a time (all 128 would not stay
+      // in registers); the second half is still there for its weights.
+      constexpr int HALF = PT_KEYS / 2;
+      uint32_t s[HALF];
       const int seen = min(limit, prefix_end - 1) - key0;  // columns up to here are this row's
       const bool special = sh.bad || __any_sync(0xffffffffu, seen < PT_KEYS - 1);
-      float mx = -INFINITY;
-      tc_ld32(ts, s[0]);
-#pragma unroll
-      for (int q = 0; q < N; q++) {
+      auto load = [&](int half) {
+        tc_ld32(ts + half * HALF, s);
+        tc_ld32(ts + half * HALF + 32, s + 32);
         tc_wait_ld();
-        if (q + 1 < N) tc_ld32(ts + (q + 1) * CH, s[(q + 1) & 1]);
-        uint32_t(&v)[CH] = s[q & 1];
-        if (special) pt_mask(a, sh, v, key0 + q * CH, seen - q * CH, prefix_end, blk0);
+        if (special) pt_mask(a, sh, s, key0 + half * HALF, seen - half * HALF, prefix_end, blk0);
+      };
+      float mx = -INFINITY;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        load(half);
         float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < CH; e += 8)
+        for (int q = 0; q < HALF; q += 8)
 #pragma unroll
-          for (int z = 0; z < 4; z++) x[z] = fmaxf(x[z], fmaxf(__uint_as_float(v[e + z]), __uint_as_float(v[e + 4 + z])));
+          for (int z = 0; z < 4; z++) x[z] = fmaxf(x[z], fmaxf(__uint_as_float(s[q + z]), __uint_as_float(s[q + 4 + z])));
         mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
       }
-      tc_ld32(ts + (N - 2) * CH, s[N & 1]);
       mx *= scale;
       const bool move = mx > m + 8.f;  // from -inf as well
       if (__any_sync(0xffffffffu, move)) {
@@ -379,23 +377,20 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
       }
       const float ref = m == -INFINITY ? 0.f : m;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      // Weights of the second half, then of the first, packed into the
+      // second half of S's columns, which is read by then.
 #pragma unroll
-      for (int q = N - 1; q >= 0; q--) {
-        uint32_t(&v)[CH] = s[q & 1];
-        if (q < N - 1) {
-          tc_wait_ld();
-          if (special) pt_mask(a, sh, v, key0 + q * CH, seen - q * CH, prefix_end, blk0);
-          if (q > 0) tc_ld32(ts + (q - 1) * CH, s[(q - 1) & 1]);
-        }
-        uint32_t w[CH / 2];
+      for (int half = 1; half >= 0; half--) {
+        if (half == 0) load(0);
+        uint32_t w[HALF / 2];
 #pragma unroll
-        for (int e = 0; e < CH; e += 2) {
-          const float2 x = fma2(make_float2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), make_float2(scale, scale), make_float2(-ref, -ref));
-          const float2 y = make_float2(ex2(x.x), ex2(x.y));
-          sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], y);
-          w[e / 2] = pack2<T>(y.x, y.y);
+        for (int q = 0; q < HALF; q += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), make_float2(scale, scale), make_float2(-ref, -ref));
+          const float2 e = make_float2(ex2(x.x), ex2(x.y));
+          sum[(q / 2) & 1] = add2(sum[(q / 2) & 1], e);
+          w[q / 2] = pack2<T>(e.x, e.y);
         }
-        tc_st16(ts + PT_KEYS / 2 + q * (CH / 2), w);
+        tc_st32(ts + HALF + half * (HALF / 2), w);
       }
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
       tc_wait_st();

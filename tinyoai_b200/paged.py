@@ -45,16 +45,20 @@ def _code(name, t):
 
 
 def _whole(name, t, dtype, device, dims=1):
-    """A contiguous tensor of whole numbers (its rows may lie apart when dims is 2)."""
+    """The address of a contiguous tensor of whole numbers (its rows may lie apart when dims is 2)."""
+    if t.dtype is dtype and t.device == device and t.dim() == dims and (t.is_contiguous() or t.stride(-1) == 1):
+        return t.data_ptr()
     if t.dtype != dtype or t.dim() != dims or t.device != device:
         raise _bad(f"{name} must be a {dims}-d {dtype} tensor on {device}, got {t.dim()}-d {t.dtype} on {t.device}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise _bad(f"{name} is not contiguous")
-    return t.data_ptr()
+    raise _bad(f"{name} is not contiguous")
 
 
-def _stream(stream, device):
-    return (torch.cuda.current_stream(device) if stream is None else stream).cuda_stream
+# The current stream's handle without a Stream object around it.
+_current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _stream(stream, index):
+    return _current(index) if stream is None else stream.cuda_stream
 
 
 def _on_gpu(name, t):
@@ -74,6 +78,7 @@ class Rotary:
             raise _bad("the rotary table is a contiguous float32 tensor [positions, pairs, 2]")
         self.table = table
         self.struct = _lib.Rotary(table.data_ptr(), table.shape[0], table.shape[1], 1 if adjacent else 0)
+        self.ref = C.byref(self.struct)
 
 
 class HeadNorm:
@@ -93,6 +98,8 @@ class HeadNorm:
         # One row of each is every head's; otherwise append checks that there is a row for each head.
         self.shared = q_weight.shape[0] == 1 and k_weight.shape[0] == 1
         self.struct = _lib.HeadNorm(_NORMS[kind], float(eps), q_weight.data_ptr(), k_weight.data_ptr(), 0 if self.shared else q_weight.shape[1])
+        self.ref, self.device, self.head_dim = C.byref(self.struct), q_weight.device, q_weight.shape[1]
+        self.heads = (q_weight.shape[0], k_weight.shape[0])
 
 
 class StepPlan:
@@ -117,31 +124,27 @@ class StepPlan:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.max_requests, self.capacity, self.page_tokens = max_requests, capacity, page_tokens
-        self._starts = torch.zeros(max_requests + 1, dtype=torch.int32, device=self.device)
-        self._lengths = torch.zeros(max_requests, dtype=torch.int32, device=self.device)
+        words = torch.zeros(2 * max_requests + 4 + capacity, dtype=torch.int32, device=self.device)
+        self._starts, self._lengths, self.counts, self.positions = words.split([max_requests + 1, max_requests, 3, capacity])
         self.starts, self.lengths = self._starts, self._lengths
-        self.positions = torch.full((capacity,), -1, dtype=torch.int32, device=self.device)
-        self.slots = torch.full((capacity,), -1, dtype=torch.int64, device=self.device)
-        self.counts = torch.zeros(3, dtype=torch.int32, device=self.device)
-        self._outs = (self._starts.data_ptr(), self._lengths.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(),
-                      self.counts.data_ptr())
+        self.slots = torch.zeros(capacity, dtype=torch.int64, device=self.device)
+        self.index, self._n, self._call = self.device.index, max_requests, lib().tcu_plan_step
+        self._outs = tuple(t.data_ptr() for t in (self._starts, self._lengths, self.positions, self.slots, self.counts))
 
     def build(self, held, fresh, tables, free_pages, stream=None):
         """held, fresh: int32 [requests], positions held and tokens added;
         tables: int32 [requests, width], updated in place; free_pages: int32.
         Returns self."""
-        d = self.device
-        n = held.shape[0] if held.dim() == 1 else -1
+        d, index = self.device, self.index
         h, f = _whole("held", held, torch.int32, d), _whole("fresh", fresh, torch.int32, d)
         t, p = _whole("tables", tables, torch.int32, d, 2), _whole("free_pages", free_pages, torch.int32, d)
-        if fresh.shape[0] != n or tables.shape[0] != n or n > self.max_requests:
-            raise _bad(f"{n} requests held, {fresh.shape[0]} fresh, {tables.shape[0]} tables, room for {self.max_requests}")
-        width = tables.shape[1]
-        stride = tables.stride(0) if n > 1 else max(width, tables.stride(0))
-        if self.starts.shape[0] != n + 1:
-            self.starts, self.lengths = self._starts[:n + 1], self._lengths[:n]
-        check(lib().tcu_plan_step(d.index, _stream(stream, d), n, h, f, self.page_tokens, t, width, stride, p, free_pages.shape[0],
-                                  self.capacity, *self._outs))
+        n, width = tables.shape
+        if len(held) != n or len(fresh) != n or n > self.max_requests:
+            raise _bad(f"{len(held)} requests held, {len(fresh)} fresh, {n} tables, room for {self.max_requests}")
+        if self._n != n:
+            self.starts, self.lengths, self._n = self._starts[:n + 1], self._lengths[:n], n
+        check(self._call(index, _stream(stream, index), n, h, f, self.page_tokens, t, width, tables.stride(0) if n > 1 else width, p,
+                         len(free_pages), self.capacity, *self._outs))
         return self
 
 
@@ -158,10 +161,13 @@ class Cache:
             raise _bad("k and v need the same strides and a contiguous last dimension")
         self.k, self.v, self.code = k, v, _code("the cache", k)
         self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
+        self._means = torch.Size((self.num_pages, self.kv_heads, self.head_dim))
+        self._scale = 1 / math.sqrt(self.head_dim) if self.head_dim else 0.0
         self.struct = _lib.PagedKV(k.data_ptr(), v.data_ptr(), self.code, self.num_pages, self.page_tokens, self.kv_heads, self.head_dim,
                                    k.stride(0), k.stride(1), k.stride(2))
         self._ref = C.byref(self.struct)
         self._sized = (None, 0)
+        self.index, self._lib = self.device.index, lib()
 
     def append(self, qkv, heads, positions, slots, rotary=None, norm=None, out=None, stream=None):
         """Norm and rotation of the step's rows and their append
@@ -169,32 +175,34 @@ class Cache:
         positions int32 and slots int64 [rows]. Returns the queries
         [rows, heads, head size]; rows that are skipped (slot -1) keep what
         `out` held."""
-        d, hd = self.device, self.head_dim
-        if qkv.dim() != 2 or qkv.device != d or qkv.shape[1] != (heads + 2 * self.kv_heads) * hd or qkv.stride(1) != 1:
+        d, index, hd = self.device, self.index, self.head_dim
+        width = (heads + 2 * self.kv_heads) * hd
+        if qkv.dim() != 2 or qkv.device != d or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise _bad(f"qkv must be rows of ({heads} + 2 * {self.kv_heads}) * {hd} values on {d}, got {tuple(qkv.shape)} on {qkv.device}")
-        rows, code = qkv.shape[0], _code("qkv", qkv)
+        rows = qkv.shape[0]
         p, s = _whole("positions", positions, torch.int32, d), _whole("slots", slots, torch.int64, d)
-        if positions.shape[0] != rows or slots.shape[0] != rows:
-            raise _bad(f"{rows} rows, {positions.shape[0]} positions, {slots.shape[0]} slots")
+        if len(positions) != rows or len(slots) != rows:
+            raise _bad(f"{rows} rows, {len(positions)} positions, {len(slots)} slots")
+        stride = heads * hd
         if out is None:
-            out = torch.empty((rows, heads, hd), dtype=qkv.dtype, device=d)
-        elif out.shape != (rows, heads, hd) or out.dtype != qkv.dtype or out.device != d or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
-            raise _bad(f"out must be [{rows}, {heads}, {hd}] of {qkv.dtype} on {d}, its heads contiguous")
+            out = qkv.new_empty((rows, heads, hd))
+        else:
+            if out.shape != (rows, heads, hd) or out.dtype != qkv.dtype or out.device != d or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
+                raise _bad(f"out must be [{rows}, {heads}, {hd}] of {qkv.dtype} on {d}, its heads contiguous")
+            stride = out.stride(0) if rows > 1 else stride
         rot = nrm = None
         if rotary is not None:
             if rotary.table.device != d:
                 raise _bad("the rotary table is on another device")
-            rot = C.byref(rotary.struct)
+            rot = rotary.ref
         if norm is not None:
-            if norm.q_weight.device != d or norm.q_weight.shape[1] != hd:
-                raise _bad(f"norm weights of head size {norm.q_weight.shape[1]} on {norm.q_weight.device}, the cache has {hd} on {d}")
-            if not norm.shared and (norm.q_weight.shape[0] != heads or norm.k_weight.shape[0] != self.kv_heads):
+            if norm.device != d or norm.head_dim != hd:
+                raise _bad(f"norm weights of head size {norm.head_dim} on {norm.device}, the cache has {hd} on {d}")
+            if not norm.shared and norm.heads != (heads, self.kv_heads):
                 raise _bad("norm weights per head must be [heads, head size] and [KV heads, head size]")
-            nrm = C.byref(norm.struct)
-        width = qkv.shape[1]
-        check(lib().tcu_paged_append(d.index, _stream(stream, d), self._ref, code, rows, heads, qkv.data_ptr(),
-                                     qkv.stride(0) if rows > 1 else max(width, qkv.stride(0)), p, s, rot, nrm, out.data_ptr(),
-                                     out.stride(0) if rows > 1 else max(heads * hd, out.stride(0))))
+            nrm = norm.ref
+        check(self._lib.tcu_paged_append(index, _stream(stream, index), self._ref, _code("qkv", qkv), rows, heads, qkv.data_ptr(),
+                                         qkv.stride(0) if rows > 1 else width, p, s, rot, nrm, out.data_ptr(), stride))
         return out
 
     def page_means(self, slots, means, stream=None):
@@ -203,7 +211,7 @@ class Cache:
         cache's type. Returns means."""
         self._check_means(means)
         s = _whole("slots", slots, torch.int64, self.device)
-        check(lib().tcu_paged_means(self.device.index, _stream(stream, self.device), self._ref, slots.shape[0], s, means.data_ptr()))
+        check(self._lib.tcu_paged_means(self.index, _stream(stream, self.index), self._ref, len(slots), s, means.data_ptr()))
         return means
 
     def attend(self, q, tables, starts, lengths, max_fresh, prefix=None, scale=None, max_length=0, out=None, stream=None):
@@ -215,16 +223,17 @@ class Cache:
         default; max_length: a bound on lengths, where the host knows one
         (sizes the work; 0: what the tables map). Returns out [rows, heads,
         head size]; rows behind starts[-1] keep what `out` held."""
-        d = self.device
-        out, queries = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
+        index = self.index
+        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
         pages, at = 0, None
         if prefix is not None:
-            at, pages = _whole("prefix", prefix, torch.int32, d), prefix.shape[0]
-        ref = C.byref(queries)
-        key = (0, q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
-        size = self._workspace_bytes(key, lambda n: lib().tcu_paged_attend_workspace(self._ref, ref, pages, max_length, n))
-        work = torch.empty(size, dtype=torch.uint8, device=d) if stream is None else self._on(stream, size)
-        check(lib().tcu_paged_attend(d.index, _stream(stream, d), self._ref, ref, at, pages, max_length, work.data_ptr(), size))
+            at, pages = _whole("prefix", prefix, torch.int32, self.device), len(prefix)
+        key = (q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
+        if self._sized[0] != key:
+            self._size(key, self._lib.tcu_paged_attend_workspace, ref, pages, max_length)
+        size = self._sized[1]
+        work = self._workspace(size, stream)
+        check(self._lib.tcu_paged_attend(index, _stream(stream, index), self._ref, ref, at, pages, max_length, work.data_ptr(), size))
         return out
 
     def attend_sparse(self, q, means, tables, starts, lengths, max_fresh, top, first=1, last=1, scale=None, out=None, pages=None, stream=None):
@@ -233,40 +242,41 @@ class Cache:
         page_means keeps them. Returns (out, pages): pages int32 [rows, KV
         heads, first + last + top], the logical pages read, ascending, -1
         behind them."""
-        d = self.device
+        d, index = self.device, self.index
         self._check_means(means)
-        out, queries = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
-        shape = (q.shape[0], self.kv_heads, first + last + top)
+        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
         if min(first, top) < 0 or last < 1:
             raise _bad(f"first {first} and top {top} must not be negative, last {last} must be at least 1")
+        shape = (q.shape[0], self.kv_heads, first + last + top)
         if pages is None:
-            pages = torch.empty(shape, dtype=torch.int32, device=d)
+            pages = tables.new_empty(shape)
         elif pages.shape != shape or pages.dtype != torch.int32 or pages.device != d or not pages.is_contiguous():
             raise _bad(f"pages must be a contiguous int32 tensor {shape} on {d}")
-        ref = C.byref(queries)
-        key = (1, q.dtype, q.shape, tables.shape, max_fresh, first, last, top)
-        size = self._workspace_bytes(key, lambda n: lib().tcu_paged_attend_sparse_workspace(self._ref, ref, first, last, top, n))
-        work = torch.empty(size, dtype=torch.uint8, device=d) if stream is None else self._on(stream, size)
-        check(lib().tcu_paged_attend_sparse(d.index, _stream(stream, d), self._ref, ref, means.data_ptr(), first, last, top, pages.data_ptr(),
-                                            work.data_ptr(), size))
+        key = (q.dtype, q.shape, tables.shape, max_fresh, first, last, top)
+        if self._sized[0] != key:
+            self._size(key, self._lib.tcu_paged_attend_sparse_workspace, ref, first, last, top)
+        size = self._sized[1]
+        work = self._workspace(size, stream)
+        check(self._lib.tcu_paged_attend_sparse(index, _stream(stream, index), self._ref, ref, means.data_ptr(), first, last, top, pages.data_ptr(),
+                                                work.data_ptr(), size))
         return out, pages
 
-    def _on(self, stream, size):
-        """A workspace that torch's allocator hands out again only behind `stream`."""
-        with torch.cuda.stream(stream):
-            return torch.empty(size, dtype=torch.uint8, device=self.device)
+    def _size(self, key, ask, ref, *counts):
+        """Workspace bytes of a call, kept for the next one of the same shape."""
+        n = C.c_uint64()
+        check(ask(self._ref, ref, *counts, C.byref(n)))
+        self._sized = (key, n.value)
 
-    def _workspace_bytes(self, key, ask):
-        """The size the library asks for; the last answer is kept for calls of the same shape."""
-        if self._sized[0] != key:
-            n = C.c_uint64()
-            check(ask(C.byref(n)))
-            self._sized = (key, n.value)
-        return self._sized[1]
+    def _workspace(self, size, stream):
+        """From torch's allocator, which hands it out again only to work behind this call on its stream."""
+        if stream is None:
+            return self.k.new_empty(size, dtype=torch.uint8)
+        with torch.cuda.stream(stream):
+            return self.k.new_empty(size, dtype=torch.uint8)
 
     def _check_means(self, means):
-        if means.shape != (self.num_pages, self.kv_heads, self.head_dim) or means.dtype != self.k.dtype or means.device != self.device or not means.is_contiguous():
-            raise _bad(f"means must be a contiguous {self.k.dtype} tensor {(self.num_pages, self.kv_heads, self.head_dim)} on {self.device}")
+        if means.shape != self._means or means.dtype is not self.k.dtype or means.device != self.device or not means.is_contiguous():
+            raise _bad(f"means must be a contiguous {self.k.dtype} tensor {tuple(self._means)} on {self.device}")
 
     def _queries(self, q, tables, starts, lengths, max_fresh, scale, out):
         d, hd = self.device, self.head_dim
@@ -275,12 +285,15 @@ class Cache:
         rows, heads, _ = q.shape
         st, le, tb = _whole("starts", starts, torch.int32, d), _whole("lengths", lengths, torch.int32, d), _whole("tables", tables, torch.int32, d, 2)
         n, width = tables.shape
-        if lengths.shape[0] != n or starts.shape[0] != n + 1:
-            raise _bad(f"{n} tables, {lengths.shape[0]} lengths, {starts.shape[0]} starts")
+        if len(lengths) != n or len(starts) != n + 1:
+            raise _bad(f"{n} tables, {len(lengths)} lengths, {len(starts)} starts")
         if out is None:
-            out = torch.empty((rows, heads, hd), dtype=q.dtype, device=d)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != d or out.stride(2) != 1:
-            raise _bad(f"out must be {tuple(q.shape)} of {q.dtype} on {d}, its last dimension contiguous")
-        stride = tables.stride(0) if n > 1 else max(width, tables.stride(0))
-        return out, _lib.PagedQueries(_code("q", q), n, rows, heads, max_fresh, width, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
-                                      out.stride(0), out.stride(1), st, le, tb, stride, 1.0 / math.sqrt(hd) if scale is None else scale)
+            out = q.new_empty((rows, heads, hd))
+            ots, ohs = heads * hd, hd
+        else:
+            if out.shape != q.shape or out.dtype != q.dtype or out.device != d or out.stride(2) != 1:
+                raise _bad(f"out must be {tuple(q.shape)} of {q.dtype} on {d}, its last dimension contiguous")
+            ots, ohs, _ = out.stride()
+        qts, qhs, _ = q.stride()
+        return out, C.byref(_lib.PagedQueries(_code("q", q), n, rows, heads, max_fresh, width, q.data_ptr(), qts, qhs, out.data_ptr(), ots, ohs, st, le, tb,
+                                              tables.stride(0) if n > 1 else width, self._scale if scale is None else scale))
