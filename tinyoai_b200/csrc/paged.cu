@@ -117,25 +117,34 @@ PagedView view_of(const tcu_paged_kv* kv) {
 }
 
 // Queues a kernel that may start while the one before it on the stream
-// drains; every kernel here waits for that one before it reads (paged.cuh).
+// drains (every kernel here waits for that one before it reads, paged.cuh), in
+// clusters of `cluster` CTAs along z.
 template <typename... P, typename... A>
-int launch(const char* name, void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t s, const A&... args) {
+int launch_cluster(const char* name, void (*kern)(P...), dim3 grid, int cluster, int block, size_t smem, cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = (unsigned)cluster;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(TCU_ECUDA, "%s: %s", name, cudaGetErrorString(e));
   }
   return TCU_OK;
+}
+
+template <typename... P, typename... A>
+int launch(const char* name, void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t s, const A&... args) {
+  return launch_cluster(name, kern, grid, 1, block, smem, s, args...);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -170,7 +179,7 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
 
 template <typename TK>
 int launch_means(const MeansArgs& a, cudaStream_t s) {
-  return launch("k_page_means", k_page_means<TK>, dim3((unsigned)ceil_div(a.T, 128), a.kv.kvh), 128, 0, s, a);
+  return launch("k_page_means", k_page_means<TK>, dim3((unsigned)ceil_div(a.T, 32), a.kv.kvh), 128, 0, s, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -178,7 +187,10 @@ int launch_means(const MeansArgs& a, cudaStream_t s) {
 
 struct AttendPlan {
   int prefix_rows = 0, prefix_chunk = 0, prefix_slots = 0, own_rows = 0, own_chunk = 0, own_slots = 0, slots = 0;
-  bool tc = false;  // the prefix on tcgen05
+  bool tc = false;      // the prefix on tcgen05
+  bool cluster = false; // the parts of a row are joined within a cluster
+  int own_begin = 0;
+  int score_per = 64, score_tiles = 0;  // pages of a scoring CTA, and such shares of a table
   PagedTcArgs tc_args{};
   int tc_tiles = 0, tc_parts = 0;
   size_t part_o = 0, part_ml = 0, keys = 0, scores = 0, eps = 0, bytes = 0;  // offsets of the workspace regions, and their size
@@ -191,6 +203,8 @@ struct AttendPlan {
 int chunk_of(int64_t positions, int64_t ctas_per_part, int P) {
   const int64_t want = std::max<int64_t>(1, 4LL * SM_COUNT / std::max<int64_t>(1, ctas_per_part));
   int64_t c = std::max<int64_t>(128, ceil_div(ceil_div(positions, want), 64) * 64);
+  // Up to 4,096 positions: eight parts at most, which a cluster joins.
+  if (positions <= 4096) c = std::max<int64_t>(c, ceil_div(ceil_div(positions, 8), 64) * 64);
   c = std::min<int64_t>(c, std::max<int64_t>(64, (int64_t)(MM_IDS - 2) * P / 64 * 64));
   return (int)std::min<int64_t>(c, 1 << 30);
 }
@@ -262,17 +276,28 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
     p.prefix_rows = rows_per_cta(kv, T * G);
     p.own_rows = rows_per_cta(kv, (int64_t)q->max_fresh * G);
     plan_tc(kv, q, prefix_pages, &p);
+    const int64_t own_tiles = (int64_t)q->requests * ceil_div((int64_t)q->max_fresh * G, p.own_rows);
     if (shared > 0 && !p.tc) {
-      p.prefix_chunk = chunk_of(shared, ceil_div(T * G, p.prefix_rows) * kv->kv_heads, P);
-      p.prefix_slots = (int)ceil_div(shared, p.prefix_chunk);
+      // One kernel over each request's whole history reads the prefix
+      // own_tiles times through L2, a kernel of its own for the prefix
+      // prefix_tiles times, and costs a launch and a join: about 6 us, in
+      // which L2 moves some 32 MB.
+      const int64_t prefix_tiles = ceil_div(T * G, p.prefix_rows), bytes = 2 * shared * kv->kv_heads * kv->head_dim * elem_bytes(kv->dtype);
+      if ((own_tiles - prefix_tiles) * bytes > (32 << 20)) {
+        p.prefix_chunk = chunk_of(shared, prefix_tiles * kv->kv_heads, P);
+        p.prefix_slots = (int)ceil_div(shared, p.prefix_chunk);
+      }
     }
-    const int64_t own = std::max<int64_t>(0, (int64_t)max_length - shared);
-    p.own_chunk = chunk_of(own, (int64_t)q->requests * kv->kv_heads * ceil_div((int64_t)q->max_fresh * G, p.own_rows), P);
+    p.own_begin = p.prefix_slots > 0 ? (int)shared : 0;
+    const int64_t own = std::max<int64_t>(0, (int64_t)max_length - p.own_begin);
+    p.own_chunk = chunk_of(own, own_tiles * kv->kv_heads, P);
     p.own_slots = (int)ceil_div(own, p.own_chunk);
   }
+  // Up to eight parts of one kernel: a cluster joins them.
+  p.cluster = p.prefix_slots == 0 && p.own_slots > 1 && p.own_slots <= 8;
   p.slots = std::max(1, p.prefix_slots + p.own_slots);
   size_t off = 0;
-  const size_t rows = p.slots > 1 || p.tc ? (size_t)T * q->heads : 0;
+  const size_t rows = (p.slots > 1 && !p.cluster) || p.tc ? (size_t)T * q->heads : 0;
   p.part_o = off;
   off += align256(rows * p.slots * kv->head_dim * sizeof(float));
   p.part_ml = off;
@@ -284,7 +309,11 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
     p.scores = off;
     off += align256(lists * q->table_width * sizeof(float));
     p.eps = off;
-    off += align256(lists * ceil_div(q->table_width, SCORE_PAGES) * sizeof(float));
+    // Scoring CTAs: four for each SM where there are few lists, 64 pages at least.
+    const int64_t shares = std::max<int64_t>(1, ceil_div(4 * SM_COUNT, std::max<int64_t>(1, (int64_t)lists)));
+    p.score_per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(q->table_width, shares)), 64) * 64);
+    p.score_tiles = (int)ceil_div(q->table_width, p.score_per);
+    off += align256(lists * p.score_tiles * sizeof(float));
   }
   p.bytes = std::max<size_t>(off, 256);
   return p;
@@ -321,21 +350,21 @@ template <typename TQ, typename TK, int NCH, int R, int SRC>
 int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, R, &tiles);
-  const size_t smem = sizeof(float) * CC_GROUPS * (NCH * 32 + 2);
-  return launch("k_attend_cc", k_attend_cc<TQ, TK, NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), CC_WARPS * 32, smem, s, a, tiles);
+  const size_t smem = sizeof(float) * (CC_GROUPS + (a.cluster ? R : 0)) * (NCH * 32 + 2);
+  return launch_cluster("k_attend_cc", k_attend_cc<TQ, TK, NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, CC_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int NT, int SRC>
 int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, 8 * NT, &tiles);
-  constexpr size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>();
+  const size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(a.cluster);
   constexpr auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
   // Beside the prefix's kernel: with half of the cache as shared memory, which
   // its own four CTAs fill, 256 requests over 32,768 shared positions take 241 us,
   // with the driver's choice 271, with all of it (no cache left for its loads) 282.
-  TRY((prepare_kernel<kern>(smem, SRC == SRC_OWN ? 50 : -1)));
-  return launch("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), MM_WARPS * 32, smem, s, a, tiles);
+  TRY((prepare_kernel<kern>(mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(true), SRC == SRC_OWN ? 50 : -1)));
+  return launch_cluster("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, MM_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int SRC>
@@ -407,7 +436,7 @@ int launch_attend(AttendArgs a, const AttendPlan& p, cudaStream_t s) {
   }
   a.overlap = p.tc;
   TRY((launch_parts<TQ, TK, SRC_OWN>(a, p.own_rows, p.own_slots, s)));
-  if (!p.tc && p.prefix_slots + p.own_slots == 1) return TCU_OK;  // the only part wrote the output
+  if (p.cluster || (!p.tc && p.prefix_slots + p.own_slots == 1)) return TCU_OK;  // the output is written
   return launch("k_attend_join", k_attend_join<TQ, 0>, dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s, a);
 }
 
@@ -442,7 +471,7 @@ int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p,
   }
   TRY(launch("k_page_choose", k_page_choose<TQ, TK>, dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s, a, c));
   TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
-  if (p.own_slots == 1) return TCU_OK;  // the only part wrote the output
+  if (p.cluster || p.own_slots == 1) return TCU_OK;  // the output is written
   return launch("k_attend_join", k_attend_join<TQ, 1>, dim3(queries, (a.H + 3) / 4), 128, 0, s, a);
 }
 
@@ -506,6 +535,8 @@ AttendArgs attend_args(const tcu_paged_kv* kv, const tcu_paged_queries* q, const
   a.prefix_slots = p.prefix_slots;
   a.prefix_chunk = p.prefix_chunk;
   a.own_chunk = p.own_chunk;
+  a.own_begin = p.own_begin;
+  a.cluster = p.cluster;
   return a;
 }
 
@@ -739,7 +770,8 @@ int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv
   c.scores = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.scores);
   c.eps = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + p.eps);
   c.width = q->table_width;
-  c.tiles = (int)ceil_div(q->table_width, SCORE_PAGES);
+  c.per = p.score_per;
+  c.tiles = p.score_tiles;
   c.pages = pages;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (q->dtype == TCU_F32 && kv->dtype == TCU_F32) return launch_sparse<float, float>(a, c, p, s);

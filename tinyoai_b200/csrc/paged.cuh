@@ -448,10 +448,11 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) k_append(AppendArgs a, int 
 
 // ---------------------------------------------------------------------------
 // Page means: for every slot that is the last of its page, the mean key of
-// the page for each KV head, float32 sums rounded once. One warp takes 32
-// slots and one KV head. hd / 8 lanes hold a position's features, eight each;
-// as many positions as the warp has lanes for are read side by side, eight
-// loads in flight a lane. The lanes' sums are added in a fixed order.
+// the page for each KV head, float32 sums rounded once. A CTA takes 32 slots
+// and one KV head and all its warps share a page: hd / 8 lanes hold a
+// position's features, eight each, and the CTA's 128 / (hd / 8) sets of lanes
+// take alternate positions, four loads in flight a lane. The sets' sums are
+// added in a fixed order.
 struct MeansArgs {
   int T;
   const int64_t* slots;
@@ -461,29 +462,29 @@ struct MeansArgs {
 
 template <typename TK>
 __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
-  __shared__ __align__(16) float sums[4][32][8];
-  const int wid = threadIdx.x >> 5, warp = blockIdx.x * 4 + wid, lane = threadIdx.x & 31;
-  const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, rows = 32 / lpr;
-  const int64_t t = (int64_t)warp * 32 + lane;
+  __shared__ __align__(16) float sums[128][8];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, sets = 128 / lpr;
+  const int64_t t = (int64_t)blockIdx.x * 32 + lane;
   pdl_wait();
   int64_t slot = t < a.T ? a.slots[t] : -1;
   if (slot >= (int64_t)a.kv.num_pages * P) slot = -1;
   const int my_page = slot < 0 ? -1 : (int)(slot / P);
-  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - (int64_t)my_page * P == P - 1);
-  const int r0 = lane / lpr, d = (lane - r0 * lpr) * 8;
-  constexpr int U = 8;
+  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - (int64_t)my_page * P == P - 1);  // the same in every warp
+  const int r0 = tid / lpr, d = (tid - r0 * lpr) * 8;
+  constexpr int U = 4;
   while (todo) {
     const int src = __ffs(todo) - 1;
     todo &= todo - 1;
     const int64_t page = __shfl_sync(0xffffffffu, my_page, src);
     const TK* base = reinterpret_cast<const TK*>(a.kv.k) + page * a.kv.sp + (int64_t)g * a.kv.sh + d;
     float s[8] = {};
-    if (r0 < rows) {
-      for (int r = r0; r < P; r += U * rows) {
+    if (r0 < sets) {
+      for (int r = r0; r < P; r += U * sets) {
         Raw8<TK> x[U];
 #pragma unroll
         for (int i = 0; i < U; i++)
-          if (r + i * rows < P) x[i].load(base + (int64_t)(r + i * rows) * a.kv.st); else x[i].zero();
+          if (r + i * sets < P) x[i].load(base + (int64_t)(r + i * sets) * a.kv.st); else x[i].zero();
 #pragma unroll
         for (int i = 0; i < U; i++) {
           float y[8];
@@ -493,18 +494,15 @@ __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
         }
       }
     }
-    __syncwarp();
-    store8(&sums[wid][lane][0], s);
-    __syncwarp();
-    if (lane < lpr) {
-      for (int i = 1; i < rows; i++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) s[e] += sums[wid][lane + i * lpr][e];
-      const float n = (float)P;
-#pragma unroll
-      for (int e = 0; e < 8; e++) s[e] = s[e] / n;
-      store8(reinterpret_cast<TK*>(a.means) + (page * a.kv.kvh + g) * a.kv.hd + d, s);
+    store8(&sums[tid][0], s);
+    __syncthreads();
+    // One feature a thread: the sets' sums in order.
+    for (int f = tid; f < a.kv.hd; f += 128) {
+      float x = 0.f;
+      for (int i = 0; i < min(sets, P); i++) x += sums[i * lpr + (f >> 3)][f & 7];
+      store_as(reinterpret_cast<TK*>(a.means) + (page * a.kv.kvh + g) * a.kv.hd + f, x / (float)P);
     }
+    __syncthreads();
   }
 }
 
@@ -538,6 +536,10 @@ struct AttendArgs {
   float2* part_ml; // [row][slot] (m, l)
   int slots, prefix_slots;
   int prefix_chunk, own_chunk;  // positions per part
+  int own_begin;                // where the requests' own parts begin: behind the prefix, or 0 (all of the history)
+  // 1: a row's parts are a cluster's CTAs, which join them through each
+  // other's shared memory and write the output; nothing goes to part_*.
+  int cluster;
   // Sparse: the pages each (query, KV head) reads (ascending, -1 behind them).
   const int* pages;  // [T][KVH][budget]
   int budget;
@@ -606,8 +608,12 @@ __device__ __forceinline__ int64_t source_at(const AttendArgs& a, const int* ids
     id = table[j];
   } else {
     t = u;
-    if (SRC == SRC_OWN && b >= a.width) return -1;
-    id = ids[b];
+    if (SRC == SRC_OWN && b < a.prefix_pages) {
+      id = a.prefix[b];
+    } else {
+      if (SRC == SRC_OWN && b >= a.width) return -1;
+      id = ids[b];
+    }
   }
   if (id < 0 || id >= a.kv.num_pages) return -1;
   return (int64_t)id * a.kv.sp + (int64_t)r * a.kv.st;
@@ -621,6 +627,60 @@ __device__ __forceinline__ float ex2(float x) {
 
 // 1 / l, 0 for a row that saw nothing; NaN stays NaN.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
+
+// The parts of a cluster's rows, joined: row r of part p is at rows + r * stride
+// (m, l, then hd sums) of the shared memory of the cluster's CTA p. CTA p
+// writes the features p * 4, (p + parts) * 4, ... of every row, each from all
+// parts in part order. Every thread of every CTA of the cluster calls this.
+template <typename TQ, typename RowOut>
+__device__ __forceinline__ void cluster_join(const AttendArgs& a, float* rows, int stride, int count, RowOut row_out) {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  uint32_t rank, parts;
+  asm("mov.u32 %0, %cluster_ctarank;" : "=r"(rank));
+  asm("mov.u32 %0, %cluster_nctarank;" : "=r"(parts));
+  const uint32_t base = smem_u32(rows);
+  const int quads = (a.hd / 4 + (int)parts - 1) / (int)parts;  // of a CTA
+  for (int e = threadIdx.x; e < count * quads; e += blockDim.x) {
+    const int r = e / quads, d = ((e - r * quads) * (int)parts + (int)rank) * 4, row = row_out(r);
+    if (row < 0 || d >= a.hd) continue;
+    const uint32_t at = base + (uint32_t)(r * stride) * 4;
+    float m[8], l[8], mx = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < 8; p++) {
+      m[p] = -INFINITY;
+      l[p] = 0.f;
+      if (p < (int)parts) {
+        uint32_t there;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(p));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(m[p]) : "r"(there));
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(l[p]) : "r"(there + 4));
+      }
+      mx = fmaxf(mx, m[p]);
+    }
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float ls = 0.f;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < 8; p++)
+      if (p < (int)parts) {
+        const float w = ex2(m[p] - ref);
+        uint32_t there;
+        float x[4];
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at + 8 + d * 4), "r"(p));
+#pragma unroll
+        for (int i = 0; i < 4; i++) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x[i]) : "r"(there + 4 * i));
+        ls = fmaf(l[p], w, ls);
+        s.x = fmaf(x[0], w, s.x);
+        s.y = fmaf(x[1], w, s.y);
+        s.z = fmaf(x[2], w, s.z);
+        s.w = fmaf(x[3], w, s.w);
+      }
+    const float inv = inverse_sum(ls);
+    store4(reinterpret_cast<TQ*>(a.out) + (int64_t)(row / a.H) * a.o_ts + (int64_t)(row % a.H) * a.o_hs + d, make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv));
+  }
+  // Nobody leaves while its shared memory is read.
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // CUDA-core parts. A warp holds four groups of eight lanes; a group takes
 // every fourth position of its warp's share and keeps a softmax state of its
@@ -672,7 +732,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
       most = max(most, q.pos);
     }
   }
-  if (token0 < 0) return;
+  if (token0 < 0) return;  // the same for all of a cluster
   const int prefix_end = a.prefix_pages * a.kv.P;
   int u0, u1;
   const int* ids;
@@ -682,7 +742,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     u1 = min(min(u0 + a.prefix_chunk, prefix_end), most + 1);
     ids = a.prefix;
   } else if (SRC == SRC_OWN) {
-    u0 = prefix_end + part * a.own_chunk;
+    u0 = a.own_begin + part * a.own_chunk;
     u1 = min(u0 + a.own_chunk, most + 1);
     ids = a.tables + (int64_t)request * a.table_stride;
   } else {
@@ -691,7 +751,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     ids = a.pages + ((int64_t)token0 * a.KVH + g) * a.budget;
     table = a.tables + (int64_t)(request / a.max_fresh) * a.table_stride;
   }
-  if (SRC == SRC_OWN && u0 >= u1 && !(part == 0 && a.slots == 1)) return;  // k_attend_join counts the parts by the same rule
+  if (SRC == SRC_OWN && u0 >= u1 && !(part == 0 && a.slots == 1) && !a.cluster) return;  // k_attend_join counts the parts by the same rule
 
   float q[R][NCH][4], o[R][NCH][4], m[R], l[R];
 #pragma unroll
@@ -812,22 +872,40 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     const bool direct = a.slots == 1;  // the only part: the output itself
     const float inv = inverse_sum(ls);
     TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)(row_out[r] / a.H) * a.o_ts + (int64_t)(row_out[r] % a.H) * a.o_hs;
+    float* mine = cc_smem + CC_GROUPS * (width + 2) + r * (width + 2);  // this part of the row, for its cluster
     for (int d = threadIdx.x; d < hd; d += CC_WARPS * 32) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < CC_GROUPS; i++) s = fmaf(so[i * width + d], w[i], s);
-      if (direct)
+      if (a.cluster)
+        mine[2 + d] = s;
+      else if (direct)
         store_as(out + d, s * inv);
       else
         a.part_o[slot * hd + d] = s;
     }
-    if (threadIdx.x == 0 && !direct) a.part_ml[slot] = make_float2(mx, ls);
+    if (threadIdx.x == 0) {
+      if (a.cluster)
+        mine[0] = mx, mine[1] = ls;
+      else if (!direct)
+        a.part_ml[slot] = make_float2(mx, ls);
+    }
+  }
+  if (a.cluster) {
+    float* rows = cc_smem + CC_GROUPS * (width + 2);
+    cluster_join<TQ>(a, rows, width + 2, R, [&](int r) {
+      int x = -1;
+#pragma unroll
+      for (int i = 0; i < R; i++)
+        if (i == r) x = row_out[i];
+      return x;
+    });
   }
 }
 
 // Parts of a row with its last position pos: the prefix's, then its own.
 __device__ __forceinline__ int own_parts(const AttendArgs& a, int pos) {
-  const int n = pos + 1 - a.prefix_pages * a.kv.P;
+  const int n = pos + 1 - a.own_begin;
   return n <= 0 ? 0 : (n + a.own_chunk - 1) / a.own_chunk;
 }
 
@@ -904,11 +982,9 @@ struct ChooseArgs {
   float* scores;             // [T][KVH][width]; NaN: no page, or a NaN score
   float* eps;                // [T][KVH][tiles]
   unsigned long long* keys;  // [T][KVH][width], of the pages scored again
-  int width, tiles;
+  int width, tiles, per;     // a scoring CTA takes `per` pages, tiles of them cover a table
   int* pages;                // [T][KVH][budget]
 };
-
-constexpr int SCORE_PAGES = 128;  // pages of a scoring CTA
 
 // c above: (2 hd + 32) steps of 2^-23 cover hd products and additions (the
 // tensor core's may truncate) and the 22-bit split of float32 queries.
@@ -937,7 +1013,7 @@ __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs
   if (q.token < 0) return;
   const int g = blockIdx.y, hd = a.hd;
   const Candidates cand = candidates_of(a, c, q.pos);
-  const int lo = max(cand.lo, (int)blockIdx.z * SCORE_PAGES), hi = min(cand.hi, (int)blockIdx.z * SCORE_PAGES + SCORE_PAGES);
+  const int lo = max(cand.lo, (int)blockIdx.z * c.per), hi = min(cand.hi, (int)blockIdx.z * c.per + c.per);
   if (lo >= hi || cand.hi - cand.lo <= c.top) return;  // nothing to choose here
   for (int e = threadIdx.x * 4; e < a.G * hd; e += 128 * 4) {
     const int h = e / hd, d = e - h * hd;
@@ -947,7 +1023,7 @@ __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs
   const int* table = a.tables + (int64_t)q.request * a.table_stride;
   const int l8 = threadIdx.x & 7;
   float most = 0.f;
-  for (int b0 = blockIdx.z * SCORE_PAGES; b0 < hi; b0 += 16) {
+  for (int b0 = blockIdx.z * c.per; b0 < hi; b0 += 16) {
     const int b = b0 + (threadIdx.x >> 3);
     const int id = b >= lo && b < hi ? table[b] : -1;
     const bool on = id >= 0 && id < a.kv.num_pages;
@@ -998,39 +1074,68 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 
 constexpr int CHOOSE_THREADS = 256;
 constexpr int CHOOSE_CACHE = 8192;  // scores a CTA keeps in shared memory; others are read again from L2
+constexpr int CHOOSE_OPEN = 64;     // pages at the border that are ordered at once
+constexpr int RADIX_BITS = 11, RADIX_BINS = 1 << RADIX_BITS, BINS_PER = RADIX_BINS / CHOOSE_THREADS;
 
-// The digit d whose bins above it hold fewer than `want` entries and with it
-// at least `want`, from a histogram of 256 bins (one per thread), and how many
-// are still wanted within it. Every thread returns the same.
-__device__ __forceinline__ void pick_digit(int count, int want, int* warp_sums, int* result, int& digit, int& left) {
+struct ChooseShared {
+  int hist[RADIX_BINS];
+  int sums[CHOOSE_THREADS / 32], ties_of[CHOOSE_THREADS / 32], result[2];
+  int sure, open;
+  uint32_t eps;
+  int list[CHOOSE_OPEN];
+  unsigned long long key[CHOOSE_OPEN];
+};
+
+// The want-th largest key (1 <= want <= number of keys) among the entries that
+// `each(f)` calls f(key) for on every thread, by digits of 11 bits from the
+// highest on; `want` becomes how many of that key itself are wanted. Eleven
+// bits: scores share their exponents, and eight would put most of them on a
+// few bins, where the counts' updates queue up.
+template <typename Key, typename Each>
+__device__ __forceinline__ Key radix_select(ChooseShared& sh, int bits, int& want, Each each) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // Sums of the bins from this one up.
-  int up = count;
+  Key prefix = 0;
+  int done = 0;  // bits of the prefix
+  while (done < bits) {
+    const int n = min(RADIX_BITS, bits - done), shift = bits - done - n;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int x = __shfl_down_sync(0xffffffffu, up, o);
-    if (lane + o < 32) up += x;
+    for (int i = 0; i < BINS_PER; i++) sh.hist[tid + i * CHOOSE_THREADS] = 0;
+    __syncthreads();
+    each([&](Key k) {
+      if (done == 0 || (k >> (shift + n)) == (prefix >> (shift + n))) atomicAdd(&sh.hist[(int)((k >> shift) & ((Key(1) << n) - 1))], 1);
+    });
+    __syncthreads();
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < BINS_PER; i++) mine += sh.hist[tid * BINS_PER + i];
+    int up = mine;  // entries in this thread's bins and above
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_down_sync(0xffffffffu, up, o);
+      if (lane + o < 32) up += x;
+    }
+    if (lane == 0) sh.sums[warp] = up;
+    __syncthreads();
+    for (int w = warp + 1; w < CHOOSE_THREADS / 32; w++) up += sh.sums[w];
+    if (up >= want && up - mine < want) {  // one thread
+      int left = want - (up - mine), d = BINS_PER - 1;
+      while (sh.hist[tid * BINS_PER + d] < left) left -= sh.hist[tid * BINS_PER + d--];
+      sh.result[0] = tid * BINS_PER + d;
+      sh.result[1] = left;
+    }
+    __syncthreads();
+    prefix |= (Key)sh.result[0] << shift;
+    want = sh.result[1];
+    done += n;
   }
-  if (lane == 0) warp_sums[warp] = up;
-  __syncthreads();
-  for (int w = warp + 1; w < 8; w++) up += warp_sums[w];
-  if (up >= want && up - count < want) {  // one thread
-    result[0] = tid;
-    result[1] = want - (up - count);
-  }
-  __syncthreads();
-  digit = result[0];
-  left = result[1];
+  return prefix;
 }
 
 // One CTA per (query, KV head): the top-th key by radix selection, then the
 // chosen pages in ascending order. grid: x = request * max_fresh + query, y = KV head.
 template <typename TQ, typename TK>
 __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, ChooseArgs c) {
-  __shared__ int hist[256];
-  __shared__ int sums[CHOOSE_THREADS / 32], result[2], ties_of[CHOOSE_THREADS / 32];
-  __shared__ int s_sure, s_open;
-  __shared__ uint32_t s_eps;
+  __shared__ ChooseShared sh;
   extern __shared__ float cache[];  // min(width, CHOOSE_CACHE)
   pdl_wait();
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
@@ -1045,38 +1150,28 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
   unsigned long long* keys = c.keys + at * c.width;
   const int kept = min(hi, min(c.width, CHOOSE_CACHE));
   auto score = [&](int b) { return b < kept ? cache[b] : scores[b]; };
-  float in_above = INFINITY, out_below = INFINITY;  // certain: score > in_above; not certain: >= out_below (and NaN, when eps is not finite)
+  float in_above = INFINITY, out_below = INFINITY;  // certain: a score above, certainly not: one below
   bool every = false;                               // all candidates are open
-  unsigned long long thr = 0;                       // open pages with a larger key are taken,
-  int ties = 0;                                     // and this many with this one
+  auto is_open = [&](float x) { return every || (x <= in_above && x >= out_below); };
+  unsigned long long thr = 0;  // open pages with a larger key are taken (~0: all open pages),
+  int ties = 0;                // and this many with this one
   if (choose) {
     if (tid == 0) {
-      s_eps = 0;
-      s_sure = s_open = 0;
+      sh.eps = 0;
+      sh.sure = sh.open = 0;
     }
     for (int b = lo + tid; b < kept; b += CHOOSE_THREADS) cache[b] = scores[b];
-    __syncthreads();
     uint32_t e = 0;
-    for (int i = lo / SCORE_PAGES + tid; i <= (hi - 1) / SCORE_PAGES; i += CHOOSE_THREADS) e = max(e, __float_as_uint(c.eps[at * c.tiles + i]) & 0x7fffffffu);
+    for (int i = lo / c.per + tid; i <= (hi - 1) / c.per; i += CHOOSE_THREADS) e = max(e, __float_as_uint(c.eps[at * c.tiles + i]) & 0x7fffffffu);
     e = __reduce_max_sync(0xffffffffu, e);
-    if (lane == 0 && e) atomicMax(&s_eps, e);
+    __syncthreads();
+    if (lane == 0 && e) atomicMax(&sh.eps, e);
     // The top-th largest float32 score.
-    uint32_t prefix = 0;
     int want = c.top;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      hist[tid] = 0;
-      __syncthreads();
-      for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
-        const uint32_t k = score_key32(score(b));
-        if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
-      }
-      __syncthreads();
-      int digit, left;
-      pick_digit(hist[tid], want, sums, result, digit, left);
-      prefix |= (uint32_t)digit << shift;
-      want = left;
-    }
-    const float eps = __uint_as_float(s_eps);
+    const uint32_t prefix = radix_select<uint32_t>(sh, 32, want, [&](auto f) {
+      for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) f(score_key32(score(b)));
+    });
+    const float eps = __uint_as_float(sh.eps);
     const float edge = float_from_order_key(prefix);
     every = !(eps < INFINITY) || prefix <= 1u || !(fabsf(edge) < INFINITY);
     if (!every) {
@@ -1086,77 +1181,91 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
       out_below = edge - r;
     }
     // Pages certainly in, and pages that float64 has to order.
-    int sure = 0, open = 0;
+    int sure = 0;
     for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
       const float x = score(b);
-      if (!every && x > in_above)
-        sure++;
-      else if (every || x >= out_below)
-        open++;
+      if (!every && x > in_above) sure++;
+      if (is_open(x)) {
+        const int i = atomicAdd(&sh.open, 1);
+        if (i < CHOOSE_OPEN) sh.list[i] = b;
+      }
     }
     sure = __reduce_add_sync(0xffffffffu, sure);
-    open = __reduce_add_sync(0xffffffffu, open);
-    if (lane == 0) {
-      atomicAdd(&s_sure, sure);
-      atomicAdd(&s_open, open);
-    }
+    if (lane == 0 && sure) atomicAdd(&sh.sure, sure);
     __syncthreads();
-    want = c.top - s_sure;
-    if (s_open == want) {
+    want = c.top - sh.sure;
+    const int open = sh.open;
+    if (open == want) {
       ties = want;
-      thr = ~0ull;  // all open pages: see `taken`
+      thr = ~0ull;
     } else {
-      // Float64 keys of the open pages, a warp each.
+      // Float64 keys, a warp a page.
       const int* table = a.tables + (int64_t)q.request * a.table_stride;
-      for (int b0 = lo + warp * 32; b0 < hi; b0 += CHOOSE_THREADS) {
-        const int mine = b0 + lane;
-        const float x = mine < hi ? score(mine) : 0.f;
-        uint32_t todo = __ballot_sync(0xffffffffu, mine < hi && (every || (x <= in_above && x >= out_below)));
-        while (todo) {
-          const int b = b0 + __ffs(todo) - 1;
-          todo &= todo - 1;
-          const int id = table[b];
-          unsigned long long key = 0;
-          if (id >= 0 && id < a.kv.num_pages) {
-            const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)id * a.KVH + g) * a.hd;
-            double best = 0.0;
-            for (int h = 0; h < a.G; h++) {
-              const TQ* qp = reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs;
-              double s = 0.0;
-              for (int d = lane * 4; d < a.hd; d += 128) {
-                const float4 u = load4(qp + d), v = load4(mp + d);
-                s = fma((double)u.x, (double)v.x, s);
-                s = fma((double)u.y, (double)v.y, s);
-                s = fma((double)u.z, (double)v.z, s);
-                s = fma((double)u.w, (double)v.w, s);
-              }
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-              // The largest of the heads; a NaN makes the page NaN.
-              if (h == 0 || (best == best && (s > best || !(s == s)))) best = s;
-            }
-            key = score_key(best);
+      auto exact_key = [&](int b) {
+        const int id = table[b];
+        if (id < 0 || id >= a.kv.num_pages) return 0ull;
+        const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)id * a.KVH + g) * a.hd;
+        double best = 0.0;
+        for (int h = 0; h < a.G; h++) {
+          const TQ* qp = reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs;
+          double s = 0.0;
+          for (int d = lane * 4; d < a.hd; d += 128) {
+            const float4 u = load4(qp + d), v = load4(mp + d);
+            s = fma((double)u.x, (double)v.x, s);
+            s = fma((double)u.y, (double)v.y, s);
+            s = fma((double)u.z, (double)v.z, s);
+            s = fma((double)u.w, (double)v.w, s);
           }
-          if (lane == 0) keys[b] = key;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+          // The largest of the heads; a NaN makes the page NaN.
+          if (h == 0 || (best == best && (s > best || !(s == s)))) best = s;
         }
-      }
-      __syncthreads();
-      for (int shift = 56; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
-          const float x = score(b);
-          if (!(every || (x <= in_above && x >= out_below))) continue;
-          const unsigned long long k = keys[b];
-          if (shift == 56 || (k >> (shift + 8)) == (thr >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        return score_key(best);
+      };
+      if (open <= CHOOSE_OPEN) {  // a few pages at the border: each counts those above it
+        for (int i = warp; i < open; i += CHOOSE_THREADS / 32) {
+          const int b = sh.list[i];
+          const unsigned long long k = exact_key(b);
+          if (lane == 0) {
+            sh.key[i] = k;
+            keys[b] = k;
+          }
         }
         __syncthreads();
-        int digit, left;
-        pick_digit(hist[tid], want, sums, result, digit, left);
-        thr |= (unsigned long long)digit << shift;
-        want = left;
+        if (tid < open) {
+          const unsigned long long k = sh.key[tid];
+          int above = 0, same = 0;
+          for (int i = 0; i < open; i++) {
+            above += sh.key[i] > k;
+            same += sh.key[i] == k;
+          }
+          if (above < want && above + same >= want) {  // this key is the border; equal ones write the same
+            sh.result[0] = tid;
+            sh.result[1] = want - above;
+          }
+        }
+        __syncthreads();
+        thr = sh.key[sh.result[0]];
+        ties = sh.result[1];
+      } else {
+        for (int b0 = lo + warp * 32; b0 < hi; b0 += CHOOSE_THREADS) {
+          const int mine = b0 + lane;
+          uint32_t todo = __ballot_sync(0xffffffffu, mine < hi && is_open(score(min(mine, hi - 1))));
+          while (todo) {
+            const int b = b0 + __ffs(todo) - 1;
+            todo &= todo - 1;
+            const unsigned long long k = exact_key(b);
+            if (lane == 0) keys[b] = k;
+          }
+        }
+        __syncthreads();
+        thr = radix_select<unsigned long long>(sh, 64, want, [&](auto f) {
+          for (int b = lo + tid; b < hi; b += CHOOSE_THREADS)
+            if (is_open(score(b))) f(keys[b]);
+        });
+        ties = want;
       }
-      ties = want;
     }
   }
   const bool keyed = choose && thr != ~0ull;
@@ -1167,7 +1276,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
     bool take = b < npages && (!inside || all), tie = false;
     if (inside && choose) {
       const float x = score(b);
-      const bool open = every || (x <= in_above && x >= out_below);
+      const bool open = is_open(x);
       const unsigned long long k = open && keyed ? keys[b] : 0;
       take = open ? !keyed || k > thr : x > in_above;
       tie = open && keyed && k == thr;
@@ -1175,22 +1284,22 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
     int before = tied;
     if (keyed) {  // ties go to the lower pages
       const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-      if (lane == 0) ties_of[warp] = __popc(tb);
+      if (lane == 0) sh.ties_of[warp] = __popc(tb);
       __syncthreads();
       before += __popc(tb & ((1u << lane) - 1));
       for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-        if (w < warp) before += ties_of[w];
-        tied += ties_of[w];
+        if (w < warp) before += sh.ties_of[w];
+        tied += sh.ties_of[w];
       }
     }
     take = take || (tie && before < ties);
     const uint32_t kb = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) sums[warp] = __popc(kb);
+    if (lane == 0) sh.sums[warp] = __popc(kb);
     __syncthreads();
     int to = done + __popc(kb & ((1u << lane) - 1)), total = 0;
     for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-      if (w < warp) to += sums[w];
-      total += sums[w];
+      if (w < warp) to += sh.sums[w];
+      total += sh.sums[w];
     }
     if (take && to < a.budget) out[to] = b;
     done += total;

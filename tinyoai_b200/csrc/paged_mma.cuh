@@ -57,10 +57,11 @@ constexpr int MM_IDS = 1024;  // page ids of a part, copied to shared memory (a 
 
 // Shared memory: the queries [PIECES][8 NT columns][HD + 32] 16-bit values (the pad puts
 // the two rows a quarter warp reads on different banks), then, when the loop
-// is over, the warps' outputs [MM_WARPS][8 NT][HD + 4] float32 and their (m, l).
+// is over, the warps' outputs [MM_WARPS][8 NT][HD + 4] float32 and their (m, l),
+// and the CTA's joint rows [8 NT][HD + 2] where a cluster joins them.
 template <int HD, int NT, int PIECES>
-constexpr size_t mm_smem() {
-  const size_t q = (size_t)PIECES * 8 * NT * (HD + 32) * 2, o = (size_t)MM_WARPS * 8 * NT * (HD + 4 + 2) * 4;
+constexpr size_t mm_smem(bool cluster) {
+  const size_t q = (size_t)PIECES * 8 * NT * (HD + 32) * 2, o = (size_t)(MM_WARPS * (HD + 4 + 2) + (cluster ? HD + 2 : 0)) * 8 * NT * 4;
   return q > o ? q : o;
 }
 
@@ -158,9 +159,9 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
     u0 = part * a.prefix_chunk;
     u1 = min(min(u0 + a.prefix_chunk, prefix_end), most + 1);
   } else if (SRC == SRC_OWN) {
-    u0 = prefix_end + part * a.own_chunk;
+    u0 = a.own_begin + part * a.own_chunk;
     u1 = min(u0 + a.own_chunk, most + 1);
-    if (u0 >= u1 && !(part == 0 && a.slots == 1)) return;  // k_attend_join counts the parts by the same rule
+    if (u0 >= u1 && !(part == 0 && a.slots == 1) && !a.cluster) return;  // k_attend_join counts the parts by the same rule
   } else {
     u0 = part * a.own_chunk;
     u1 = min(u0 + a.own_chunk, a.budget * a.kv.P);
@@ -184,7 +185,9 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
     } else {
       const int* ids = SRC == SRC_PREFIX ? a.prefix : a.tables + (int64_t)request * a.table_stride;
       for (int e = tid; e < nb; e += MM_WARPS * 32) {
-        int id = SRC == SRC_PREFIX || b0 + e < a.width ? ids[b0 + e] : -1;
+        const int b = b0 + e;
+        int id = SRC == SRC_PREFIX || b < a.width ? ids[b] : -1;
+        if (SRC == SRC_OWN && b < a.prefix_pages) id = a.prefix[b];
         if (id >= a.kv.num_pages) id = -1;
         s_ids[e] = id;
       }
@@ -384,6 +387,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
     }
   __syncthreads();
   const bool direct = a.slots == 1;  // the only part: the output itself
+  float* rows = so + MM_WARPS * COLS * (OS + 2);  // this part of the rows, for its cluster
   for (int e = tid; e < COLS * (HD / 4); e += MM_WARPS * 32) {
     const int col = e / (HD / 4), d = (e % (HD / 4)) * 4, row = s_row[col];
     if (row < 0 || d >= hd) continue;
@@ -404,7 +408,14 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
       x.z = fmaf(y.z, f, x.z);
       x.w = fmaf(y.w, f, x.w);
     }
-    if (direct) {
+    if (a.cluster) {
+      float* mine = rows + col * (HD + 2);
+      mine[2 + d] = x.x;
+      mine[3 + d] = x.y;
+      mine[4 + d] = x.z;
+      mine[5 + d] = x.w;
+      if (d == 0) mine[0] = mx, mine[1] = ls;
+    } else if (direct) {
       const float inv = inverse_sum(ls);
       TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)(row / a.H) * a.o_ts + (int64_t)(row % a.H) * a.o_hs + d;
       store4(out, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
@@ -414,6 +425,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
       if (d == 0) a.part_ml[slot] = make_float2(mx, ls);
     }
   }
+  if (a.cluster) cluster_join<TQ>(a, rows, HD + 2, COLS, [&](int r) { return s_row[r]; });
 }
 
 template <typename TQ, typename TK, int HD, int NT, int SRC>
@@ -428,7 +440,7 @@ __global__ void __launch_bounds__(MM_WARPS * 32, NT == 1 && HD <= 128 ? 4 : NT =
 // the error bound; both cost nothing beside the means' bytes.
 // grid: x = request * max_fresh + query, y = KV head, z = page tile.
 template <typename TQ, typename TK, int HD>
-__global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a, ChooseArgs c) {
+__global__ void __launch_bounds__(MM_WARPS * 32, HD <= 128 ? 4 : 2) k_page_scores_mma(AttendArgs a, ChooseArgs c) {
   constexpr int PIECES = sizeof(TQ) == 4 ? 2 : 1;
   constexpr int KG = (HD + 31) / 32, QS = HD + 32;
   extern __shared__ __align__(16) uint8_t mm_mem[];  // [PIECES][groups of 8][HD + 32]
@@ -442,34 +454,45 @@ __global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a,
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = lane >> 2, cc = lane & 3;
   const int g = blockIdx.y, hd = a.hd, groups = (a.G + 7) / 8;
   const Candidates cand = candidates_of(a, c, q.pos);
-  const int lo = max(cand.lo, (int)blockIdx.z * SCORE_PAGES), hi = min(cand.hi, (int)blockIdx.z * SCORE_PAGES + SCORE_PAGES);
+  const int lo = max(cand.lo, (int)blockIdx.z * c.per), hi = min(cand.hi, (int)blockIdx.z * c.per + c.per);
   if (lo >= hi || cand.hi - cand.lo <= c.top) return;  // nothing to choose here
-  // The means of this warp's pages, both tiles' loads in flight while the queries come.
-  constexpr int TILES = SCORE_PAGES / (16 * MM_WARPS);
-  uint4 kx[TILES][2][KG];
-  bool on[TILES][2];
   const int* table = a.tables + (int64_t)q.request * a.table_stride;
-#pragma unroll
-  for (int t = 0; t < TILES; t++)
+  // A warp takes every fourth tile of 16 pages; the next tile's means are on
+  // their way while it works on one, and the ids of the one after that.
+  constexpr int STEP = 16 * MM_WARPS;
+  auto ids = [&](int b0, int (&id)[2]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-      const int b = blockIdx.z * SCORE_PAGES + (t * MM_WARPS + warp) * 16 + r + 8 * i;
-      const int id = b >= lo && b < hi ? table[b] : -1;
-      on[t][i] = id >= 0 && id < a.kv.num_pages;
-      const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)(on[t][i] ? id : 0) * a.KVH + g) * hd;
+      const int b = b0 + r + 8 * i;
+      id[i] = b >= lo && b < hi ? table[b] : -1;
+      if (id[i] >= a.kv.num_pages) id[i] = -1;
+    }
+  };
+  auto means = [&](const int (&id)[2], uint4 (&x)[2][KG]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)max(id[i], 0) * a.KVH + g) * hd;
 #pragma unroll
       for (int k = 0; k < KG; k++) {
         const int d = k * 32 + cc * 8;
-        kx[t][i][k] = on[t][i] && d < hd ? ld_stream16(mp + d) : make_uint4(0, 0, 0, 0);
+        x[i][k] = id[i] >= 0 && d < hd ? ld_stream16(mp + d) : make_uint4(0, 0, 0, 0);
       }
     }
+  };
+  const int first = blockIdx.z * c.per + warp * 16;
+  int id[2], id_next[2], id_after[2];
+  uint4 kx[2][KG], kn[2][KG];
+  ids(first, id);
+  ids(first + STEP, id_next);
+  means(id, kx);
   if (tid < groups * 8) s_row[tid] = tid < a.G ? q.token * a.H + g * a.G + tid : -1;
   __syncthreads();
   mm_load_queries<TQ, TK, HD, PIECES>(a, qs, s_row, s_scale, groups * 8, 1.f);
   __syncthreads();
   float most = 0.f;
-#pragma unroll
-  for (int t = 0; t < TILES; t++) {
+  for (int b0 = first; b0 < hi; b0 += STEP) {
+    means(id_next, kn);
+    ids(b0 + 2 * STEP, id_after);
     float best[2] = {-INFINITY, -INFINITY};
     uint32_t nan = 0;
     for (int n = 0; n < groups; n++) {
@@ -479,7 +502,7 @@ __global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a,
 #pragma unroll
         for (int p = 0; p < PIECES; p++) {
           const uint4 y = *reinterpret_cast<const uint4*>(qs + (p * groups * 8 + n * 8 + r) * QS + k * 32 + cc * 8);
-          const uint4 u = kx[t][0][k], v = kx[t][1][k];
+          const uint4 u = kx[0][k], v = kx[1][k];
           constexpr uint32_t M = 0x7fff7fffu;
           mma16816<TK>(s, u.x, v.x, u.y, v.y, y.x, y.y);
           mma16816<TK>(s, u.z, v.z, u.w, v.w, y.z, y.w);
@@ -504,8 +527,15 @@ __global__ void __launch_bounds__(MM_WARPS * 32) k_page_scores_mma(AttendArgs a,
         best[i] = fmaxf(best[i], __shfl_xor_sync(0xffffffffu, best[i], o));
         nan |= __shfl_xor_sync(0xffffffffu, nan, o);
       }
-      const int b = blockIdx.z * SCORE_PAGES + (t * MM_WARPS + warp) * 16 + r + 8 * i;
-      if (cc == 0 && b >= lo && b < hi) c.scores[((int64_t)q.token * a.KVH + g) * c.width + b] = on[t][i] && !(nan >> i & 1) ? best[i] : NAN;
+      const int b = b0 + r + 8 * i;
+      if (cc == 0 && b >= lo && b < hi) c.scores[((int64_t)q.token * a.KVH + g) * c.width + b] = id[i] >= 0 && !(nan >> i & 1) ? best[i] : NAN;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      id[i] = id_next[i];
+      id_next[i] = id_after[i];
+#pragma unroll
+      for (int k = 0; k < KG; k++) kx[i][k] = kn[i][k];
     }
   }
   const uint32_t w = __reduce_max_sync(0xffffffffu, __float_as_uint(most) & 0x7fffffffu);
