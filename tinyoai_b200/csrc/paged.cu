@@ -158,12 +158,14 @@ template <typename TQ, typename TK>
 int launch_append(const AppendArgs& a, cudaStream_t s) {
   const int heads = a.H + 2 * a.KVH;
   auto go = [&](auto kern, int lph) {
-    // A CTA takes all heads of a token when there are tokens enough to fill
-    // the GPU twice over, otherwise as many as its groups of lanes hold at once.
+    // A CTA takes all heads of a token where there are tokens enough to fill
+    // the GPU, otherwise as many as its groups of lanes hold at once; three
+    // CTAs an SM go through the tokens.
     const int groups = APPEND_THREADS / lph;
     const int64_t shares = std::max<int64_t>(1, std::min<int64_t>(ceil_div(heads, groups), ceil_div(8 * SM_COUNT, a.T)));
     const int per = (int)(ceil_div(ceil_div(heads, shares), groups) * groups);
-    return launch("k_append", kern, dim3((unsigned)a.T, (unsigned)ceil_div(heads, per)), APPEND_THREADS, 0, s, a, per);
+    const int64_t y = ceil_div(heads, per), x = std::min<int64_t>(a.T, std::max<int64_t>(1, 3 * SM_COUNT / y));
+    return launch("k_append", kern, dim3((unsigned)x, (unsigned)y), APPEND_THREADS, 0, s, a, per);
   };
   auto pick = [&](auto turn) {
     constexpr int TURN = decltype(turn)::value;
@@ -179,7 +181,9 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
 
 template <typename TK>
 int launch_means(const MeansArgs& a, cudaStream_t s) {
-  return launch("k_page_means", k_page_means<TK>, dim3((unsigned)ceil_div(a.T, 32), a.kv.kvh), 128, 0, s, a);
+  if (ceil_div(a.T, 128) * a.kv.kvh < 2 * SM_COUNT)
+    return launch("k_page_means", k_page_means<TK, 4>, dim3((unsigned)ceil_div(a.T, 32), a.kv.kvh), 128, 0, s, a);
+  return launch("k_page_means", k_page_means<TK, 1>, dim3((unsigned)ceil_div(a.T, 128), a.kv.kvh), 128, 0, s, a);
 }
 
 // ---------------------------------------------------------------------------
@@ -657,7 +661,7 @@ int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32
   TRY(check_ptr("q_out", q_out, device, 16));
   TRY(check_ptr("positions", positions, device, 4));
   TRY(check_ptr("slots", slots, device, 8));
-  if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 8));
+  if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 16));
   if (a.norm) {
     TRY(check_ptr("q_weight", a.qw, device, 16));
     TRY(check_ptr("k_weight", a.kw, device, 16));

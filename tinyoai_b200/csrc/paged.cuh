@@ -278,8 +278,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
 // lanes hold a head, eight values each, and all heads of a group of lanes
 // that the CTA has (three at a time, two of float32) are loaded before the
 // token's position and slot are known. A lane has the same features of every
-// head, so it keeps their cosines and sines in registers; the partner of a
-// rotary pair comes from another lane (through shared memory where pairs do
+// head, so it keeps their cosines and sines in registers (read straight from
+// the table, 64 bytes a lane apart, they cost more of L1 than the values do).
+// The partner of a rotary pair comes from another lane (through shared memory where pairs do
 // not fall on whole lanes).
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
@@ -307,6 +308,7 @@ template <typename T>
 struct Raw8 {
   uint4 v;
   __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void stream(const T* p) { v = ld_stream16(p); }  // read once, and not moved among other such loads
   __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     unpack2(T(), v.x, x[0], x[1]);
@@ -322,6 +324,11 @@ struct Raw8<float> {
     a = load4(p);
     b = load4(p + 4);
   }
+  __device__ __forceinline__ void stream(const float* p) {
+    const uint4 u = ld_stream16(p), w = ld_stream16(p + 4);
+    a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+    b = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
+  }
   __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
@@ -331,116 +338,147 @@ struct Raw8<float> {
 // How a rotary pair's other value is found.
 enum { TURN_NONE = 0, TURN_LANES = 1, TURN_OWN = 2, TURN_SHARED = 3 };
 
-// grid: x = token, y = share of the heads (heads_per_cta of them).
+// grid: x = tokens x, x + gridDim.x, ...; y = share of the heads (heads_per_cta of them).
 template <typename TQ, typename TK, int LPH, int TURN>
-__global__ void __launch_bounds__(APPEND_THREADS, 4) k_append(AppendArgs a, int heads_per_cta) {
+__global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int heads_per_cta) {
   constexpr int GROUPS = APPEND_THREADS / LPH;
   constexpr int APPEND_HEADS = sizeof(TQ) == 4 ? 2 : 3;  // heads of a group of lanes in flight (64 registers)
   __shared__ __align__(16) float stage[TURN == TURN_SHARED ? GROUPS : 1][LPH * 8 + 4];
+  __shared__ float4 turn[TURN == TURN_LANES ? APPEND_THREADS / 32 : 1][64];
   const int grp = threadIdx.x / LPH, lane = threadIdx.x % LPH;
-  const int t = blockIdx.x, heads = a.H + 2 * a.KVH;
+  const int heads = a.H + 2 * a.KVH;
   const int h0 = blockIdx.y * heads_per_cta, h1 = min(heads, h0 + heads_per_cta);
   const int d = lane * 8;
   const bool in = d < a.hd;
-  const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + d;
+  const float inv = 1.f / (float)a.hd;
   pdl_wait();
-  Raw8<TQ> raw[APPEND_HEADS];
-  auto fetch = [&](int hb) {
+  Raw8<TQ> raw[APPEND_HEADS], coming[APPEND_HEADS];
+  auto fetch = [&](Raw8<TQ> (&to)[APPEND_HEADS], int t, int hb) {
+    const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + d;
 #pragma unroll
     for (int i = 0; i < APPEND_HEADS; i++) {
       const int h = hb + i * GROUPS + grp;
-      if (in && h < h1) raw[i].load(src + (int64_t)h * a.hd); else raw[i].zero();
+      if (in && h < h1) to[i].load(src + (int64_t)h * a.hd); else to[i].zero();
     }
   };
-  fetch(h0);
-  const int pos = a.positions[t];
-  const int64_t slot = a.slots[t];
-  // Padding, and positions or slots outside the table and the pool: nothing is written.
-  const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (TURN == TURN_NONE || pos < a.max_positions);
-  if (!live) return;
-  // x' = x cs + other sn for this lane's features (cs = 1, sn = 0 past the rotary ones).
-  float cs[8], sn[8];
-  if (TURN != TURN_NONE) {
-    const float2* tab = a.table + (int64_t)pos * a.pairs;
+  int t = blockIdx.x, pos_coming = a.positions[t];
+  int64_t slot_coming = a.slots[t];
+  fetch(coming, t, h0);
+  for (; t < a.T; t += gridDim.x) {
+    const int pos = pos_coming;
+    const int64_t slot = slot_coming;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int f = d + e;
-      const bool turned = f < 2 * a.pairs, second = TURN == TURN_OWN ? f & 1 : f >= a.pairs;
-      const int i = TURN == TURN_OWN ? f >> 1 : second ? f - a.pairs : f;
-      const float2 v = turned ? tab[i] : make_float2(1.f, 0.f);
-      cs[e] = v.x;
-      sn[e] = second ? v.y : -v.y;
+    for (int i = 0; i < APPEND_HEADS; i++) raw[i] = coming[i];
+    const int next = t + gridDim.x;
+    if (next < a.T) {  // on its way while this token is worked on
+      fetch(coming, next, h0);
+      pos_coming = a.positions[next];
+      slot_coming = a.slots[next];
     }
-  }
-  const int64_t page = slot / a.kv.P, row = slot - page * a.kv.P;
-  const int64_t kv_off = page * a.kv.sp + row * a.kv.st + d;
-  TQ* q_out = reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride + d;
-  const float inv = 1.f / (float)a.hd;
-  // Every group runs as often, so that its warp's shuffles see all lanes.
-  for (int hb = h0; hb < h1; hb += GROUPS * APPEND_HEADS) {
-    if (hb > h0) fetch(hb);
+    // Padding, and positions or slots outside the table and the pool: nothing is written.
+    const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (TURN == TURN_NONE || pos < a.max_positions);
+    if (!live) continue;
+    // x' = x cs + other sn for this lane's features (cs = 1, sn = 0 past the rotary ones).
+    float cs[8], sn[8];
+    if (TURN == TURN_LANES) {
+      // Each warp copies the row of the table, two pairs a lane, in an order in
+      // which lanes with neighbouring features read neighbouring 16 bytes.
+      const int step = a.pairs / 8, wl = threadIdx.x & 31;
+      float4* row = turn[threadIdx.x >> 5];
+      const float4* tab = reinterpret_cast<const float4*>(a.table + (int64_t)pos * a.pairs);
+      __syncwarp();
+      for (int c = wl; c < 4 * step; c += 32) row[(c & 3) * step + (c >> 2)] = tab[c];
+      __syncwarp();
+      const int j = lane < step ? lane : lane - step;
 #pragma unroll
-    for (int i = 0; i < APPEND_HEADS; i++) {
-      const int h = hb + i * GROUPS + grp;
-      const bool rot = h < a.H + a.KVH;
-      float x[8];
-      raw[i].get(x);
-      if (a.norm != NORM_NONE) {
-        float mean = 0.f;
-        if (a.norm == NORM_LAYER) {
-          float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      for (int k = 0; k < 4; k++) {
+        const float4 v = lane < 2 * step ? row[k * step + j] : make_float4(1.f, 0.f, 1.f, 0.f);
+        cs[2 * k] = v.x;
+        sn[2 * k] = lane < step ? -v.y : v.y;
+        cs[2 * k + 1] = v.z;
+        sn[2 * k + 1] = lane < step ? -v.w : v.w;
+      }
+    } else if (TURN != TURN_NONE) {
+      const float2* tab = a.table + (int64_t)pos * a.pairs;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int f = d + e;
+        const bool turned = f < 2 * a.pairs, second = TURN == TURN_OWN ? f & 1 : f >= a.pairs;
+        const int i = TURN == TURN_OWN ? f >> 1 : second ? f - a.pairs : f;
+        const float2 v = turned ? tab[i] : make_float2(1.f, 0.f);
+        cs[e] = v.x;
+        sn[e] = second ? v.y : -v.y;
+      }
+    }
+    const int64_t page = slot / a.kv.P, row = slot - page * a.kv.P;
+    const int64_t kv_off = page * a.kv.sp + row * a.kv.st + d;
+    TQ* q_out = reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride + d;
+    // Every group runs as often, so that its warp's shuffles see all lanes.
+    for (int hb = h0; hb < h1; hb += GROUPS * APPEND_HEADS) {
+      if (hb > h0) fetch(raw, t, hb);
+#pragma unroll
+      for (int i = 0; i < APPEND_HEADS; i++) {
+        const int h = hb + i * GROUPS + grp;
+        const bool rot = h < a.H + a.KVH;
+        float x[8];
+        raw[i].get(x);
+        if (a.norm != NORM_NONE) {
+          float mean = 0.f;
+          if (a.norm == NORM_LAYER) {
+            float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            mean = s * inv;
+          }
+          float s = 0.f;
+          if (in)
+#pragma unroll
+            for (int e = 0; e < 8; e++) s = fmaf(x[e] - mean, x[e] - mean, s);
 #pragma unroll
           for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          mean = s * inv;
-        }
-        float s = 0.f;
-        if (in)
+          if (rot && h < h1 && in) {
+            const float r = rsqrtf(fmaf(s, inv, a.eps));
+            float w[8];
+            load8((h < a.H ? a.qw + h * a.w_stride : a.kw + (h - a.H) * a.w_stride) + d, w);
 #pragma unroll
-          for (int e = 0; e < 8; e++) s = fmaf(x[e] - mean, x[e] - mean, s);
-#pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (rot && h < h1 && in) {
-          const float r = rsqrtf(fmaf(s, inv, a.eps));
-          float w[8];
-          load8((h < a.H ? a.qw + h * a.w_stride : a.kw + (h - a.H) * a.w_stride) + d, w);
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = (x[e] - mean) * r * w[e];
-        }
-      }
-      if (TURN == TURN_OWN) {
-        if (rot)
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            if (d + e >= 2 * a.pairs) continue;
-            const float u = x[e], v = x[e + 1];
-            x[e] = fmaf(u, cs[e], v * sn[e]);
-            x[e + 1] = fmaf(v, cs[e + 1], u * sn[e + 1]);
+            for (int e = 0; e < 8; e++) x[e] = (x[e] - mean) * r * w[e];
           }
-      } else if (TURN == TURN_LANES) {
-        const int step = a.pairs / 8, from = lane < step ? lane + step : lane < 2 * step ? lane - step : lane;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float other = __shfl_sync(0xffffffffu, x[e], from, LPH);
-          if (rot && lane < 2 * step) x[e] = fmaf(x[e], cs[e], other * sn[e]);
         }
-      } else if (TURN == TURN_SHARED) {
-        float* st = stage[grp];
-        __syncwarp();
-        *reinterpret_cast<float4*>(st + d) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(st + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        __syncwarp();
-        if (rot)
+        if (TURN == TURN_OWN) {
+          if (rot)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              if (d + e >= 2 * a.pairs) continue;
+              const float u = x[e], v = x[e + 1];
+              x[e] = fmaf(u, cs[e], v * sn[e]);
+              x[e + 1] = fmaf(v, cs[e + 1], u * sn[e + 1]);
+            }
+        } else if (TURN == TURN_LANES) {
+          const int step = a.pairs / 8, from = lane < step ? lane + step : lane < 2 * step ? lane - step : lane;
 #pragma unroll
           for (int e = 0; e < 8; e++) {
-            const int f = d + e;
-            if (f < 2 * a.pairs) x[e] = fmaf(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs] * sn[e]);
+            const float other = __shfl_sync(0xffffffffu, x[e], from, LPH);
+            if (rot && lane < 2 * step) x[e] = fmaf(x[e], cs[e], other * sn[e]);
           }
-      }
-      if (h < h1 && in) {
-        if (h < a.H)
-          store8(q_out + (int64_t)h * a.hd, x);
-        else
-          store8(reinterpret_cast<TK*>(rot ? a.kv.k : a.kv.v) + kv_off + (int64_t)(rot ? h - a.H : h - a.H - a.KVH) * a.kv.sh, x);
+        } else if (TURN == TURN_SHARED) {
+          float* st = stage[grp];
+          __syncwarp();
+          *reinterpret_cast<float4*>(st + d) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(st + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          __syncwarp();
+          if (rot)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const int f = d + e;
+              if (f < 2 * a.pairs) x[e] = fmaf(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs] * sn[e]);
+            }
+        }
+        if (h < h1 && in) {
+          if (h < a.H)
+            store8(q_out + (int64_t)h * a.hd, x);
+          else
+            store8(reinterpret_cast<TK*>(rot ? a.kv.k : a.kv.v) + kv_off + (int64_t)(rot ? h - a.H : h - a.H - a.KVH) * a.kv.sh, x);
+        }
       }
     }
   }
@@ -448,11 +486,12 @@ __global__ void __launch_bounds__(APPEND_THREADS, 4) k_append(AppendArgs a, int 
 
 // ---------------------------------------------------------------------------
 // Page means: for every slot that is the last of its page, the mean key of
-// the page for each KV head, float32 sums rounded once. A CTA takes 32 slots
-// and one KV head and all its warps share a page: hd / 8 lanes hold a
-// position's features, eight each, and the CTA's 128 / (hd / 8) sets of lanes
-// take alternate positions, four loads in flight a lane. The sets' sums are
-// added in a fixed order.
+// the page for each KV head, float32 sums rounded once. WARPS warps take 32
+// slots and one KV head: hd / 8 lanes hold a position's features, eight each,
+// and the sets of lanes that fit take alternate positions, a page of 32 in
+// one go. The sets' sums are added in a fixed order. One warp where there are
+// slots enough to fill the GPU (16,384 of the 3B shape: 23 us, with four 32),
+// four, which share each page, where there are not (256 slots: 4.9 us, with one 7.9).
 struct MeansArgs {
   int T;
   const int64_t* slots;
@@ -460,19 +499,20 @@ struct MeansArgs {
   PagedView kv;
 };
 
-template <typename TK>
+template <typename TK, int WARPS>
 __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
+  constexpr int LANES = WARPS * 32;
   __shared__ __align__(16) float sums[128][8];
-  const int tid = threadIdx.x, lane = tid & 31;
-  const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, sets = 128 / lpr;
-  const int64_t t = (int64_t)blockIdx.x * 32 + lane;
+  const int tid = threadIdx.x % LANES, lane = tid & 31, base_row = threadIdx.x - tid;
+  const int g = blockIdx.y, P = a.kv.P, lpr = a.kv.hd / 8, sets = LANES / lpr;
+  const int64_t t = ((int64_t)blockIdx.x * (128 / LANES) + threadIdx.x / LANES) * 32 + lane;
   pdl_wait();
   int64_t slot = t < a.T ? a.slots[t] : -1;
   if (slot >= (int64_t)a.kv.num_pages * P) slot = -1;
   const int my_page = slot < 0 ? -1 : (int)(slot / P);
-  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - (int64_t)my_page * P == P - 1);  // the same in every warp
+  uint32_t todo = __ballot_sync(0xffffffffu, slot >= 0 && slot - (int64_t)my_page * P == P - 1);  // the same in all WARPS warps
   const int r0 = tid / lpr, d = (tid - r0 * lpr) * 8;
-  constexpr int U = 4;
+  constexpr int U = WARPS > 1 ? 4 : sizeof(TK) == 4 ? 8 : 16;
   while (todo) {
     const int src = __ffs(todo) - 1;
     todo &= todo - 1;
@@ -481,28 +521,29 @@ __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
     float s[8] = {};
     if (r0 < sets) {
       for (int r = r0; r < P; r += U * sets) {
+        // Rows behind the page's last are read as that one and not added.
         Raw8<TK> x[U];
 #pragma unroll
-        for (int i = 0; i < U; i++)
-          if (r + i * sets < P) x[i].load(base + (int64_t)(r + i * sets) * a.kv.st); else x[i].zero();
+        for (int i = 0; i < U; i++) x[i].stream(base + (int64_t)min(r + i * sets, P - 1) * a.kv.st);
 #pragma unroll
         for (int i = 0; i < U; i++) {
           float y[8];
           x[i].get(y);
+          if (r + i * sets < P)
 #pragma unroll
-          for (int e = 0; e < 8; e++) s[e] += y[e];
+            for (int e = 0; e < 8; e++) s[e] += y[e];
         }
       }
     }
-    store8(&sums[tid][0], s);
-    __syncthreads();
+    store8(&sums[threadIdx.x][0], s);
+    if (WARPS > 1) __syncthreads(); else __syncwarp();
     // One feature a thread: the sets' sums in order.
-    for (int f = tid; f < a.kv.hd; f += 128) {
+    for (int f = tid; f < a.kv.hd; f += LANES) {
       float x = 0.f;
-      for (int i = 0; i < min(sets, P); i++) x += sums[i * lpr + (f >> 3)][f & 7];
+      for (int i = 0; i < min(sets, P); i++) x += sums[base_row + i * lpr + (f >> 3)][f & 7];
       store_as(reinterpret_cast<TK*>(a.means) + (page * a.kv.kvh + g) * a.kv.hd + f, x / (float)P);
     }
-    __syncthreads();
+    if (WARPS > 1) __syncthreads(); else __syncwarp();
   }
 }
 
