@@ -447,7 +447,7 @@ int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, 
                   int32_t table_width, int64_t table_stride, const int32_t* free_pages, int32_t n_free, int32_t capacity, int32_t* starts,
                   int32_t* lengths, int32_t* positions, int64_t* slots, int32_t* counts);
 
-/* Rotary table: max_positions x pairs float32 pairs (cos, sin), 16-byte
+/* Rotary table: max_positions x pairs float32 pairs (cos, sin), 8-byte
  * aligned. Pair i is features (i, i + pairs) of a head, or (2i, 2i + 1) when
  * adjacent != 0; features from 2 * pairs on pass unchanged. */
 typedef struct {

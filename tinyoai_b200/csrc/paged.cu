@@ -113,6 +113,7 @@ PagedView view_of(const tcu_paged_kv* kv) {
   v.sh = kv->head_stride;
   v.st = kv->token_stride;
   v.divP = FastDiv::of((uint32_t)kv->page_tokens);
+  v.small = (int64_t)kv->num_pages * kv->page_tokens < 0x7fffffffll;
   return v;
 }
 
@@ -167,15 +168,20 @@ int launch_append(const AppendArgs& a, cudaStream_t s) {
     const int64_t y = ceil_div(heads, per), x = std::min<int64_t>(a.T, std::max<int64_t>(1, 3 * SM_COUNT / y));
     return launch("k_append", kern, dim3((unsigned)x, (unsigned)y), APPEND_THREADS, 0, s, a, per);
   };
+  auto pick_norm = [&](auto turn, auto norm) {
+    constexpr int TURN = decltype(turn)::value, NORM = decltype(norm)::value;
+    if (a.hd <= 64) return go(k_append<TQ, TK, 8, TURN, NORM>, 8);
+    if (a.hd <= 128) return go(k_append<TQ, TK, 16, TURN, NORM>, 16);
+    return go(k_append<TQ, TK, 32, TURN, NORM>, 32);
+  };
   auto pick = [&](auto turn) {
-    constexpr int TURN = decltype(turn)::value;
-    if (a.hd <= 64) return go(k_append<TQ, TK, 8, TURN>, 8);
-    if (a.hd <= 128) return go(k_append<TQ, TK, 16, TURN>, 16);
-    return go(k_append<TQ, TK, 32, TURN>, 32);
+    if (a.norm == NORM_RMS) return pick_norm(turn, std::integral_constant<int, NORM_RMS>());
+    if (a.norm == NORM_LAYER) return pick_norm(turn, std::integral_constant<int, NORM_LAYER>());
+    return pick_norm(turn, std::integral_constant<int, NORM_NONE>());
   };
   if (a.pairs == 0) return pick(std::integral_constant<int, TURN_NONE>());
-  if (a.adjacent) return pick(std::integral_constant<int, TURN_OWN>());
-  if (a.pairs % 8 == 0) return pick(std::integral_constant<int, TURN_LANES>());
+  if (a.adjacent) return pick(std::integral_constant<int, TURN_BESIDE>());
+  if (a.pairs % 4 == 0) return pick(std::integral_constant<int, TURN_RUNS>());
   return pick(std::integral_constant<int, TURN_SHARED>());
 }
 
@@ -313,8 +319,8 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
     p.scores = off;
     off += align256(lists * q->table_width * sizeof(float));
     p.eps = off;
-    // Scoring CTAs: four for each SM where there are few lists, 64 pages at least.
-    const int64_t shares = std::max<int64_t>(1, ceil_div(4 * SM_COUNT, std::max<int64_t>(1, (int64_t)lists)));
+    // Scoring CTAs: up to four for each SM (its room), of 64 pages at least.
+    const int64_t shares = std::max<int64_t>(1, 4 * SM_COUNT / std::max<int64_t>(1, (int64_t)lists));
     p.score_per = (int)(ceil_div(std::max<int64_t>(1, ceil_div(q->table_width, shares)), 64) * 64);
     p.score_tiles = (int)ceil_div(q->table_width, p.score_per);
     off += align256(lists * p.score_tiles * sizeof(float));
@@ -473,7 +479,11 @@ int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p,
     else
       TRY((launch_scores<TQ, TK, 256>(a, c, queries, s)));
   }
-  TRY(launch("k_page_choose", k_page_choose<TQ, TK>, dim3(queries, a.KVH), CHOOSE_THREADS, sizeof(float) * std::min(c.width, CHOOSE_CACHE), s, a, c));
+  const size_t cache = sizeof(uint32_t) * std::min(c.width, CHOOSE_CACHE);
+  if (c.width <= 1024)
+    TRY((launch("k_page_choose", k_page_choose<TQ, TK, 256>, dim3(queries, a.KVH), 256, cache, s, a, c)));
+  else
+    TRY((launch("k_page_choose", k_page_choose<TQ, TK, 1024>, dim3(queries, a.KVH), 1024, cache, s, a, c)));
   TRY((launch_parts<TQ, TK, SRC_LIST>(a, p.own_rows, p.own_slots, s)));
   if (p.cluster || p.own_slots == 1) return TCU_OK;  // the output is written
   return launch("k_attend_join", k_attend_join<TQ, 1>, dim3(queries, (a.H + 3) / 4), 128, 0, s, a);
@@ -661,7 +671,7 @@ int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32
   TRY(check_ptr("q_out", q_out, device, 16));
   TRY(check_ptr("positions", positions, device, 4));
   TRY(check_ptr("slots", slots, device, 8));
-  if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 16));
+  if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 8));
   if (a.norm) {
     TRY(check_ptr("q_weight", a.qw, device, 16));
     TRY(check_ptr("k_weight", a.kw, device, 16));

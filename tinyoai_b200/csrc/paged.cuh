@@ -47,6 +47,7 @@ struct PagedView {
   int num_pages, P, kvh, hd;
   int64_t sp, sh, st;  // strides of a page, a head, a position, in values
   FastDiv divP;
+  int small;  // 1: the pool has fewer than 2^31 positions
 };
 
 // Values of a row, four at a time, as float32.
@@ -273,15 +274,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
 //          a' = a c - b s, b' = b c + a s
 //   split halves: a = y[i], b = y[i + pairs]; adjacent: a = y[2i], b = y[2i + 1].
 //
-// Float32 throughout, rounded once when stored. Bytes bound it: each value is
-// read and written once. A CTA takes one token and a share of its heads; LPH
-// lanes hold a head, eight values each, and all heads of a group of lanes
-// that the CTA has (three at a time, two of float32) are loaded before the
-// token's position and slot are known. A lane has the same features of every
-// head, so it keeps their cosines and sines in registers (read straight from
-// the table, 64 bytes a lane apart, they cost more of L1 than the values do).
-// The partner of a rotary pair comes from another lane (through shared memory where pairs do
-// not fall on whole lanes).
+// Float32 throughout, rounded once when stored. Each value is read and written
+// once. A CTA takes one token at a time and a share of its heads; LPH lanes
+// hold a head, eight values each, the next token's heads already on their
+// way. A lane has the same features of every head, so it keeps their cosines,
+// sines and shared norm weights in registers. Instructions count here beside
+// bytes (4,096 rows of 32 + 8 + 8 heads of 128 took 33 us with a rotary pair's
+// other value fetched from another lane, TODO_FIGURE so): where pairs come in
+// fours a lane holds both values of four pairs, two runs of four features.
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
 struct AppendArgs {
@@ -335,149 +335,199 @@ struct Raw8<float> {
   }
 };
 
-// How a rotary pair's other value is found.
-enum { TURN_NONE = 0, TURN_LANES = 1, TURN_OWN = 2, TURN_SHARED = 3 };
+template <typename T>
+__device__ __forceinline__ void load4to(const T* p, float* x) {
+  const float4 v = load4(p);
+  x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+
+// Where a rotary pair's other value is: in the same lane, in its second run of
+// four features (TURN_RUNS) or beside the first (TURN_BESIDE), or anywhere
+// (TURN_SHARED: through shared memory).
+enum { TURN_NONE = 0, TURN_RUNS = 1, TURN_BESIDE = 2, TURN_SHARED = 3 };
+
+// Four stored values, as loaded.
+template <typename T>
+struct Raw4 {
+  uint2 v;
+  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint2*>(p); }
+  __device__ __forceinline__ void zero() { v = make_uint2(0, 0); }
+  __device__ __forceinline__ void get(float* x) const {
+    unpack2(T(), v.x, x[0], x[1]);
+    unpack2(T(), v.y, x[2], x[3]);
+  }
+};
+template <>
+struct Raw4<float> {
+  float4 v;
+  __device__ __forceinline__ void load(const float* p) { v = load4(p); }
+  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float* x) const {
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  }
+};
 
 // grid: x = tokens x, x + gridDim.x, ...; y = share of the heads (heads_per_cta of them).
-template <typename TQ, typename TK, int LPH, int TURN>
+template <typename TQ, typename TK, int LPH, int TURN, int NORM>
 __global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int heads_per_cta) {
   constexpr int GROUPS = APPEND_THREADS / LPH;
-  constexpr int APPEND_HEADS = sizeof(TQ) == 4 ? 2 : 3;  // heads of a group of lanes in flight (64 registers)
+  constexpr int HEADS = sizeof(TQ) == 4 ? 2 : 3;  // heads of a group of lanes at a time
   __shared__ __align__(16) float stage[TURN == TURN_SHARED ? GROUPS : 1][LPH * 8 + 4];
-  __shared__ float4 turn[TURN == TURN_LANES ? APPEND_THREADS / 32 : 1][64];
   const int grp = threadIdx.x / LPH, lane = threadIdx.x % LPH;
-  const int heads = a.H + 2 * a.KVH;
-  const int h0 = blockIdx.y * heads_per_cta, h1 = min(heads, h0 + heads_per_cta);
-  const int d = lane * 8;
-  const bool in = d < a.hd;
+  const int h0 = blockIdx.y * heads_per_cta, h1 = min(a.H + 2 * a.KVH, h0 + heads_per_cta);
+  // This lane's features: four from da and four from db on.
+  const bool turns = TURN == TURN_RUNS && lane < a.pairs / 4;
+  const int da = turns ? lane * 4 : TURN == TURN_RUNS ? 2 * a.pairs + (lane - a.pairs / 4) * 8 : lane * 8;
+  const int db = turns ? a.pairs + lane * 4 : da + 4;
   const float inv = 1.f / (float)a.hd;
   pdl_wait();
-  Raw8<TQ> raw[APPEND_HEADS], coming[APPEND_HEADS];
-  auto fetch = [&](Raw8<TQ> (&to)[APPEND_HEADS], int t, int hb) {
-    const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride + d;
-#pragma unroll
-    for (int i = 0; i < APPEND_HEADS; i++) {
-      const int h = hb + i * GROUPS + grp;
-      if (in && h < h1) to[i].load(src + (int64_t)h * a.hd); else to[i].zero();
-    }
+  struct Head {
+    Raw4<TQ> lo, hi;
   };
-  int t = blockIdx.x, pos_coming = a.positions[t];
-  int64_t slot_coming = a.slots[t];
-  fetch(coming, t, h0);
-  for (; t < a.T; t += gridDim.x) {
-    const int pos = pos_coming;
-    const int64_t slot = slot_coming;
+  for (int hb = h0; hb < h1; hb += GROUPS * HEADS) {
+    // What does not change from token to token. A lane without work has on false.
+    bool on[HEADS], rot[HEADS], is_q[HEADS];
+    int in_at[HEADS];       // of the row
+    int64_t out_at[HEADS];  // of the query row, or of the slot's place in the cache
+    TK* cache[HEADS];
+    const float* weight[HEADS];
 #pragma unroll
-    for (int i = 0; i < APPEND_HEADS; i++) raw[i] = coming[i];
-    const int next = t + gridDim.x;
-    if (next < a.T) {  // on its way while this token is worked on
-      fetch(coming, next, h0);
-      pos_coming = a.positions[next];
-      slot_coming = a.slots[next];
+    for (int i = 0; i < HEADS; i++) {
+      const int h = hb + i * GROUPS + grp, g = h < a.H + a.KVH ? h - a.H : h - a.H - a.KVH;
+      on[i] = h < h1 && da < a.hd;
+      rot[i] = h < a.H + a.KVH;
+      is_q[i] = h < a.H;
+      in_at[i] = h * a.hd;
+      out_at[i] = is_q[i] ? (int64_t)h * a.hd : (int64_t)g * a.kv.sh;
+      cache[i] = reinterpret_cast<TK*>(rot[i] ? a.kv.k : a.kv.v);
+      weight[i] = is_q[i] ? a.qw + h * a.w_stride : a.kw + g * a.w_stride;
     }
-    // Padding, and positions or slots outside the table and the pool: nothing is written.
-    const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (TURN == TURN_NONE || pos < a.max_positions);
-    if (!live) continue;
-    // x' = x cs + other sn for this lane's features (cs = 1, sn = 0 past the rotary ones).
-    float cs[8], sn[8];
-    if (TURN == TURN_LANES) {
-      // Each warp copies the row of the table, two pairs a lane, in an order in
-      // which lanes with neighbouring features read neighbouring 16 bytes.
-      const int step = a.pairs / 8, wl = threadIdx.x & 31;
-      float4* row = turn[threadIdx.x >> 5];
-      const float4* tab = reinterpret_cast<const float4*>(a.table + (int64_t)pos * a.pairs);
-      __syncwarp();
-      for (int c = wl; c < 4 * step; c += 32) row[(c & 3) * step + (c >> 2)] = tab[c];
-      __syncwarp();
-      const int j = lane < step ? lane : lane - step;
+    Head coming[HEADS];
+    auto fetch = [&](int t) {
+      const TQ* src = reinterpret_cast<const TQ*>(a.qkv) + (int64_t)t * a.qkv_stride;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float4 v = lane < 2 * step ? row[k * step + j] : make_float4(1.f, 0.f, 1.f, 0.f);
-        cs[2 * k] = v.x;
-        sn[2 * k] = lane < step ? -v.y : v.y;
-        cs[2 * k + 1] = v.z;
-        sn[2 * k + 1] = lane < step ? -v.w : v.w;
+      for (int i = 0; i < HEADS; i++) {
+        if (on[i]) {
+          coming[i].lo.load(src + in_at[i] + da);
+          coming[i].hi.load(src + in_at[i] + db);
+        } else {
+          coming[i].lo.zero();
+          coming[i].hi.zero();
+        }
       }
-    } else if (TURN != TURN_NONE) {
+    };
+    int t = blockIdx.x, pos_coming = a.positions[t];
+    int64_t slot_coming = a.slots[t];
+    fetch(t);
+    for (; t < a.T; t += gridDim.x) {
+      const int pos = pos_coming;
+      const int64_t slot = slot_coming;
+      Head raw[HEADS];
+#pragma unroll
+      for (int i = 0; i < HEADS; i++) raw[i] = coming[i];
+      const int next = t + gridDim.x;
+      if (next < a.T) {  // on its way while this token is worked on
+        fetch(next);
+        pos_coming = a.positions[next];
+        slot_coming = a.slots[next];
+      }
+      // Padding, and positions or slots outside the table and the pool: nothing is written.
+      const bool live = slot >= 0 && slot < (int64_t)a.kv.num_pages * a.kv.P && pos >= 0 && (TURN == TURN_NONE || pos < a.max_positions);
+      if (!live) continue;
+      // Cosines and sines of this lane's pairs, or (TURN_SHARED) of its features.
+      float cs[8], sn[8];
       const float2* tab = a.table + (int64_t)pos * a.pairs;
+      if (TURN == TURN_RUNS || TURN == TURN_BESIDE) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int f = d + e;
-        const bool turned = f < 2 * a.pairs, second = TURN == TURN_OWN ? f & 1 : f >= a.pairs;
-        const int i = TURN == TURN_OWN ? f >> 1 : second ? f - a.pairs : f;
-        const float2 v = turned ? tab[i] : make_float2(1.f, 0.f);
-        cs[e] = v.x;
-        sn[e] = second ? v.y : -v.y;
+        for (int e = 0; e < 4; e++) {
+          const int i = lane * 4 + e;
+          const float2 v = i < a.pairs ? tab[i] : make_float2(1.f, 0.f);
+          cs[e] = v.x;
+          sn[e] = v.y;
+        }
+      } else if (TURN == TURN_SHARED) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int f = da + e;
+          const bool second = f >= a.pairs;
+          const float2 v = f < 2 * a.pairs ? tab[second ? f - a.pairs : f] : make_float2(1.f, 0.f);
+          cs[e] = v.x;
+          sn[e] = second ? v.y : -v.y;
+        }
       }
-    }
-    const int64_t page = slot / a.kv.P, row = slot - page * a.kv.P;
-    const int64_t kv_off = page * a.kv.sp + row * a.kv.st + d;
-    TQ* q_out = reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride + d;
-    // Every group runs as often, so that its warp's shuffles see all lanes.
-    for (int hb = h0; hb < h1; hb += GROUPS * APPEND_HEADS) {
-      if (hb > h0) fetch(raw, t, hb);
+      const int64_t page = a.kv.small ? (int64_t)a.kv.divP.div((uint32_t)slot) : slot / a.kv.P;
+      const int64_t kv_off = page * a.kv.sp + (slot - page * a.kv.P) * a.kv.st;
+      TQ* q_out = reinterpret_cast<TQ*>(a.q_out) + (int64_t)t * a.q_stride;
+      // Every lane takes part in the shuffles, with or without work.
 #pragma unroll
-      for (int i = 0; i < APPEND_HEADS; i++) {
-        const int h = hb + i * GROUPS + grp;
-        const bool rot = h < a.H + a.KVH;
+      for (int i = 0; i < HEADS; i++) {
         float x[8];
-        raw[i].get(x);
-        if (a.norm != NORM_NONE) {
-          float mean = 0.f;
-          if (a.norm == NORM_LAYER) {
-            float s = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        raw[i].lo.get(x);
+        raw[i].hi.get(x + 4);
+        if (NORM != NORM_NONE) {
+          float mean = 0.f, s = 0.f;
+          if (NORM == NORM_LAYER) {
+            float z = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
 #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            mean = s * inv;
+            for (int o = LPH / 2; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+            mean = z * inv;
+            if (rot[i])
+#pragma unroll
+              for (int e = 0; e < 8; e++) x[e] -= mean;
           }
-          float s = 0.f;
-          if (in)
+          if (on[i])
 #pragma unroll
-            for (int e = 0; e < 8; e++) s = fmaf(x[e] - mean, x[e] - mean, s);
+            for (int e = 0; e < 8; e++) s = fmaf(x[e], x[e], s);
 #pragma unroll
           for (int o = LPH / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-          if (rot && h < h1 && in) {
+          if (rot[i] && on[i]) {
             const float r = rsqrtf(fmaf(s, inv, a.eps));
             float w[8];
-            load8((h < a.H ? a.qw + h * a.w_stride : a.kw + (h - a.H) * a.w_stride) + d, w);
+            load4to(weight[i] + da, w);
+            load4to(weight[i] + db, w + 4);
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = (x[e] - mean) * r * w[e];
+            for (int e = 0; e < 8; e++) x[e] = x[e] * r * w[e];
           }
         }
-        if (TURN == TURN_OWN) {
-          if (rot)
+        if (TURN == TURN_RUNS) {
+          if (rot[i] && turns)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              if (d + e >= 2 * a.pairs) continue;
-              const float u = x[e], v = x[e + 1];
-              x[e] = fmaf(u, cs[e], v * sn[e]);
-              x[e + 1] = fmaf(v, cs[e + 1], u * sn[e + 1]);
+            for (int e = 0; e < 4; e++) {
+              const float u = x[e], v = x[4 + e];
+              x[e] = fmaf(u, cs[e], -(v * sn[e]));
+              x[4 + e] = fmaf(v, cs[e], u * sn[e]);
             }
-        } else if (TURN == TURN_LANES) {
-          const int step = a.pairs / 8, from = lane < step ? lane + step : lane < 2 * step ? lane - step : lane;
+        } else if (TURN == TURN_BESIDE) {
+          if (rot[i])
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float other = __shfl_sync(0xffffffffu, x[e], from, LPH);
-            if (rot && lane < 2 * step) x[e] = fmaf(x[e], cs[e], other * sn[e]);
-          }
+            for (int e = 0; e < 4; e++)
+              if (lane * 4 + e < a.pairs) {
+                const float u = x[2 * e], v = x[2 * e + 1];
+                x[2 * e] = fmaf(u, cs[e], -(v * sn[e]));
+                x[2 * e + 1] = fmaf(v, cs[e], u * sn[e]);
+              }
         } else if (TURN == TURN_SHARED) {
           float* st = stage[grp];
           __syncwarp();
-          *reinterpret_cast<float4*>(st + d) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4*>(st + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
+          *reinterpret_cast<float4*>(st + da) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(st + da + 4) = make_float4(x[4], x[5], x[6], x[7]);
           __syncwarp();
-          if (rot)
+          if (rot[i])
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-              const int f = d + e;
+              const int f = da + e;
               if (f < 2 * a.pairs) x[e] = fmaf(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs] * sn[e]);
             }
         }
-        if (h < h1 && in) {
-          if (h < a.H)
-            store8(q_out + (int64_t)h * a.hd, x);
-          else
-            store8(reinterpret_cast<TK*>(rot ? a.kv.k : a.kv.v) + kv_off + (int64_t)(rot ? h - a.H : h - a.H - a.KVH) * a.kv.sh, x);
+        if (on[i]) {
+          const float4 lo = make_float4(x[0], x[1], x[2], x[3]), hi = make_float4(x[4], x[5], x[6], x[7]);
+          if (is_q[i]) {
+            store4(q_out + out_at[i] + da, lo);
+            store4(q_out + out_at[i] + db, hi);
+          } else {
+            store4(cache[i] + kv_off + out_at[i] + da, lo);
+            store4(cache[i] + kv_off + out_at[i] + db, hi);
+          }
         }
       }
     }
@@ -1113,31 +1163,33 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
   return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
 }
 
-constexpr int CHOOSE_THREADS = 256;
+constexpr int CHOOSE_MAX = 1024;    // threads of a choosing CTA at most
 constexpr int CHOOSE_CACHE = 8192;  // scores a CTA keeps in shared memory; others are read again from L2
 constexpr int CHOOSE_OPEN = 64;     // pages at the border that are ordered at once
-constexpr int RADIX_BITS = 11, RADIX_BINS = 1 << RADIX_BITS, BINS_PER = RADIX_BINS / CHOOSE_THREADS;
+constexpr int RADIX_BITS = 11, RADIX_BINS = 1 << RADIX_BITS;
 
 struct ChooseShared {
   int hist[RADIX_BINS];
-  int sums[CHOOSE_THREADS / 32], ties_of[CHOOSE_THREADS / 32], result[2];
+  int sums[CHOOSE_MAX / 32], result[2];
   int sure, open;
   uint32_t eps;
   int list[CHOOSE_OPEN];
   unsigned long long key[CHOOSE_OPEN];
 };
 
-// The want-th largest key (1 <= want <= number of keys) among the entries that
-// `each(f)` calls f(key) for on every thread, by digits of 11 bits from the
-// highest on; `want` becomes how many of that key itself are wanted. Eleven
+// The top `stop` of `bits` bits of the want-th largest key (1 <= want <= number
+// of keys) among the entries that `each(f)` calls f(key) for on every thread,
+// by digits of 11 bits from the highest on; `want` becomes how many of the keys
+// with these bits are wanted. Eleven
 // bits: scores share their exponents, and eight would put most of them on a
 // few bins, where the counts' updates queue up.
-template <typename Key, typename Each>
-__device__ __forceinline__ Key radix_select(ChooseShared& sh, int bits, int& want, Each each) {
+template <int CHOOSE_THREADS, typename Key, typename Each>
+__device__ __forceinline__ Key radix_select(ChooseShared& sh, int bits, int stop, int& want, Each each) {
+  constexpr int BINS_PER = RADIX_BINS / CHOOSE_THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Key prefix = 0;
   int done = 0;  // bits of the prefix
-  while (done < bits) {
+  while (done < stop) {
     const int n = min(RADIX_BITS, bits - done), shift = bits - done - n;
 #pragma unroll
     for (int i = 0; i < BINS_PER; i++) sh.hist[tid + i * CHOOSE_THREADS] = 0;
@@ -1172,12 +1224,15 @@ __device__ __forceinline__ Key radix_select(ChooseShared& sh, int bits, int& wan
   return prefix;
 }
 
-// One CTA per (query, KV head): the top-th key by radix selection, then the
-// chosen pages in ascending order. grid: x = request * max_fresh + query, y = KV head.
-template <typename TQ, typename TK>
+// One CTA per (query, KV head): a narrow interval around the top-th key by
+// radix selection, the pages in and around it ordered in float64, then the
+// chosen pages in ascending order. 256 threads, or 1,024 where tables have
+// more than 1,024 pages (each takes 16 of 4,096 pages with 256: 17 us).
+// grid: x = request * max_fresh + query, y = KV head.
+template <typename TQ, typename TK, int CHOOSE_THREADS>
 __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, ChooseArgs c) {
   __shared__ ChooseShared sh;
-  extern __shared__ float cache[];  // min(width, CHOOSE_CACHE)
+  extern __shared__ uint32_t cache[];  // keys, min(width, CHOOSE_CACHE)
   pdl_wait();
   const Query q = query_at(a, blockIdx.x / a.max_fresh, blockIdx.x % a.max_fresh);
   if (q.token < 0) return;
@@ -1190,10 +1245,11 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
   const float* scores = c.scores + at * c.width;
   unsigned long long* keys = c.keys + at * c.width;
   const int kept = min(hi, min(c.width, CHOOSE_CACHE));
-  auto score = [&](int b) { return b < kept ? cache[b] : scores[b]; };
-  float in_above = INFINITY, out_below = INFINITY;  // certain: a score above, certainly not: one below
-  bool every = false;                               // all candidates are open
-  auto is_open = [&](float x) { return every || (x <= in_above && x >= out_below); };
+  auto key32 = [&](int b) { return b < kept ? cache[b] : score_key32(scores[b]); };
+  // Keys above in_above: certainly in; below out_below: certainly not; those
+  // between are open (all of them, where the bound is not finite).
+  uint32_t in_above = 0xffffffffu, out_below = 0;
+  auto is_open = [&](uint32_t k) { return k <= in_above && k >= out_below; };
   unsigned long long thr = 0;  // open pages with a larger key are taken (~0: all open pages),
   int ties = 0;                // and this many with this one
   if (choose) {
@@ -1201,31 +1257,33 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
       sh.eps = 0;
       sh.sure = sh.open = 0;
     }
-    for (int b = lo + tid; b < kept; b += CHOOSE_THREADS) cache[b] = scores[b];
+#pragma unroll 4
+    for (int b = lo + tid; b < kept; b += CHOOSE_THREADS) cache[b] = score_key32(scores[b]);
     uint32_t e = 0;
     for (int i = lo / c.per + tid; i <= (hi - 1) / c.per; i += CHOOSE_THREADS) e = max(e, __float_as_uint(c.eps[at * c.tiles + i]) & 0x7fffffffu);
     e = __reduce_max_sync(0xffffffffu, e);
     __syncthreads();
     if (lane == 0 && e) atomicMax(&sh.eps, e);
-    // The top-th largest float32 score.
+    // The upper 22 bits of the top-th largest float32 score's key: it lies in
+    // [prefix, prefix + 1023], about the width of the error bound.
     int want = c.top;
-    const uint32_t prefix = radix_select<uint32_t>(sh, 32, want, [&](auto f) {
-      for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) f(score_key32(score(b)));
+    const uint32_t prefix = radix_select<CHOOSE_THREADS, uint32_t>(sh, 32, 2 * RADIX_BITS, want, [&](auto f) {
+#pragma unroll 4
+      for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) f(key32(b));
     });
     const float eps = __uint_as_float(sh.eps);
-    const float edge = float_from_order_key(prefix);
-    every = !(eps < INFINITY) || prefix <= 1u || !(fabsf(edge) < INFINITY);
-    if (!every) {
+    const float low = float_from_order_key(prefix), high = float_from_order_key(prefix | 1023u);
+    if (eps < INFINITY && prefix > 1u && fabsf(low) < INFINITY && fabsf(high) < INFINITY) {
       // Rounded outwards by the additions' own half steps.
-      const float r = 2.f * eps + 2e-7f * fabsf(edge);
-      in_above = edge + r;
-      out_below = edge - r;
+      in_above = score_key32(high + (2.f * eps + 2e-7f * fabsf(high)));
+      out_below = max(2u, score_key32(low - (2.f * eps + 2e-7f * fabsf(low))));
     }
     // Pages certainly in, and pages that float64 has to order.
     int sure = 0;
+#pragma unroll 4
     for (int b = lo + tid; b < hi; b += CHOOSE_THREADS) {
-      const float x = score(b);
-      if (!every && x > in_above) sure++;
+      const uint32_t x = key32(b);
+      sure += x > in_above;
       if (is_open(x)) {
         const int i = atomicAdd(&sh.open, 1);
         if (i < CHOOSE_OPEN) sh.list[i] = b;
@@ -1292,7 +1350,7 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
       } else {
         for (int b0 = lo + warp * 32; b0 < hi; b0 += CHOOSE_THREADS) {
           const int mine = b0 + lane;
-          uint32_t todo = __ballot_sync(0xffffffffu, mine < hi && is_open(score(min(mine, hi - 1))));
+          uint32_t todo = __ballot_sync(0xffffffffu, mine < hi && is_open(key32(min(mine, hi - 1))));
           while (todo) {
             const int b = b0 + __ffs(todo) - 1;
             todo &= todo - 1;
@@ -1301,52 +1359,69 @@ __global__ void __launch_bounds__(CHOOSE_THREADS) k_page_choose(AttendArgs a, Ch
           }
         }
         __syncthreads();
-        thr = radix_select<unsigned long long>(sh, 64, want, [&](auto f) {
+        thr = radix_select<CHOOSE_THREADS, unsigned long long>(sh, 64, 64, want, [&](auto f) {
           for (int b = lo + tid; b < hi; b += CHOOSE_THREADS)
-            if (is_open(score(b))) f(keys[b]);
+            if (is_open(key32(b))) f(keys[b]);
         });
         ties = want;
       }
     }
   }
+  // The chosen pages in order: each thread looks through a run of pages (an
+  // odd number, so that a warp's reads of the scores fall on different banks),
+  // and one sum over the threads says where its pages go. Ties go to the lower
+  // pages: their count before a thread's run needs a sum of its own.
   const bool keyed = choose && thr != ~0ull;
-  int done = 0, tied = 0;  // pages written, ties seen
-  for (int b0 = 0; b0 < npages; b0 += CHOOSE_THREADS) {
-    const int b = b0 + tid;
-    const bool inside = b >= lo && b < hi;
-    bool take = b < npages && (!inside || all), tie = false;
-    if (inside && choose) {
-      const float x = score(b);
-      const bool open = is_open(x);
-      const unsigned long long k = open && keyed ? keys[b] : 0;
-      take = open ? !keyed || k > thr : x > in_above;
-      tie = open && keyed && k == thr;
+  const int per = ((npages + CHOOSE_THREADS - 1) / CHOOSE_THREADS) | 1;
+  const int b0 = min(npages, tid * per), b1 = min(npages, b0 + per);
+  // -1: not taken, 0: a tie, 1: taken.
+  auto verdict = [&](int b) {
+    if (b < lo || b >= hi || all) return 1;
+    if (!choose) return -1;
+    const uint32_t x = key32(b);
+    if (!is_open(x)) return x > in_above ? 1 : -1;
+    if (!keyed) return 1;
+    const unsigned long long k = keys[b];
+    return k > thr ? 1 : k == thr ? 0 : -1;
+  };
+  auto sum_before = [&](int mine, int& total) {
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    int before = tied;
-    if (keyed) {  // ties go to the lower pages
-      const uint32_t tb = __ballot_sync(0xffffffffu, tie);
-      if (lane == 0) sh.ties_of[warp] = __popc(tb);
-      __syncthreads();
-      before += __popc(tb & ((1u << lane) - 1));
-      for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-        if (w < warp) before += sh.ties_of[w];
-        tied += sh.ties_of[w];
-      }
-    }
-    take = take || (tie && before < ties);
-    const uint32_t kb = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) sh.sums[warp] = __popc(kb);
     __syncthreads();
-    int to = done + __popc(kb & ((1u << lane) - 1)), total = 0;
+    if (lane == 31) sh.sums[warp] = x;
+    __syncthreads();
+    int before = x - mine;
+    total = 0;
     for (int w = 0; w < CHOOSE_THREADS / 32; w++) {
-      if (w < warp) to += sh.sums[w];
+      if (w < warp) before += sh.sums[w];
       total += sh.sums[w];
     }
-    if (take && to < a.budget) out[to] = b;
-    done += total;
-    __syncthreads();
+    return before;
+  };
+  int tied = 0, total;
+  if (keyed) {
+    int mine = 0;
+    for (int b = b0; b < b1; b++) mine += verdict(b) == 0;
+    tied = sum_before(mine, total);
   }
-  for (int e = done + tid; e < a.budget; e += CHOOSE_THREADS) out[e] = -1;
+  int mine = 0;
+  for (int b = b0, t = tied; b < b1; b++) {
+    const int v = verdict(b);
+    mine += v > 0 || (v == 0 && t++ < ties);
+  }
+  int to = sum_before(mine, total);
+  for (int b = b0, t = tied; b < b1; b++) {
+    const int v = verdict(b);
+    if (v > 0 || (v == 0 && t++ < ties)) {
+      if (to < a.budget) out[to] = b;
+      to++;
+    }
+  }
+  for (int e = total + tid; e < a.budget; e += CHOOSE_THREADS) out[e] = -1;
 }
 
 }  // namespace tcu
