@@ -431,6 +431,116 @@ def test_attend(qt, kt, case):
     assert bool((out[s["T"]:] == 5).all())  # rows behind the last request
 
 
+LONG = [
+    # lens, fresh, H, KVH, hd, P, prefix pages: kernels and joins that only many or long requests reach
+    ([2048 + 17 + i % 5 for i in range(64)], [1] * 64, 2, 2, 64, 16, 128),   # a prefix of its own kernel for every type
+    ([2048 + 60 + i % 9 for i in range(40)], [1 + i % 3 for i in range(40)], 6, 2, 128, 32, 64),
+    ([9000], [1], 4, 2, 128, 32, 0),                                          # more parts than a cluster joins
+    ([5000, 4200], [3, 1], 8, 2, 256, 16, 40),
+    ([3000, 900], [1, 1], 4, 4, 80, 7, 0),                                    # eight parts, pages of 7
+    ([1200, 1300, 0, 40], [1, 2, 1, 1], 20, 1, 64, 16, 0),                    # clusters with parts that have nothing
+]
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("case", range(len(LONG)))
+def test_attend_long(qt, kt, case):
+    lens, fresh, H, KVH, hd, P, prefix = LONG[case]
+    qt, kt = TYPES[qt], TYPES[kt]
+    s = attention_state(lens, fresh, H, KVH, hd, P, qt, kt, seed=40 + case, prefix=prefix)
+    out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], max(fresh), prefix=s["prefix"] if prefix else None,
+                                             max_length=s["lim"])
+    want, tol = expected(s, lens, fresh, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
+    # Sums over up to 9,000 positions, 2,304 in one chain of a lane at most.
+    near(out[:s["T"]], want, 2 * tol)
+
+
+def test_out_may_be_q():
+    """The queries' own buffer as the output: each row is read before it is written."""
+    for n, prefix, lens in ((3, 0, [700, 90, 33]), (48, 40, [1280 + i for i in range(48)]), (1, 0, [9000])):
+        s = attention_state(lens, [1] * n, 8, 2, 64, 32, torch.bfloat16, torch.bfloat16, seed=n, prefix=prefix)
+        c = paged.Cache(s["k"], s["v"])
+        args = (s["table"], s["starts"], s["lengths"], 1)
+        want = c.attend(s["q"], *args, prefix=s["prefix"] if prefix else None)
+        q = s["q"].clone()
+        c.attend(q, *args, prefix=s["prefix"] if prefix else None, out=q)
+        assert torch.equal(q[:n], want[:n])
+
+
+def test_a_max_length_that_cuts():
+    """Positions from max_length on are not attended."""
+    s = attention_state([100, 40], [1, 1], 4, 2, 64, 16, torch.float32, torch.float32, seed=2)
+    out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], 1, max_length=64)
+    want, tol = expected(s, [64, 40], [1, 1], 4, 2, 64, 16, 1 / 8, 0)
+    near(out[:2], want, tol)
+
+
+FIRST_CALL = """
+import torch
+from tinyoai_b200 import paged
+n = 40
+k = torch.randn(64 + n, 2, 16, 64, device="cuda").bfloat16(); v = torch.randn_like(k)
+c = paged.Cache(k, v)
+held = torch.full((n,), 1030, dtype=torch.int32, device="cuda"); fresh = torch.ones_like(held)
+tables = torch.arange(65, device="cuda").int().repeat(n, 1)
+tables[:, 64] += torch.arange(n, device="cuda").int()  # a page of its own behind the shared ones
+plan = paged.StepPlan(n, n, 16)
+qkv = torch.randn(n, 8 * 64, device="cuda").bfloat16()
+free = tables[0].clone(); prefix = tables[0, :64].clone()
+means = torch.zeros(64 + n, 2, 64, dtype=torch.bfloat16, device="cuda")
+def step():
+    plan.build(held, fresh, tables, free)
+    q = c.append(qkv, 4, plan.positions, plan.slots)
+    c.page_means(plan.slots, means)
+    return c.attend(q, tables, plan.starts, plan.lengths, 1, prefix=prefix), *c.attend_sparse(q, means, tables, plan.starts, plan.lengths, 1, top=3)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in got]
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+print("same")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls of all are captured ones."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "same" in r.stdout, r.stderr[-2000:]
+
+
+def test_calls_from_two_threads():
+    """One cache, two threads, different shapes, each on a stream of its own."""
+    import threading
+    s = attention_state([900, 700, 333, 64], [1] * 4, 16, 4, 128, 32, torch.bfloat16, torch.bfloat16, seed=6)
+    c = paged.Cache(s["k"], s["v"])
+    whole = (s["q"], s["table"], s["starts"], s["lengths"])
+    part = (s["q"][:2].clone(), s["table"][:2], s["starts"][:3], s["lengths"][:2])
+    want = [c.attend(*a, 1).clone() for a in (whole, part)]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(args, w, rows):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(50):
+                if not torch.equal(c.attend(*args, 1)[:rows], w[:rows]):
+                    bad.append(rows)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((whole, want[0], 4), (part, want[1], 2))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 SHARED = [
     # requests, fresh, H, KVH, hd, P, prefix pages, own positions, order: row tiles of the tensor cores
     (40, 1, 4, 4, 80, 32, 17, 40, "heads"),          # one tile, the streams take alternate blocks, a part block at the end
@@ -551,6 +661,9 @@ SPARSE = [
     ([9000], [2], 4, 2, 64, 16, 1, 3, 100, "heads"),               # several tiles of pages
     ([64, 65], [1, 1], 32, 1, 40, 1, 0, 1, 20, "heads"),
     ([400], [1], 4, 2, 64, 16, 1, 1, 64, "heads"),                 # more room than pages: everything
+    ([9000, 8000], [1, 1], 4, 2, 64, 16, 1, 1, 300, "heads"),      # more parts than a cluster joins
+    ([20011], [1], 2, 1, 64, 2, 1, 2, 700, "heads"),               # ten thousand pages: scores that do not all stay in shared memory
+    ([2200], [1], 2, 2, 64, 1, 0, 1, 1500, "positions"),           # over a thousand pages of one position
 ]
 
 

@@ -228,10 +228,9 @@ class Cache:
         pages, at = 0, None
         if prefix is not None:
             at, pages = _whole("prefix", prefix, torch.int32, self.device), len(prefix)
-        key = (q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
-        if self._sized[0] != key:
-            self._size(key, self._lib.tcu_paged_attend_workspace, ref, pages, max_length)
-        size = self._sized[1]
+        key = ("attend", q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
+        sized = self._sized  # one read: another thread may replace it
+        size = sized[1] if sized[0] == key else self._size(key, self._lib.tcu_paged_attend_workspace, ref, pages, max_length)
         work = self._workspace(size, stream)
         check(self._lib.tcu_paged_attend(index, _stream(stream, index), self._ref, ref, at, pages, max_length, work.data_ptr(), size))
         return out
@@ -252,10 +251,9 @@ class Cache:
             pages = tables.new_empty(shape)
         elif pages.shape != shape or pages.dtype != torch.int32 or pages.device != d or not pages.is_contiguous():
             raise _bad(f"pages must be a contiguous int32 tensor {shape} on {d}")
-        key = (q.dtype, q.shape, tables.shape, max_fresh, first, last, top)
-        if self._sized[0] != key:
-            self._size(key, self._lib.tcu_paged_attend_sparse_workspace, ref, first, last, top)
-        size = self._sized[1]
+        key = ("sparse", q.dtype, q.shape, tables.shape, max_fresh, first, last, top)
+        sized = self._sized
+        size = sized[1] if sized[0] == key else self._size(key, self._lib.tcu_paged_attend_sparse_workspace, ref, first, last, top)
         work = self._workspace(size, stream)
         check(self._lib.tcu_paged_attend_sparse(index, _stream(stream, index), self._ref, ref, means.data_ptr(), first, last, top, pages.data_ptr(),
                                                 work.data_ptr(), size))
@@ -266,6 +264,7 @@ class Cache:
         n = C.c_uint64()
         check(ask(self._ref, ref, *counts, C.byref(n)))
         self._sized = (key, n.value)
+        return n.value
 
     def _workspace(self, size, stream):
         """From torch's allocator, which hands it out again only to work behind this call on its stream."""
