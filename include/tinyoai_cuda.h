@@ -347,6 +347,16 @@ int tcu_batch_forward(tcu_batch* batch, tcu_session* const* sessions, const int3
  * penalties penalties[i]; writes n x k ids and scores. */
 int tcu_batch_sample_candidates(tcu_batch* batch, int32_t n, const int32_t* history, const int32_t* history_len,
                                 const tcu_penalties* penalties, int32_t k, int32_t* ids, double* scores);
+/* Lets steps of this batch whose sessions all begin with the same KV pages
+ * (forks of one session, tcu_session_fork) read those pages once for all of
+ * them: a step of two rows or more that share at least min_positions positions
+ * in whole pages attends through tcu_paged_append and tcu_paged_attend (below)
+ * instead of row by row. 0 (the default) turns it off. The rows then differ
+ * from the unshared step's by float32 rounding, not in what they compute.
+ * Allocates the step's buffers; a step whose workspace has to grow allocates
+ * again. Not for tensor-parallel models (TCU_EUNSUP), nor for head sizes that
+ * are not a multiple of 8. */
+int tcu_batch_share_prefix(tcu_batch* batch, int32_t min_positions);
 int tcu_batch_close(tcu_batch* batch);
 
 /* Sampling shortlist over a logits row the caller already holds in device

@@ -912,3 +912,65 @@ def test_refusals():
     none = torch.zeros((0, 4, 64), dtype=torch.float16, device=DEV)
     assert c.attend(none, t[:0], i32([0]), i32([]), 1).shape == (0, 4, 64)
     assert c.append(normal((0, 8 * 64), g, torch.float16), 4, i32([]), torch.zeros(0, dtype=torch.int64, device=DEV)).shape == (0, 4, 64)
+
+
+# ---------------------------------------------------------------------------
+# The batch step of the library's own sessions
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("heads, kv_heads, hidden", [(4, 4, 320), (8, 2, 512)])
+def test_batch_of_forks_shares_its_prefix(kv, heads, kv_heads, hidden):
+    """Forks of one session advance together with share_prefix on; every row
+    equals the same step with it off (the tolerance of a batch row against a
+    session of its own), and so does the cache: the steps after it go on
+    unshared. Sessions of other prefixes in the batch turn it off by themselves."""
+    import numpy as np
+
+    from tinyoai_b200 import Model
+    from tinyoai_b200.synth import prompt_ids, synth_stablelm
+
+    cfg, tensors = synth_stablelm(dict(model_type="stablelm", vocab_size=2048, hidden_size=hidden, intermediate_size=864, num_hidden_layers=3,
+                                       num_attention_heads=heads, num_key_value_heads=kv_heads, max_position_embeddings=1024, layer_norm_eps=1e-5,
+                                       rope_theta=10000.0, partial_rotary_factor=0.25, use_parallel_residual=True, use_qkv_bias=False,
+                                       qk_layernorm=False, tie_word_embeddings=False, hidden_act="silu", bos_token_id=0, eos_token_id=0), "Q8_0", seed=7)
+    m = Model.load_stablelm(cfg, tensors)
+    opened = []
+    try:
+        parent = m.session(kv)
+        opened.append(parent)
+        parent.forward(0, prompt_ids(300, cfg["vocab_size"], seed=1), want_logits=False)
+        groups = []
+        for _ in range(2):  # the same forks twice: shared and not
+            forks = [parent.fork() for _ in range(7)]
+            opened.extend(forks)
+            for i, f in enumerate(forks):  # ragged continuations of 0 to 40 tokens
+                if i:
+                    f.forward(300, prompt_ids(i * 7 - 2, cfg["vocab_size"], seed=20 + i), want_logits=False)
+            groups.append(forks)
+        shared, plain = m.batch(8), m.batch(8)
+        opened.extend([shared, plain])
+        shared.share_prefix(256)
+        toks = prompt_ids(7, cfg["vocab_size"], seed=9)
+        for step in range(5):
+            if step == 3:
+                shared.share_prefix(0)
+            rows, ids = shared.forward(groups[0], toks)
+            want, want_ids = plain.forward(groups[1], toks)
+            for i in range(7):
+                span = float(np.max(want[i]) - np.min(want[i]))
+                assert float(np.max(np.abs(rows[i] - want[i]))) <= 1e-4 * span, (step, i)
+            toks = want_ids.astype(np.int32)
+        shared.share_prefix(256)
+        other = m.session(kv)
+        opened.append(other)
+        other.forward(0, prompt_ids(40, cfg["vocab_size"], seed=3), want_logits=False)
+        rows, _ = shared.forward([groups[0][0], other], toks[:2])  # nothing in common
+        want = other.forward(40, [int(toks[1])])  # the batch step's own position once more
+        assert float(np.max(np.abs(rows[1] - want))) <= 1e-4 * float(np.max(want) - np.min(want))
+        with pytest.raises(BackendError):
+            shared.share_prefix(-1)
+    finally:
+        for x in reversed(opened):
+            x.close()
+        m.close()

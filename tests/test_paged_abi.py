@@ -123,9 +123,15 @@ def test_workspace_sizes_need_no_gpu():
     assert _lib.lib().tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries()), 0, 0, C.byref(n)) == _lib.TCU_OK
     assert n.value > 0
     small = n.value
-    assert _lib.lib().tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries(rows=64, requests=64)), 0, 0, C.byref(n)) == _lib.TCU_OK
+    # Parts of one row that no cluster joins.
+    long = dict(table_width=4096, table_stride=4096)
+    assert _lib.lib().tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries(**long)), 0, 0, C.byref(n)) == _lib.TCU_OK
     assert n.value > small
     assert _lib.lib().tcu_paged_attend_sparse_workspace(C.byref(kv()), C.byref(queries()), 1, 1, 4, C.byref(n)) == _lib.TCU_OK
+
+
+def test_share_prefix_needs_a_batch():
+    refused(_lib.lib().tcu_batch_share_prefix(None, 64), _lib.TCU_EINVAL, "null argument")
 
 
 def test_valid_calls_reach_the_device_check():

@@ -437,6 +437,12 @@ class Batch:
                                       ids.ctypes.data_as(C.POINTER(C.c_int32))))
         return rows, ids
 
+    def share_prefix(self, min_positions):
+        """Steps whose sessions all begin with the same pages (forks), at
+        least min_positions positions of them, read those once for all rows
+        (tcu_batch_share_prefix); 0 turns it off."""
+        check(lib().tcu_batch_share_prefix(self._h, min_positions))
+
     def sample_candidates(self, histories, k, penalties=None):
         """tcu_batch_sample_candidates over the last step's rows: histories is
         one id list per row, penalties one dict per row (or None: neutral).

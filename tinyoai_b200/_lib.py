@@ -23,7 +23,7 @@ EXPORTS = [
     "tcu_tp_unique_id", "tcu_stablelm_load_tp", "tcu_tp_plan", "tcu_tp_exchange_handle", "tcu_tp_exchange_open",
     "tcu_gguf_open", "tcu_gguf_config", "tcu_gguf_tensor_count", "tcu_gguf_tensor", "tcu_gguf_load_stablelm", "tcu_gguf_close",
     "tcu_session_save_cache", "tcu_session_load_cache",
-    "tcu_plan_step", "tcu_paged_append", "tcu_paged_means", "tcu_paged_attend_workspace", "tcu_paged_attend",
+    "tcu_batch_share_prefix", "tcu_plan_step", "tcu_paged_append", "tcu_paged_means", "tcu_paged_attend_workspace", "tcu_paged_attend",
     "tcu_paged_attend_sparse_workspace", "tcu_paged_attend_sparse",
 ]
 
@@ -153,6 +153,7 @@ def lib():
     i32, i64, u64p = C.c_int32, C.c_int64, C.POINTER(C.c_uint64)
     kvp, qp = C.POINTER(PagedKV), C.POINTER(PagedQueries)
     sig |= {
+        "tcu_batch_share_prefix": ([P, i32], C.c_int),
         "tcu_plan_step": ([i32, P, i32, P, P, i32, P, i32, i64, P, i32, i32, P, P, P, P, P], C.c_int),
         "tcu_paged_append": ([i32, P, kvp, i32, i32, i32, P, i64, P, P, C.POINTER(Rotary), C.POINTER(HeadNorm), P, i64], C.c_int),
         "tcu_paged_means": ([i32, P, kvp, i32, P, P], C.c_int),

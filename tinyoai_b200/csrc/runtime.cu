@@ -919,6 +919,9 @@ struct Work {
   float* xdn = nullptr;
   // Branch steps: leading history splits whose pages every row shares.
   int shared_splits = 0;
+  // Batch steps whose rows share a prefix (tcu_batch_share_prefix): the
+  // step's attention goes to the paged operators while this is set.
+  struct SharedStep* share = nullptr;
   uint32_t* adig = nullptr;
   float* asx = nullptr;
   int asx_stride = 0;
@@ -1633,8 +1636,76 @@ static size_t attn_decode_smem(const tcu_model* m) {
   return sizeof(float) * ((size_t)G * hd + 2 * (size_t)split * (hd + 1) + (size_t)G * split + 2 * hd);
 }
 
+// Attention of a batch step through the paged operators: the rows are
+// rotated and appended by tcu_paged_append, and tcu_paged_attend reads the
+// pages all rows begin with once. Lives in the batch; device buffers.
+struct SharedStep {
+  float* q = nullptr;        // [max_rows][aw]
+  int64_t* slots = nullptr;  // [max_rows]
+  int* starts = nullptr;     // 0, 1, ... max_rows
+  int* lengths = nullptr;    // [max_rows]
+  void* workspace = nullptr;
+  uint64_t workspace_bytes = 0;
+  int pages = 0, max_length = 0;  // of the step
+  int rc = TCU_OK;                // first failure of the step's launches
+};
+
+static tcu_paged_kv shared_kv(const KVPool* pool, int layer) {
+  const size_t off = (size_t)layer * pool->num_pages * pool->page_elems() * pool->elem();
+  tcu_paged_kv kv{};
+  kv.k = (uint8_t*)pool->k + off;
+  kv.v = (uint8_t*)pool->v + off;
+  kv.dtype = pool->half ? TCU_F16 : TCU_F32;
+  kv.num_pages = pool->num_pages;
+  kv.page_tokens = pool->P;
+  kv.kv_heads = pool->kvh;
+  kv.head_dim = pool->hd;
+  kv.page_stride = (int64_t)pool->page_elems();
+  kv.head_stride = (int64_t)pool->P * pool->hd;
+  kv.token_stride = pool->hd;
+  return kv;
+}
+
+static tcu_paged_queries shared_queries(const tcu_model* m, const Work* w, int M) {
+  tcu_paged_queries q{};
+  q.dtype = TCU_F32;
+  q.requests = q.rows = M;
+  q.heads = m->H;
+  q.max_fresh = 1;
+  q.table_width = w->pt_stride;
+  q.table_stride = w->pt_stride;
+  q.q = w->share->q;
+  q.q_token_stride = m->aw;
+  q.q_head_stride = m->hd;
+  q.out = w->ah;
+  q.out_token_stride = m->aw + m->ff;
+  q.out_head_stride = m->hd;
+  q.starts = w->share->starts;
+  q.lengths = w->share->lengths;
+  q.tables = w->pt;
+  q.scale = (float)(1.0 / sqrt((double)m->hd));
+  return q;
+}
+
+static int enqueue_shared_attention(const tcu_model* m, KVPool* pool, Work* w, int M, int layer, cudaStream_t s) {
+  SharedStep& sh = *w->share;
+  const tcu_paged_kv kv = shared_kv(pool, layer);
+  const tcu_paged_queries q = shared_queries(m, w, M);
+  const tcu_rotary rot{reinterpret_cast<const float*>(m->rope.table), m->max_pos, m->rope.pairs, m->rope.mode == 1};
+  TRY(tcu_paged_append(m->device, s, &kv, TCU_F32, M, m->H, w->qkv, m->aw + 2 * m->kvw, w->pos, sh.slots, &rot, nullptr, sh.q, m->aw));
+  // Row 0's table begins with the shared pages.
+  return tcu_paged_attend(m->device, s, &kv, &q, w->pt, sh.pages, sh.max_length, sh.workspace, sh.workspace_bytes);
+}
+
 static void launch_attn_decode(const tcu_model* m, KVPool* pool, Work* w, int M, int layer, int grid_splits, cudaStream_t s) {
   PROF_BEGIN(ST_ATTN, s);
+  if (w->share) {
+    const int rc = enqueue_shared_attention(m, pool, w, M, layer, s);
+    if (rc != TCU_OK && w->share->rc == TCU_OK) w->share->rc = rc;
+    NOTE("paged attention");
+    PROF_END(s);
+    return;
+  }
   DecodeAttnArgs a;
   a.M = M;
   a.H = m->H;
@@ -3540,9 +3611,97 @@ struct tcu_batch {
   int last_rows = 0;  // rows of the last successful step (their logits stay in w->logits)
   Work* w = nullptr;  // from the model's workspace pool (work_take)
   cudaStream_t stream = nullptr;
+  int share_min = 0;  // shared positions from which the paged operators attend; 0: never
+  SharedStep share;
 };
 
+// Pages that every session's table begins with, all of them behind the
+// positions the step writes.
+static int common_pages(const KVPool* pool, tcu_session* const* sessions, int n) {
+  size_t common = SIZE_MAX;
+  const std::vector<int>& first = sessions[0]->pages;
+  for (int i = 0; i < n; i++) {
+    common = std::min(common, (size_t)(sessions[i]->length / pool->P));
+    common = std::min({common, first.size(), sessions[i]->pages.size()});
+    for (size_t j = 0; j < common; j++)
+      if (sessions[i]->pages[j] != first[j]) common = j;
+  }
+  return (int)common;
+}
+
+// Uploads the step's slots and lengths and reserves its workspace.
+static int share_step(tcu_batch* b, KVPool* pool, tcu_session* const* sessions, int n, int pages, int max_len) {
+  SharedStep& sh = b->share;
+  std::vector<int64_t> slots(n);
+  std::vector<int> lengths(n);
+  for (int i = 0; i < n; i++) {
+    const int pos = sessions[i]->length;
+    slots[i] = (int64_t)sessions[i]->pages[pos / pool->P] * pool->P + pos % pool->P;
+    lengths[i] = pos + 1;
+  }
+  CK(cudaMemcpyAsync(sh.slots, slots.data(), n * sizeof(int64_t), cudaMemcpyHostToDevice, b->stream));
+  CK(cudaMemcpyAsync(sh.lengths, lengths.data(), n * sizeof(int), cudaMemcpyHostToDevice, b->stream));
+  sh.pages = pages;
+  sh.max_length = max_len;
+  sh.rc = TCU_OK;
+  b->w->share = &sh;
+  const tcu_paged_kv kv = shared_kv(pool, 0);
+  const tcu_paged_queries q = shared_queries(b->m, b->w, n);
+  uint64_t bytes = 0;
+  TRY(tcu_paged_attend_workspace(&kv, &q, pages, max_len, &bytes));
+  if (bytes > sh.workspace_bytes) {
+    CK(cudaStreamSynchronize(b->stream));
+    if (sh.workspace) cudaFree(sh.workspace);
+    sh.workspace = nullptr;
+    sh.workspace_bytes = 0;
+    if (cudaMalloc(&sh.workspace, bytes) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(TCU_ENOMEM, "%llu bytes for a shared-prefix step", (unsigned long long)bytes);
+    }
+    sh.workspace_bytes = bytes;
+  }
+  return TCU_OK;
+}
+
+static void share_free(tcu_batch* b) {
+  for (void* p : {(void*)b->share.q, (void*)b->share.slots, (void*)b->share.starts, (void*)b->share.lengths, b->share.workspace})
+    if (p) cudaFree(p);
+  b->share = SharedStep();
+  b->share_min = 0;
+}
+
 extern "C" {
+
+int tcu_batch_share_prefix(tcu_batch* b, int32_t min_positions) {
+  if (!b) return fail(TCU_EINVAL, "null argument");
+  if (min_positions < 0) return fail(TCU_EINVAL, "min_positions %d", min_positions);
+  tcu_model* m = b->m;
+  CK(cudaSetDevice(m->device));
+  if (min_positions > 0 && b->share_min == 0) {
+    if (m->tp_world > 1) return fail(TCU_EUNSUP, "a tensor-parallel model does not share prefixes in a batch");
+    if (m->hd % 8 || (m->aw + m->ff) % 4) return fail(TCU_EUNSUP, "head size %d or MLP width %d does not suit the paged operators", m->hd, m->ff);
+    std::vector<int> iota(b->max_rows + 1);
+    for (int i = 0; i <= b->max_rows; i++) iota[i] = i;
+    SharedStep& sh = b->share;
+    const size_t n = (size_t)b->max_rows;
+    if (cudaMalloc((void**)&sh.q, n * m->aw * sizeof(float)) != cudaSuccess || cudaMalloc((void**)&sh.slots, n * sizeof(int64_t)) != cudaSuccess ||
+        cudaMalloc((void**)&sh.starts, (n + 1) * sizeof(int)) != cudaSuccess || cudaMalloc((void**)&sh.lengths, n * sizeof(int)) != cudaSuccess) {
+      cudaGetLastError();
+      share_free(b);
+      return fail(TCU_ENOMEM, "buffers of a shared-prefix step");
+    }
+    cudaError_t e = cudaMemcpy(sh.starts, iota.data(), iota.size() * sizeof(int), cudaMemcpyHostToDevice);
+    if (e != cudaSuccess) {
+      share_free(b);
+      return fail(TCU_ECUDA, "starts copy: %s", cudaGetErrorString(e));
+    }
+  } else if (min_positions == 0) {
+    if (b->stream) cudaStreamSynchronize(b->stream);
+    share_free(b);
+  }
+  b->share_min = min_positions;
+  return TCU_OK;
+}
 
 int tcu_batch_open(tcu_model* m, int32_t max_rows, tcu_batch** out) {
   if (!m || !out) return fail(TCU_EINVAL, "null argument");
@@ -3602,9 +3761,15 @@ int tcu_batch_forward(tcu_batch* b, tcu_session* const* sessions, const int32_t*
     cudaMemsetAsync(b->w->argmax, 0, n * sizeof(unsigned long long), b->stream);
     const int split = SPLIT_PAGES * m->P;
     b->w->shared_splits = 0;
-    enqueue_decode(m, pool, b->w, n, false, (max_len + split - 1) / split, true, b->stream);
+    if (b->share_min > 0 && n > 1) {
+      const int pages = common_pages(pool, sessions, n);
+      if ((int64_t)pages * pool->P >= b->share_min) rc = share_step(b, pool, sessions, n, pages, max_len);
+    }
+    if (rc == TCU_OK) enqueue_decode(m, pool, b->w, n, false, (max_len + split - 1) / split, true, b->stream);
+    if (rc == TCU_OK && b->w->share) rc = b->w->share->rc;
+    b->w->share = nullptr;
     cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) rc = fail(TCU_ECUDA, "launch: %s", cudaGetErrorString(e));
+    if (e != cudaSuccess && rc == TCU_OK) rc = fail(TCU_ECUDA, "launch: %s", cudaGetErrorString(e));
     if (rc == TCU_OK) rc = comm_check();
     if (rc == TCU_OK && rows_out) {
       e = cudaMemcpyAsync(rows_out, b->w->logits, (size_t)n * m->V * 4, cudaMemcpyDeviceToHost, b->stream);
@@ -3652,6 +3817,7 @@ int tcu_batch_close(tcu_batch* b) {
     cudaStreamSynchronize(b->stream);
     cudaStreamDestroy(b->stream);
   }
+  share_free(b);
   work_give(b->m, b->w);
   delete b;
   return TCU_OK;
