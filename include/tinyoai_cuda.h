@@ -532,8 +532,8 @@ typedef struct {
  * read. prefix_pages 0: nothing is shared. max_length bounds the requests'
  * lengths (0: what the tables and the prefix map); positions from it on are
  * not attended. workspace: at least the bytes that the _workspace call
- * reports for the same arguments (it reads no device memory), 256-byte
- * aligned, its content irrelevant before and after; calls that may run at
+ * reports for the same arguments (it reads no device memory; 0: the call
+ * needs none and workspace may be NULL), 256-byte aligned, its content irrelevant before and after; calls that may run at
  * the same time (two streams, two captured graphs) need one each. */
 int tcu_paged_attend_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* queries, int32_t prefix_pages, int32_t max_length,
                                uint64_t* bytes);

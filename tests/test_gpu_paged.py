@@ -899,15 +899,18 @@ def test_refusals():
     bad(lambda: paged.StepPlan(1, 1, 16, "cpu"), "lives on a GPU")
     bad(lambda: paged.StepPlan(1, 1, 16, DEV).build(i32([1, 2]), i32([1, 2]), t, i32([])), "room for 1")
     # A workspace that is too small or not aligned, and host memory, at the C entry.
-    out, qs = c._queries(q, t, st, le, 1, None, None)
+    wide = torch.zeros((1, 4096), dtype=torch.int32, device=DEV)
+    out, qs = c._queries(q, wide, st, le, 1, None, None)
     L = _lib.lib()
-    w = torch.empty(1 << 16, dtype=torch.uint8, device=DEV)
+    w = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
     assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, w.data_ptr(), 16) == _lib.TCU_EINVAL
     assert b"workspace of 16 bytes" in L.tcu_last_error()
-    assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, w.data_ptr() + 16, 1 << 15) == _lib.TCU_EINVAL
-    host = torch.zeros(1 << 16, dtype=torch.uint8)
-    assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, (host.data_ptr() + 255) // 256 * 256, 1 << 15) == _lib.TCU_EINVAL
-    assert L.tcu_paged_attend(7, None, c._ref, qs, None, 0, 0, w.data_ptr(), 1 << 16) == _lib.TCU_ENODEV
+    assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, w.data_ptr() + 16, 1 << 19) == _lib.TCU_EINVAL
+    assert b"256-byte aligned" in L.tcu_last_error()
+    host = torch.zeros(1 << 20, dtype=torch.uint8)
+    assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, (host.data_ptr() + 255) // 256 * 256, 1 << 19) == _lib.TCU_EINVAL
+    assert b"device memory" in L.tcu_last_error()
+    assert L.tcu_paged_attend(7, None, c._ref, qs, None, 0, 0, w.data_ptr(), 1 << 20) == _lib.TCU_ENODEV
     # Nothing to do is not an error.
     none = torch.zeros((0, 4, 64), dtype=torch.float16, device=DEV)
     assert c.attend(none, t[:0], i32([0]), i32([]), 1).shape == (0, 4, 64)

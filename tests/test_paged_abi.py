@@ -121,8 +121,8 @@ def test_plan():
 def test_workspace_sizes_need_no_gpu():
     n = C.c_uint64()
     assert _lib.lib().tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries()), 0, 0, C.byref(n)) == _lib.TCU_OK
-    assert n.value > 0
     small = n.value
+    assert small == 0  # one part: the output is written at once
     # Parts of one row that no cluster joins.
     long = dict(table_width=4096, table_stride=4096)
     assert _lib.lib().tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries(**long)), 0, 0, C.byref(n)) == _lib.TCU_OK

@@ -1002,8 +1002,8 @@ __device__ __forceinline__ int own_parts(const AttendArgs& a, int pos) {
 }
 
 // Adds up the parts of one row (warp per row): out = sum_j w_j o_j / sum_j w_j
-// l_j with w_j = 2^(m_j - max m), in part order; a part without weight is not
-// read. grid: x = request * max_fresh + query, y = heads / 4.
+// l_j with w_j = 2^(m_j - max m), in part order; a part without weight adds
+// nothing, whatever it holds. grid: x = request * max_fresh + query, y = heads / 4.
 template <typename TQ, int LIST>
 __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
   pdl_wait();
@@ -1035,14 +1035,14 @@ __global__ void __launch_bounds__(128) k_attend_join(AttendArgs a) {
         float4 x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-          wp[e] = __shfl_sync(0xffffffffu, w, (p1 + e) & 31);
-          l = fmaf(__shfl_sync(0xffffffffu, mine.y, (p1 + e) & 31), wp[e], l);
-          if (p1 + e >= n) wp[e] = 0.f;
-          x[e] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (wp[e] != 0.f && d < a.hd) x[e] = *reinterpret_cast<const float4*>(po + (int64_t)(p0 + p1 + e) * a.hd + d);
+          // Not held back by the part's statistics, which are on their way too.
+          x[e] = p1 + e < n && d < a.hd ? *reinterpret_cast<const float4*>(po + (int64_t)(p0 + p1 + e) * a.hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) {
+          wp[e] = __shfl_sync(0xffffffffu, w, (p1 + e) & 31);
+          l = fmaf(__shfl_sync(0xffffffffu, mine.y, (p1 + e) & 31), wp[e], l);
+          if (wp[e] == 0.f) continue;
           s.x = fmaf(x[e].x, wp[e], s.x);
           s.y = fmaf(x[e].y, wp[e], s.y);
           s.z = fmaf(x[e].z, wp[e], s.z);

@@ -14,7 +14,8 @@
 // covers the other's products: two tiles of rows over the same blocks
 // (more than 128 rows) or one tile of rows over alternate blocks, each
 // stream then leaving a partial result of its own. Warps 0-3 and 4-7 are the
-// streams' softmax, warp 8 issues the TMA loads, warp 9 the products.
+// streams' softmax, warp 8 issues the TMA loads (from the moment the page ids
+// are there, while the others bring the queries), warp 9 the products.
 //
 // A row's reference m moves only when a block's maximum passes it by more
 // than 2^8 (weights up to 256 fit both types), which spares the
@@ -58,7 +59,7 @@ struct PtShared {
   uint64_t k_full[PT_MAX_STAGES], k_empty[PT_MAX_STAGES], v_full[PT_MAX_STAGES], v_empty[PT_MAX_STAGES];
   uint64_t s_full[2], p_full[2], o_done[2];
   uint32_t tmem;
-  int err, bad;
+  int err;
   int row[2 * PT_ROWS], limit[2 * PT_ROWS];
   int ids[PT_IDS];
 };
@@ -163,7 +164,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
   const int tiles = p.split_keys ? 1 : 2;
 
   // The rows, the page ids, the barriers.
-  int valid = 0;
+  int valid = 0, none = 0;
   if (tid < tiles * PT_ROWS) {
     const int row = blockIdx.x * tiles * PT_ROWS + tid;
     const Query q = query_of(a, row / a.G);
@@ -171,24 +172,20 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     sh.limit[tid] = q.token < 0 ? -1 : q.pos;
     valid = q.token >= 0;
   }
-  if (tid == 0) {
-    sh.err = 0;
-    sh.bad = 0;
-  }
-  if (!__syncthreads_or(valid)) return;  // padding rows only
+  const int first = (int)a.kv.divP.div(blk0 * PT_KEYS);
   {
-    const int first = (int)a.kv.divP.div(blk0 * PT_KEYS);
     const int last = (int)a.kv.divP.div(min(prefix_end, (blk0 + nblk) * PT_KEYS) - 1);
     for (int e = tid; e <= last - first; e += PT_THREADS) {
       int id = a.prefix[first + e];
       if (id < 0 || id >= a.kv.num_pages) {
         id = -1;
-        sh.bad = 1;
+        none = 1;
       }
       sh.ids[e] = id;
     }
   }
   if (tid == 0) {
+    sh.err = 0;
     for (int i = 0; i < p.stages; i++) {
       mbar_init(&sh.k_full[i], 1);
       mbar_init(&sh.k_empty[i], 1);
@@ -202,32 +199,37 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     }
     fence_barrier_init();
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  // Queries, swizzled as the descriptors read them; a negative scale is taken
-  // into their sign, so that the largest score is the largest S.
-  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-  for (int e = tid; e < tiles * PT_ROWS * SUB * 8; e += PT_THREADS) {
-    const int rr = e / (SUB * 8), ch = e % (SUB * 8), row = sh.row[rr], d = ch * 8;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (row >= 0 && d < a.hd)
-      x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
-    x.x ^= flip;
-    x.y ^= flip;
-    x.z ^= flip;
-    x.w ^= flip;
-    const int t = rr / PT_ROWS, r = rr % PT_ROWS;
-    *reinterpret_cast<uint4*>(qs + (size_t)(t * SUB + (ch >> 3)) * PT_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  if (!__syncthreads_or(valid)) return;  // padding rows only
+  const bool bad = __syncthreads_or(none) != 0;
   // TMEM columns: S of stream t at t * 128, P over its second half, O of stream t at 256 + t * 128.
   const int count[2] = {p.split_keys ? (nblk + 1) / 2 : nblk, p.split_keys ? nblk / 2 : nblk};
+  uint32_t tmem = 0;
+  if (warp != 8) {  // the loads of keys and values begin at once
+    if (warp == 9) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // Queries, swizzled as the descriptors read them; a negative scale is taken
+    // into their sign, so that the largest score is the largest S.
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    for (int e = tid < 256 ? tid : tiles * PT_ROWS * SUB * 8; e < tiles * PT_ROWS * SUB * 8; e += 256) {
+      const int rr = e / (SUB * 8), ch = e % (SUB * 8), row = sh.row[rr], d = ch * 8;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (row >= 0 && d < a.hd)
+        x = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs + d);
+      x.x ^= flip;
+      x.y ^= flip;
+      x.z ^= flip;
+      x.w ^= flip;
+      const int t = rr / PT_ROWS, r = rr % PT_ROWS;
+      *reinterpret_cast<uint4*>(qs + (size_t)(t * SUB + (ch >> 3)) * PT_SUB + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc_fence_before();
+    named_bar_sync(1, PT_THREADS - 32);
+    tc_fence_after();
+    tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
+  }
 
   if (warp == 8) {
     if (lane == 0) {
@@ -248,7 +250,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
           for (int x = 0; x < boxes; x++) {
             const int key = key0 + x * p.box;
             const int pg = (int)a.kv.divP.div(key), row0 = key - pg * a.kv.P;
-            int id = key < prefix_end ? sh.ids[pg - (int)a.kv.divP.div(blk0 * PT_KEYS)] : -1;
+            int id = key < prefix_end ? sh.ids[pg - first] : -1;
             if (id < 0) id = a.kv.num_pages;  // behind the pool: zeros
             for (int s = 0; s < SUB; s++) pt_load(dst + (size_t)s * PT_SUB + x * p.box * 128, kv ? &vmap : &kmap, s * 64, row0, g, id, full);
           }
@@ -348,7 +350,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
       constexpr int HALF = PT_KEYS / 2;
       uint32_t s[HALF];
       const int seen = min(limit, prefix_end - 1) - key0;  // columns up to here are this row's
-      const bool special = sh.bad || __any_sync(0xffffffffu, seen < PT_KEYS - 1);
+      const bool special = bad || __any_sync(0xffffffffu, seen < PT_KEYS - 1);
       auto load = [&](int half) {
         tc_ld32(ts + half * HALF, s);
         tc_ld32(ts + half * HALF + 32, s + 32);
@@ -415,7 +417,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
   }

@@ -124,10 +124,10 @@ class StepPlan:
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.max_requests, self.capacity, self.page_tokens = max_requests, capacity, page_tokens
-        words = torch.zeros(2 * max_requests + 4 + capacity, dtype=torch.int32, device=self.device)
+        words = torch.empty(2 * max_requests + 4 + capacity, dtype=torch.int32, device=self.device)
         self._starts, self._lengths, self.counts, self.positions = words.split([max_requests + 1, max_requests, 3, capacity])
         self.starts, self.lengths = self._starts, self._lengths
-        self.slots = torch.zeros(capacity, dtype=torch.int64, device=self.device)
+        self.slots = torch.empty(capacity, dtype=torch.int64, device=self.device)
         self.index, self._n, self._call = self.device.index, max_requests, lib().tcu_plan_step
         self._outs = tuple(t.data_ptr() for t in (self._starts, self._lengths, self.positions, self.slots, self.counts))
 
@@ -231,8 +231,8 @@ class Cache:
         key = ("attend", q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
         sized = self._sized  # one read: another thread may replace it
         size = sized[1] if sized[0] == key else self._size(key, self._lib.tcu_paged_attend_workspace, ref, pages, max_length)
-        work = self._workspace(size, stream)
-        check(self._lib.tcu_paged_attend(index, _stream(stream, index), self._ref, ref, at, pages, max_length, work.data_ptr(), size))
+        work = self._workspace(size, stream) if size else None
+        check(self._lib.tcu_paged_attend(index, _stream(stream, index), self._ref, ref, at, pages, max_length, work.data_ptr() if size else None, size))
         return out
 
     def attend_sparse(self, q, means, tables, starts, lengths, max_fresh, top, first=1, last=1, scale=None, out=None, pages=None, stream=None):
