@@ -354,8 +354,8 @@ int tcu_batch_sample_candidates(tcu_batch* batch, int32_t n, const int32_t* hist
  * instead of row by row. 0 (the default) turns it off. The rows then differ
  * from the unshared step's by float32 rounding, not in what they compute.
  * Allocates the step's buffers; a step whose workspace has to grow allocates
- * again. Not for tensor-parallel models (TCU_EUNSUP), nor for head sizes that
- * are not a multiple of 8. */
+ * again. Not for tensor-parallel models, nor for shapes outside the limits of
+ * the operators below (TCU_EUNSUP). */
 int tcu_batch_share_prefix(tcu_batch* batch, int32_t min_positions);
 int tcu_batch_close(tcu_batch* batch);
 
@@ -425,6 +425,7 @@ int tcu_shortlist_static(int32_t device, const float* logits, int32_t vocab, int
 #define TCU_PAGED_MAX_GROUP 64           /* query heads per KV head */
 #define TCU_PAGED_MAX_PAGE_TOKENS 65536
 #define TCU_PAGED_MAX_SELECTED 65536     /* first + last + top of a sparse call */
+/* Tables, prefixes and selections map at most 2^30 positions. */
 
 /* Value d of position r of page p, KV head g of k (and of v) is at
  * p * page_stride + g * head_stride + r * token_stride + d. */

@@ -855,9 +855,8 @@ def test_two_streams_at_once():
     want2 = c.attend(q2, s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"]).clone()
     torch.cuda.synchronize()
     one, two = torch.cuda.Stream(), torch.cuda.Stream()
-    outs = [(torch.empty_like(want1), torch.empty_like(want2)) for _ in range(20)]
+    outs = [(c.attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], stream=one), torch.empty_like(want2)) for _ in range(20)]
     for x, y in outs:
-        c.attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], out=x, stream=one)
         with torch.cuda.stream(two):
             c.attend(q2, s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], out=y)
     torch.cuda.synchronize()
@@ -900,7 +899,7 @@ def test_refusals():
     bad(lambda: paged.StepPlan(1, 1, 16, DEV).build(i32([1, 2]), i32([1, 2]), t, i32([])), "room for 1")
     # A workspace that is too small or not aligned, and host memory, at the C entry.
     wide = torch.zeros((1, 4096), dtype=torch.int32, device=DEV)
-    out, qs = c._queries(q, wide, st, le, 1, None, None)
+    out, qs = c._queries(q, wide, st, le, 1, None, None, None)
     L = _lib.lib()
     w = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
     assert L.tcu_paged_attend(0, None, c._ref, qs, None, 0, 0, w.data_ptr(), 16) == _lib.TCU_EINVAL

@@ -61,7 +61,7 @@ def test_caches(over, code, text):
     (dict(requests=-1), _lib.TCU_EINVAL, "negative count"),
     (dict(rows=-1), _lib.TCU_EINVAL, "negative count"),
     (dict(table_stride=1), _lib.TCU_EINVAL, "table stride"),
-    (dict(table_width=1 << 27, table_stride=1 << 27), _lib.TCU_EINVAL, "pass 2^31"),
+    (dict(table_width=1 << 27, table_stride=1 << 27), _lib.TCU_EINVAL, "pass 2^30"),
     (dict(requests=1 << 20, max_fresh=1 << 12), _lib.TCU_EINVAL, "too many rows"),
     (dict(q_token_stride=260), _lib.TCU_EINVAL, "multiples of 16 bytes"),
     (dict(out_head_stride=-64), _lib.TCU_EINVAL, "negative query stride"),
@@ -80,6 +80,8 @@ def test_other_arguments():
     refused(sparse(kv(), queries(), last=0), _lib.TCU_EINVAL, "at least 1")
     refused(sparse(kv(), queries(), first=-1), _lib.TCU_EINVAL, "must not be negative")
     refused(sparse(kv(), queries(), top=65536), _lib.TCU_EINVAL, "pages a query")
+    refused(sparse(kv(page_tokens=65536, token_stride=64, head_stride=1 << 22, page_stride=1 << 23), queries(), top=30000), _lib.TCU_EINVAL, "pass 2^30")
+    refused(attend(kv(), queries(), pages=1 << 27), _lib.TCU_EINVAL, "prefix of")
     refused(L.tcu_paged_attend_workspace(None, None, 0, 0, C.byref(C.c_uint64())), _lib.TCU_EINVAL, "null cache")
     refused(L.tcu_paged_attend_workspace(C.byref(kv()), None, 0, 0, C.byref(C.c_uint64())), _lib.TCU_EINVAL, "null queries")
     refused(L.tcu_paged_attend_workspace(C.byref(kv()), C.byref(queries()), 0, 0, None), _lib.TCU_EINVAL, "null argument")

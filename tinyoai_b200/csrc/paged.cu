@@ -195,6 +195,10 @@ int launch_means(const MeansArgs& a, cudaStream_t s) {
 // ---------------------------------------------------------------------------
 // Attention
 
+// Positions of a request in attention: the end of a part, up to as long again,
+// stays a 32-bit number.
+constexpr int64_t MAX_POSITIONS = 1ll << 30;
+
 struct AttendPlan {
   int prefix_rows = 0, prefix_chunk = 0, prefix_slots = 0, own_rows = 0, own_chunk = 0, own_slots = 0, slots = 0;
   bool tc = false;      // the prefix on tcgen05
@@ -216,7 +220,7 @@ int chunk_of(int64_t positions, int64_t ctas_per_part, int P) {
   // Up to 4,096 positions: eight parts at most, which a cluster joins.
   if (positions <= 4096) c = std::max<int64_t>(c, ceil_div(ceil_div(positions, 8), 64) * 64);
   c = std::min<int64_t>(c, std::max<int64_t>(64, (int64_t)(MM_IDS - 2) * P / 64 * 64));
-  return (int)std::min<int64_t>(c, 1 << 30);
+  return (int)std::min<int64_t>(c, MAX_POSITIONS);
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -279,8 +283,9 @@ AttendPlan plan_attend(const tcu_paged_kv* kv, const tcu_paged_queries* q, int p
   const int64_t T = q->rows;
   if (budget > 0) {
     p.own_rows = rows_per_cta(kv, G);
-    p.own_chunk = chunk_of((int64_t)budget * P, T * kv->kv_heads * ceil_div(G, p.own_rows), P);
-    p.own_slots = (int)ceil_div((int64_t)budget * P, p.own_chunk);
+    const int64_t most = (int64_t)std::max(1, std::min(budget, q->table_width)) * P;  // a list holds no more pages than a table
+    p.own_chunk = chunk_of(most, T * kv->kv_heads * ceil_div(G, p.own_rows), P);
+    p.own_slots = (int)ceil_div(most, p.own_chunk);
   } else {
     const int64_t shared = (int64_t)prefix_pages * P;
     p.prefix_rows = rows_per_cta(kv, T * G);
@@ -497,7 +502,7 @@ int check_queries(const tcu_paged_kv* kv, const tcu_paged_queries* q) {
   if (q->heads / kv->kv_heads > TCU_PAGED_MAX_GROUP) return fail(TCU_EUNSUP, "%d query heads a KV head, at most %d", q->heads / kv->kv_heads, TCU_PAGED_MAX_GROUP);
   if (q->max_fresh < 1) return fail(TCU_EINVAL, "max_fresh %d", q->max_fresh);
   if (q->table_stride < q->table_width) return fail(TCU_EINVAL, "table stride %lld below the width %d", (long long)q->table_stride, q->table_width);
-  if ((int64_t)q->table_width * kv->page_tokens > 0x7fffffffll) return fail(TCU_EINVAL, "tables of %d pages pass 2^31 positions", q->table_width);
+  if ((int64_t)q->table_width * kv->page_tokens > MAX_POSITIONS) return fail(TCU_EINVAL, "tables of %d pages pass 2^30 positions", q->table_width);
   const int G = q->heads / kv->kv_heads;
   if ((int64_t)q->requests * q->max_fresh * G > 0x7fffffffll || (int64_t)q->rows * q->heads > 0x7fffffffll)
     return fail(TCU_EINVAL, "too many rows for one call");
@@ -561,7 +566,7 @@ int check_workspace(const AttendPlan& p, void* workspace, uint64_t bytes, int de
 }
 
 int check_prefix(const tcu_paged_kv* kv, int32_t prefix_pages, int32_t max_length) {
-  if (prefix_pages < 0 || (int64_t)prefix_pages * kv->page_tokens > 0x7fffffffll) return fail(TCU_EINVAL, "prefix of %d pages", prefix_pages);
+  if (prefix_pages < 0 || (int64_t)prefix_pages * kv->page_tokens > MAX_POSITIONS) return fail(TCU_EINVAL, "prefix of %d pages", prefix_pages);
   if (max_length < 0) return fail(TCU_EINVAL, "max_length %d", max_length);
   return TCU_OK;
 }
@@ -569,13 +574,15 @@ int check_prefix(const tcu_paged_kv* kv, int32_t prefix_pages, int32_t max_lengt
 // Positions a request can hold: what its table (or the prefix) maps.
 int length_bound(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_pages, int max_length) {
   const int64_t mapped = (int64_t)std::max(prefix_pages, q->table_width) * kv->page_tokens;
-  return (int)std::min<int64_t>(max_length > 0 ? std::min<int64_t>(max_length, mapped) : mapped, 0x7fffffff);
+  return (int)(max_length > 0 ? std::min<int64_t>(max_length, mapped) : mapped);
 }
 
-int check_sparse(const tcu_paged_queries* q, int32_t first, int32_t last, int32_t top) {
+int check_sparse(const tcu_paged_kv* kv, int32_t first, int32_t last, int32_t top) {
   if (first < 0 || last < 1 || top < 0) return fail(TCU_EINVAL, "first %d and top %d must not be negative, last %d must be at least 1", first, top, last);
   if ((int64_t)first + last + top > TCU_PAGED_MAX_SELECTED)
     return fail(TCU_EINVAL, "%lld pages a query, at most %d", (long long)first + last + top, TCU_PAGED_MAX_SELECTED);
+  if (((int64_t)first + last + top) * kv->page_tokens > MAX_POSITIONS)
+    return fail(TCU_EINVAL, "%lld pages of %d positions a query pass 2^30", (long long)first + last + top, kv->page_tokens);
   return TCU_OK;
 }
 
@@ -754,7 +761,7 @@ int tcu_paged_attend_sparse_workspace(const tcu_paged_kv* kv, const tcu_paged_qu
   if (!bytes) return fail(TCU_EINVAL, "null argument");
   TRY(check_kv(kv));
   TRY(check_queries(kv, q));
-  TRY(check_sparse(q, first, last, top));
+  TRY(check_sparse(kv, first, last, top));
   *bytes = plan_attend(kv, q, 0, 0, first + last + top).bytes;
   return TCU_OK;
 }
@@ -763,7 +770,7 @@ int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv
                             int32_t last, int32_t top, int32_t* pages, void* workspace, uint64_t workspace_bytes) {
   TRY(check_kv(kv));
   TRY(check_queries(kv, q));
-  TRY(check_sparse(q, first, last, top));
+  TRY(check_sparse(kv, first, last, top));
   OnDevice on(device);
   TRY(on.rc);
   if (q->requests == 0 || q->rows == 0) return TCU_OK;
@@ -773,7 +780,7 @@ int tcu_paged_attend_sparse(int32_t device, void* stream, const tcu_paged_kv* kv
   const AttendPlan p = plan_attend(kv, q, 0, 0, first + last + top);
   TRY(check_workspace(p, workspace, workspace_bytes, device));
   AttendArgs a = attend_args(kv, q, p, workspace);
-  a.max_length = (int)std::min<int64_t>((int64_t)q->table_width * kv->page_tokens, 0x7fffffff);
+  a.max_length = q->table_width * kv->page_tokens;
   a.pages = pages;
   a.budget = first + last + top;
   ChooseArgs c{};

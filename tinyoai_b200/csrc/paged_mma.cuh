@@ -183,7 +183,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
         int id = j >= 0 && j < a.width ? table[j] : -1;
         if (id >= a.kv.num_pages) id = -1;
         s_ids[e] = id;
-        s_first[e] = id < 0 ? 0x3fffffff : j * a.kv.P;
+        s_first[e] = id < 0 ? 0 : j * a.kv.P;
       }
     } else {
       const int* ids = SRC == SRC_PREFIX ? a.prefix : a.tables + (int64_t)request * a.table_stride;
@@ -219,6 +219,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
   const TK* kb = reinterpret_cast<const TK*>(a.kv.k) + (int64_t)g * a.kv.sh;
   const TK* vb = reinterpret_cast<const TK*>(a.kv.v) + (int64_t)g * a.kv.sh;
   const bool aligned = (a.kv.P & 15) == 0;  // a 16-position tile lies in one page
+  constexpr int NOWHERE = 0x7ffffff0;       // behind every position, with room for a tile
   for (int ub = u0 + warp * 16; ub < u1; ub += MM_WARPS * 16) {
     // Cache rows: positions r and r + 8 of the tile for K, 2c, 2c + 1, 2c + 8 and 2c + 9 for V.
     int64_t ko[2], vo[4];
@@ -226,7 +227,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
     if (aligned) {
       const int b = (int)a.kv.divP.div(ub), row0 = ub - b * a.kv.P, id = s_ids[b - b0];
       const int64_t base = (int64_t)id * a.kv.sp + (int64_t)row0 * a.kv.st;
-      const int t0 = id < 0 ? 0x3fffffff : SRC == SRC_LIST ? s_first[b - b0] + row0 : ub;
+      const int t0 = id < 0 ? NOWHERE : SRC == SRC_LIST ? s_first[b - b0] + row0 : ub;
 #pragma unroll
       for (int i = 0; i < 2; i++) {
         ko[i] = base + (int64_t)(r + 8 * i) * a.kv.st;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
     } else {
       auto at = [&](int u, int64_t& off, int& t) {
         off = 0;
-        t = 0x3fffffff;
+        t = NOWHERE;
         if (u >= u1) return;
         const int b = (int)a.kv.divP.div(u), row = u - b * a.kv.P, id = s_ids[b - b0];
         if (id < 0) return;

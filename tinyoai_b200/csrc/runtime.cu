@@ -3679,7 +3679,9 @@ int tcu_batch_share_prefix(tcu_batch* b, int32_t min_positions) {
   CK(cudaSetDevice(m->device));
   if (min_positions > 0 && b->share_min == 0) {
     if (m->tp_world > 1) return fail(TCU_EUNSUP, "a tensor-parallel model does not share prefixes in a batch");
-    if (m->hd % 8 || (m->aw + m->ff) % 4) return fail(TCU_EUNSUP, "head size %d or MLP width %d does not suit the paged operators", m->hd, m->ff);
+    if (m->hd % 8 || m->hd > TCU_PAGED_MAX_HEAD_DIM || (m->aw + m->ff) % 4 || m->H / m->KVH > TCU_PAGED_MAX_GROUP || m->P > TCU_PAGED_MAX_PAGE_TOKENS)
+      return fail(TCU_EUNSUP, "heads of %d values, %d a KV head, MLP width %d or pages of %d do not suit the paged operators", m->hd, m->H / m->KVH, m->ff,
+                  m->P);
     std::vector<int> iota(b->max_rows + 1);
     for (int i = 0; i <= b->max_rows; i++) iota[i] = i;
     SharedStep& sh = b->share;

@@ -15,8 +15,9 @@ mathematics, the types and the limits). A step over a cache:
 Every call queues its work on `stream` (a torch.cuda.Stream; None: torch's
 current stream of the cache's device) and returns. Nothing synchronises, so
 the calls can be captured into CUDA graphs; results and workspaces come from
-torch's allocator unless `out` is given. A tensor that was made on another
-stream has to be ordered with `stream` by the caller, as for any torch call.
+torch's allocator, on that stream, unless `out` is given. A tensor that was
+made on another stream has to be ordered with `stream` by the caller, as for
+any torch call. The operators serve; they record no gradients.
 Bad arguments raise BackendError with the library's TCU_EINVAL or TCU_EUNSUP.
 """
 import ctypes as C
@@ -59,6 +60,15 @@ _current = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index
 
 def _stream(stream, index):
     return _current(index) if stream is None else stream.cuda_stream
+
+
+def _new(like, shape, stream, dtype=None):
+    """A tensor from torch's allocator, which hands its memory out again only
+    to work behind this call on the stream it is used on."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _on_gpu(name, t):
@@ -185,7 +195,7 @@ class Cache:
             raise _bad(f"{rows} rows, {len(positions)} positions, {len(slots)} slots")
         stride = heads * hd
         if out is None:
-            out = qkv.new_empty((rows, heads, hd))
+            out = _new(qkv, (rows, heads, hd), stream)
         else:
             if out.shape != (rows, heads, hd) or out.dtype != qkv.dtype or out.device != d or out.stride(2) != 1 or (heads > 1 and out.stride(1) != hd):
                 raise _bad(f"out must be [{rows}, {heads}, {hd}] of {qkv.dtype} on {d}, its heads contiguous")
@@ -224,14 +234,14 @@ class Cache:
         (sizes the work; 0: what the tables map). Returns out [rows, heads,
         head size]; rows behind starts[-1] keep what `out` held."""
         index = self.index
-        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
+        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out, stream)
         pages, at = 0, None
         if prefix is not None:
             at, pages = _whole("prefix", prefix, torch.int32, self.device), len(prefix)
         key = ("attend", q.dtype, q.shape, tables.shape, max_fresh, pages, max_length)
         sized = self._sized  # one read: another thread may replace it
         size = sized[1] if sized[0] == key else self._size(key, self._lib.tcu_paged_attend_workspace, ref, pages, max_length)
-        work = self._workspace(size, stream) if size else None
+        work = _new(self.k, size, stream, torch.uint8) if size else None
         check(self._lib.tcu_paged_attend(index, _stream(stream, index), self._ref, ref, at, pages, max_length, work.data_ptr() if size else None, size))
         return out
 
@@ -243,18 +253,18 @@ class Cache:
         behind them."""
         d, index = self.device, self.index
         self._check_means(means)
-        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out)
+        out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out, stream)
         if min(first, top) < 0 or last < 1:
             raise _bad(f"first {first} and top {top} must not be negative, last {last} must be at least 1")
         shape = (q.shape[0], self.kv_heads, first + last + top)
         if pages is None:
-            pages = tables.new_empty(shape)
+            pages = _new(tables, shape, stream)
         elif pages.shape != shape or pages.dtype != torch.int32 or pages.device != d or not pages.is_contiguous():
             raise _bad(f"pages must be a contiguous int32 tensor {shape} on {d}")
         key = ("sparse", q.dtype, q.shape, tables.shape, max_fresh, first, last, top)
         sized = self._sized
         size = sized[1] if sized[0] == key else self._size(key, self._lib.tcu_paged_attend_sparse_workspace, ref, first, last, top)
-        work = self._workspace(size, stream)
+        work = _new(self.k, size, stream, torch.uint8)
         check(self._lib.tcu_paged_attend_sparse(index, _stream(stream, index), self._ref, ref, means.data_ptr(), first, last, top, pages.data_ptr(),
                                                 work.data_ptr(), size))
         return out, pages
@@ -266,18 +276,11 @@ class Cache:
         self._sized = (key, n.value)
         return n.value
 
-    def _workspace(self, size, stream):
-        """From torch's allocator, which hands it out again only to work behind this call on its stream."""
-        if stream is None:
-            return self.k.new_empty(size, dtype=torch.uint8)
-        with torch.cuda.stream(stream):
-            return self.k.new_empty(size, dtype=torch.uint8)
-
     def _check_means(self, means):
         if means.shape != self._means or means.dtype is not self.k.dtype or means.device != self.device or not means.is_contiguous():
             raise _bad(f"means must be a contiguous {self.k.dtype} tensor {tuple(self._means)} on {self.device}")
 
-    def _queries(self, q, tables, starts, lengths, max_fresh, scale, out):
+    def _queries(self, q, tables, starts, lengths, max_fresh, scale, out, stream):
         d, hd = self.device, self.head_dim
         if q.dim() != 3 or q.shape[2] != hd or q.device != d or q.stride(2) != 1:
             raise _bad(f"q must be [rows, heads, {hd}] on {d}, its last dimension contiguous, got {tuple(q.shape)} on {q.device}")
@@ -287,7 +290,7 @@ class Cache:
         if len(lengths) != n or len(starts) != n + 1:
             raise _bad(f"{n} tables, {len(lengths)} lengths, {len(starts)} starts")
         if out is None:
-            out = q.new_empty((rows, heads, hd))
+            out = _new(q, (rows, heads, hd), stream)
             ots, ohs = heads * hd, hd
         else:
             if out.shape != q.shape or out.dtype != q.dtype or out.device != d or out.stride(2) != 1:
