@@ -254,9 +254,13 @@ void plan_tc(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_page
   p->tc_tiles = (int)ceil_div(rows, split ? PT_ROWS : 2 * PT_ROWS);
   const int64_t units = (int64_t)p->tc_tiles * kv->kv_heads;
   const int64_t most = std::max<int64_t>(1, std::min<int64_t>(blocks, (int64_t)(PT_IDS - 2) * P / PT_KEYS));
-  // Blocks per part: waves of one CTA per SM, each block about 1.3 us (half
-  // of that where the streams share the blocks), three blocks' worth of
-  // set-up, and the join's traffic of every part.
+  // Blocks per part: waves of one CTA per SM, three blocks' worth of set-up,
+  // and the join's traffic of every part. A block takes 1.3 us on an SM whose
+  // products never wait (half of that where the streams share the blocks) and
+  // about 2.5 as they do; the lower figure stands because SMs that a short last
+  // wave leaves idle go to the requests' own positions: 256 requests over
+  // 32,768 positions take 242 us in 4 parts (128 CTAs), 273 in the 9 (288
+  // CTAs, 2 waves) that 2.5 would choose.
   double best = 1e30;
   const double join = 1e-6 * q->rows * q->heads * hd * 8 / 4.0 * (split ? 2 : 1);  // us a part at 4 TB/s
   for (int64_t parts = ceil_div(blocks, most); parts <= std::min<int64_t>(blocks, ceil_div(blocks, most) + 64); parts++) {
