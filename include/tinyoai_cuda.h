@@ -509,9 +509,10 @@ int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_
  * maps its pages. max_fresh is at least the largest starts[i + 1] - starts[i]
  * (later rows of a longer request are left as they were), and rows behind
  * starts[requests] are left as they were. A row at a negative position
- * attends to nothing and is zero. heads is a multiple of kv_heads; query head
- * h reads KV head h / (heads / kv_heads). The weight of position t is
- * softmax(scale * q . k_t). */
+ * attends to nothing and is zero. What lies at positions that a row does not
+ * attend to never reaches it, infinities and NaN among them. heads is a
+ * multiple of kv_heads; query head h reads KV head h / (heads / kv_heads). The
+ * weight of position t is softmax(scale * q . k_t). */
 typedef struct {
   int32_t dtype;
   int32_t requests, rows, heads, max_fresh;

@@ -318,7 +318,7 @@ def attention_ref(q, k, v, scale, visible):
     top = s.amax(-1, keepdim=True)
     w = torch.exp(s - torch.where(top.isinf(), 0.0, top))
     l = w.sum(-1, keepdim=True)
-    w = torch.where(l > 0, w / l, 0.0)
+    w = torch.where(l == 0, 0.0, w / l)
     return torch.einsum("rht,thd->rhd", w, v), torch.einsum("rht,thd->rhd", w, v.abs()), size.masked_fill(~mask, 0).amax(-1)
 
 
@@ -605,6 +605,43 @@ def test_attend_ignores_missing_pages_and_stale_values(qt, kt):
         want, tol = expected(s, lens, fresh, 4, 2, 64, 16, 1 / math.sqrt(64), 0)
         near(out[:3], want, tol)
         assert bool((out[2] == 0).all())
+
+
+UNSEEN = [
+    # lens, fresh, H, KVH, hd, P, prefix pages, (request, position) of the values that are no numbers
+    ([70, 300], [8, 5], 8, 2, 64, 16, 0, (0, 66)),                                # later tokens of a chunk
+    ([70, 300], [8, 5], 8, 2, 64, 16, 0, (1, 299)),                               # the last of all
+    ([3000], [40], 2, 1, 80, 7, 0, (0, 2965)),                                    # parts joined in a cluster, pages of 7
+    ([9000], [3], 4, 2, 256, 32, 0, (0, 8998)),                                   # and in a join of their own
+    ([40, 300, 33], [2, 4, 1], 4, 2, 128, 32, 4, (1, 100)),                       # requests shorter than a short prefix
+    ([2100] * 26 + [700, 1, 0, 1999], [1] * 30, 2, 2, 128, 16, 128, (0, 1200)),   # a prefix of its own kernel
+    ([2100] * 41 + [700, 1, 0, 1200, 1201], [1] * 46, 2, 2, 128, 16, 128, (0, 1200)),   # of tensor-core tiles: one tile
+    ([2100] * 41 + [700, 1, 0, 1200, 1201], [1] * 46, 8, 2, 80, 32, 64, (0, 2047)),     # two, the prefix's last position
+    ([700] * 40 + [1201] * 2, [1] * 42, 4, 2, 64, 8, 256, (40, 1200)),            # most see little of it
+]
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("case", range(len(UNSEEN)))
+def test_attend_values_of_unseen_positions(qt, kt, case):
+    """Infinities and NaN at a position that later rows of the step, or longer
+    requests, attend to stay out of the rows that do not."""
+    lens, fresh, H, KVH, hd, P, prefix, (i, x) = UNSEEN[case]
+    qt, kt = TYPES[qt], TYPES[kt]
+    for fill in (math.inf, math.nan):
+        s = attention_state(lens, fresh, H, KVH, hd, P, qt, kt, seed=50 + case, prefix=prefix)
+        page = (s["prefix"] if x // P < prefix else s["table"][i])[x // P].long()
+        s["v"][page, :, x % P, ::3] = fill
+        if fill != fill:
+            s["k"][page, 0, x % P, 1] = fill
+        out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], max(fresh), prefix=s["prefix"] if prefix else None,
+                                                 max_length=s["lim"])[:s["T"]]
+        want, tol = expected(s, lens, fresh, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
+        there = want.isfinite()
+        rows = there.all(-1).all(-1)
+        assert bool(rows.any()) and not bool(rows.all())
+        assert torch.equal(out.isfinite(), there)
+        near(out[there], want[there], (2 if max(lens) > 2000 else 1) * tol[there])  # long sums as above
 
 
 @pytest.mark.parametrize("qt, kt", PAIRS)

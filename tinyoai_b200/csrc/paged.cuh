@@ -723,6 +723,65 @@ __device__ __forceinline__ float ex2(float x) {
 // 1 / l, 0 for a row that saw nothing; NaN stays NaN.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
 
+// A matrix product takes in every position of its tile, those a row does not
+// attend to with weight 0; an infinity or NaN among their values makes the
+// row's sums NaN. Such rows (not finite, and short of the part's last
+// position) are summed again by this: a warp adds 2^(score - m) v over the
+// part's positions up to `last` one by one, score and m in units of log2, and
+// writes the sums to dst. The part is the tiles of `tile` positions every `step`
+// from u0 on, up to u1.
+template <typename TQ, typename TK, int HD, int SRC>
+__device__ __noinline__ void sum_row(const AttendArgs& a, int row, int g, int request, int u0, int u1, int tile, int step, int last, float m, float* dst) {
+  constexpr int NCH = (HD + 127) / 128;
+  const int lane = threadIdx.x & 31;
+  const TQ* qp = reinterpret_cast<const TQ*>(a.q) + (int64_t)(row / a.H) * a.q_ts + (int64_t)(row % a.H) * a.q_hs;
+  const TK* kb = reinterpret_cast<const TK*>(a.kv.k) + (int64_t)g * a.kv.sh;
+  const TK* vb = reinterpret_cast<const TK*>(a.kv.v) + (int64_t)g * a.kv.sh;
+  const int* ids = SRC == SRC_PREFIX ? a.prefix : a.tables + (int64_t)request * a.table_stride;
+  float4 q[NCH], o[NCH];
+#pragma unroll
+  for (int c = 0; c < NCH; c++) {
+    const int d = (c * 32 + lane) * 4;
+    q[c] = d < a.hd ? load4(qp + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  const float ref = m == -INFINITY ? 0.f : m;
+  for (int ub = u0; ub < u1 && ub <= last; ub += step)
+    for (int u = ub; u < min(ub + tile, u1) && u <= last; u++) {
+      int t;
+      const int64_t off = source_at<SRC>(a, ids, nullptr, u, t);
+      if (off < 0) continue;
+      float s = 0.f;
+#pragma unroll
+      for (int c = 0; c < NCH; c++) {
+        const int d = (c * 32 + lane) * 4;
+        if (d < a.hd) {
+          const float4 k = load4(kb + off + d);
+          s = fmaf(q[c].x, k.x, fmaf(q[c].y, k.y, fmaf(q[c].z, k.z, fmaf(q[c].w, k.w, s))));
+        }
+      }
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+      const float p = ex2(fmaf(s, a.scale, -ref));
+#pragma unroll
+      for (int c = 0; c < NCH; c++) {
+        const int d = (c * 32 + lane) * 4;
+        if (d < a.hd) {
+          const float4 v = load4(vb + off + d);
+          o[c].x = fmaf(p, v.x, o[c].x);
+          o[c].y = fmaf(p, v.y, o[c].y);
+          o[c].z = fmaf(p, v.z, o[c].z);
+          o[c].w = fmaf(p, v.w, o[c].w);
+        }
+      }
+    }
+#pragma unroll
+  for (int c = 0; c < NCH; c++) {
+    const int d = (c * 32 + lane) * 4;
+    if (d < a.hd) *reinterpret_cast<float4*>(dst + d) = o[c];
+  }
+}
+
 // The parts of a cluster's rows, joined: row r of part p is at rows + r * stride
 // (m, l, then hd sums) of the shared memory of the cluster's CTA p. CTA p
 // writes the features p * 4, (p + parts) * 4, ... of every row, each from all
@@ -932,6 +991,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
         for (int j = 0; j < 4; j++) o[r][c][j] *= alpha;
 #pragma unroll
         for (int i = 0; i < U; i++) {
+          if (SRC != SRC_LIST && t[i] > limit[r]) continue;  // zero times an infinity is none; a list's rows share a limit
           o[r][c][0] = fmaf(p[i], vx[i][c].x, o[r][c][0]);
           o[r][c][1] = fmaf(p[i], vx[i][c].y, o[r][c][1]);
           o[r][c][2] = fmaf(p[i], vx[i][c].z, o[r][c][2]);

@@ -389,6 +389,17 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
         }
       if (r == 0) sml[warp * COLS + col] = make_float2(m[t][e], l[t][e]);
     }
+  if (SRC != SRC_LIST && least < min(u1 - 1, most)) {  // some row is short of positions that entered its products
+    __syncwarp();
+    for (int col = 0; col < COLS; col++) {
+      if (s_row[col] < 0 || s_limit[col] >= u1 - 1) continue;
+      float* dst = so + (warp * COLS + col) * OS;
+      bool odd = false;
+      for (int d = lane; d < hd; d += 32) odd |= !(fabsf(dst[d]) < INFINITY);
+      if (__any_sync(0xffffffffu, odd))
+        sum_row<TQ, TK, HD, SRC>(a, s_row[col], g, request, u0 + warp * 16, u1, 16, MM_WARPS * 16, s_limit[col], sml[warp * COLS + col].x, dst);
+    }
+  }
   __syncthreads();
   const bool direct = a.slots == 1;  // the only part: the output itself
   float* rows = so + MM_WARPS * COLS * (OS + 2);  // this part of the rows, for its cluster

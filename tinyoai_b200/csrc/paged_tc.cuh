@@ -412,6 +412,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     ok = __all_sync(0xffffffffu, ok);
     tc_fence_after();
     const int64_t slot = (int64_t)(row < 0 ? 0 : row) * a.slots + (p.split_keys ? 2 * part + t : part);
+    float odd = 0.f;  // NaN once a sum is not finite
     for (int q = 0; q < p.hdp; q += 16) {
       uint32_t x[16] = {};
       if (count[t] > 0) pt_ld16(to + q, x);
@@ -419,6 +420,20 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
           if (q + e < a.hd) *reinterpret_cast<uint4*>(a.part_o + slot * a.hd + q + e) = make_uint4(x[e], x[e + 1], x[e + 2], x[e + 3]);
+#pragma unroll
+        for (int e = 0; e < 16; e++) odd = fmaf(__uint_as_float(x[e]), 0.f, odd);
+      }
+    }
+    // Rows that the part's last positions, which are not theirs, left without a finite sum.
+    const int part_end = min(prefix_end, (blk0 + nblk) * PT_KEYS);
+    uint32_t again = __ballot_sync(0xffffffffu, row >= 0 && limit < part_end - 1 && odd != odd);
+    if (again) {
+      __syncwarp();  // the first sums are written
+      for (; again; again &= again - 1) {
+        const int from = __ffs(again) - 1, at_row = __shfl_sync(0xffffffffu, row, from), tile = blk0 + (p.split_keys ? t : 0);
+        sum_row<T, T, SUB * 64, SRC_PREFIX>(a, at_row, g, 0, tile * PT_KEYS, part_end, PT_KEYS, (p.split_keys ? 2 : 1) * PT_KEYS,
+                                            __shfl_sync(0xffffffffu, limit, from), __shfl_sync(0xffffffffu, m, from),
+                                            a.part_o + __shfl_sync(0xffffffffu, slot, from) * a.hd);
       }
     }
     if (row >= 0) a.part_ml[slot] = ok ? make_float2(m, l) : make_float2(NAN, NAN);
