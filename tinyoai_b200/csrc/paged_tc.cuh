@@ -65,7 +65,7 @@ struct PagedTcArgs {
 
 struct PtShared {
   uint64_t k_full[PT_MAX_STAGES], k_empty[PT_MAX_STAGES], v_full[PT_MAX_STAGES], v_empty[PT_MAX_STAGES];
-  uint64_t s_full[2], p_full[2], o_done[2];
+  uint64_t s_full[2], p_full[2], o_done[2], gone;
   uint32_t tmem;
   int err;
   int row[2 * PT_ROWS], limit[2 * PT_ROWS];
@@ -205,6 +205,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
       mbar_init(&sh.p_full[t], 4);
       mbar_init(&sh.o_done[t], 1);
     }
+    mbar_init(&sh.gone, 1);
     fence_barrier_init();
   }
   if (!__syncthreads_or(valid)) return;  // padding rows only
@@ -331,8 +332,8 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
         }
     }
     if (!ok && leader) {  // products in flight read shared memory: let them finish
-      tc_commit(&sh.o_done[0]);
-      pt_drain(&sh.o_done[0], 0);
+      tc_commit(&sh.gone);
+      pt_drain(&sh.gone, 0);
     }
     __syncwarp();
   } else {
