@@ -645,6 +645,30 @@ def test_attend_values_of_unseen_positions(qt, kt, case):
 
 
 @pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("prefix", [0, 2, 300])
+def test_rows_before_the_first_position(qt, kt, prefix):
+    """Requests shorter than their tokens of the step: rows at -1, -2, -9 are zero, in every attention."""
+    lens, fresh, H, KVH, hd, P = [1, 0, 5, 40], [9, 6, 5, 3], 4, 2, 64, 16
+    if prefix == 300:
+        lens, fresh = [1, 0, 5] + [4840] * 30, [9, 6, 5] + [1] * 30
+    qt, kt = TYPES[qt], TYPES[kt]
+    s = attention_state(lens, fresh, H, KVH, hd, P, qt, kt, seed=31, prefix=prefix)
+    before = torch.cat([torch.arange(f, device=DEV) < f - x for x, f in zip(lens, fresh)])
+    c = paged.Cache(s["k"], s["v"])
+    out = torch.full((s["T"] + 2, H, hd), 5.0, dtype=qt, device=DEV)
+    c.attend(s["q"], s["table"], s["starts"], s["lengths"], max(fresh), prefix=s["prefix"] if prefix else None, out=out)
+    want, tol = expected(s, lens, fresh, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
+    near(out[:s["T"]], want, (2 if prefix == 300 else 1) * tol)
+    assert bool((out[:s["T"]][before] == 0).all()) and bool((out[s["T"]:] == 5).all())
+    if prefix == 0:
+        means = torch.zeros((len(s["k"]), KVH, hd), dtype=kt, device=DEV)
+        out.fill_(5.0)
+        got, pages = c.attend_sparse(s["q"], means, s["table"], s["starts"], s["lengths"], max(fresh), first=1, last=1, top=1, out=out)
+        assert bool((out[:s["T"]][before] == 0).all()) and bool((pages[:s["T"]][before] == -1).all())
+        near(out[:s["T"]], want, tol)  # three pages hold every request
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
 def test_attend_extreme_scores(qt, kt):
     """Scores far apart and scores at the type's lowest value: one position
     takes all the weight, or all weights are equal."""

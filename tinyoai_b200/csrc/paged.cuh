@@ -659,7 +659,7 @@ __device__ __forceinline__ void overlap_end(const AttendArgs& a) {
 struct Query {
   int token;     // row of q, -1: none
   int request;
-  int pos;       // its position
+  int pos;       // its position, -1 for every negative one
 };
 
 // Query j of request i.
@@ -667,7 +667,7 @@ __device__ __forceinline__ Query query_at(const AttendArgs& a, int i, int j) {
   const int s = a.starts[i], fresh = a.starts[i + 1] - s;
   const int token = s + j;
   if (j >= fresh || s < 0 || token >= a.T) return Query{-1, i, -1};
-  return Query{token, i, min(a.lengths[i] - fresh + j, a.max_length - 1)};
+  return Query{token, i, max(min(a.lengths[i] - fresh + j, a.max_length - 1), -1)};
 }
 
 // The request of row `token` of q: the last i with starts[i] <= token.
@@ -682,7 +682,7 @@ __device__ __forceinline__ Query query_of(const AttendArgs& a, int token) {
   const int fresh = a.starts[l + 1] - a.starts[l];
   const int j = token - a.starts[l];
   if (j >= a.max_fresh || j >= fresh) return Query{-1, l, -1};
-  return Query{token, l, min(a.lengths[l] - fresh + j, a.max_length - 1)};
+  return Query{token, l, max(min(a.lengths[l] - fresh + j, a.max_length - 1), -1)};
 }
 
 // Where position index u of a part's history lies: offset of the row in the
