@@ -668,6 +668,25 @@ def test_rows_before_the_first_position(qt, kt, prefix):
         near(out[:s["T"]], want, tol)  # three pages hold every request
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_strides_of_dimensions_of_one(t):
+    """One row, one head, one page, one position: what torch keeps as that dimension's stride is no stride."""
+    dt, hd = TYPES[t], 64
+    for lens, fresh, H, P in (([5], [1], 1, 8), ([1], [1], 1, 1), ([9], [3], 1, 16), ([40], [1], 2, 8)):
+        s = attention_state(lens, fresh, H, 1, hd, P, dt, dt, seed=len(lens) + P)
+        args = (s["table"], s["starts"], s["lengths"], max(fresh))
+        want, tol = expected(s, lens, fresh, H, 1, hd, P, 1 / math.sqrt(hd), 0)
+        near(paged.Cache(s["k"], s["v"]).attend(s["q"], *args)[:s["T"]], want, tol)
+
+        def odd(x):  # dimensions of one get a stride of 3
+            return x.as_strided(x.shape, [st if n > 1 else 3 for n, st in zip(x.shape[:-1], x.stride())] + [1])
+        k, v, q = (odd(x) for x in (s["k"], s["v"], s["q"][:s["T"]].clone()))
+        out = odd(torch.zeros_like(q))
+        paged.Cache(k, s["v"]).attend(q, *args, out=out)
+        near(out, want, tol)
+        near(paged.Cache(k, v).attend(q, *args), want, tol)
+
+
 @pytest.mark.parametrize("qt, kt", PAIRS)
 def test_attend_extreme_scores(qt, kt):
     """Scores far apart and scores at the type's lowest value: one position

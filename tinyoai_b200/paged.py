@@ -167,14 +167,16 @@ class Cache:
         self.device = _on_gpu("k", k)
         if k.dim() != 4 or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
             raise _bad("k and v are tensors [pages, KV heads, positions, head size] of one shape, type and device")
-        if k.stride() != v.stride() or k.stride(3) != 1:
+        # A dimension of one has no stride to speak of.
+        strides, other = ([t.stride(i) if t.shape[i] > 1 else t.shape[3] for i in range(3)] for t in (k, v))
+        if strides != other or k.stride(3) != 1 or v.stride(3) != 1:
             raise _bad("k and v need the same strides and a contiguous last dimension")
         self.k, self.v, self.code = k, v, _code("the cache", k)
         self.num_pages, self.kv_heads, self.page_tokens, self.head_dim = k.shape
         self._means = torch.Size((self.num_pages, self.kv_heads, self.head_dim))
         self._scale = 1 / math.sqrt(self.head_dim) if self.head_dim else 0.0
         self.struct = _lib.PagedKV(k.data_ptr(), v.data_ptr(), self.code, self.num_pages, self.page_tokens, self.kv_heads, self.head_dim,
-                                   k.stride(0), k.stride(1), k.stride(2))
+                                   *strides)
         self._ref = C.byref(self.struct)
         self._sized = (None, 0)
         self.index, self._lib = self.device.index, lib()
@@ -297,5 +299,9 @@ class Cache:
                 raise _bad(f"out must be {tuple(q.shape)} of {q.dtype} on {d}, its last dimension contiguous")
             ots, ohs, _ = out.stride()
         qts, qhs, _ = q.stride()
+        if rows == 1:  # the stride of a dimension of one means nothing
+            qts = ots = heads * hd
+        if heads == 1:
+            qhs = ohs = hd
         return out, C.byref(_lib.PagedQueries(_code("q", q), n, rows, heads, max_fresh, width, q.data_ptr(), qts, qhs, out.data_ptr(), ots, ohs, st, le, tb,
                                               tables.stride(0) if n > 1 else width, self._scale if scale is None else scale))
