@@ -412,8 +412,11 @@ int tcu_shortlist_static(int32_t device, const float* logits, int32_t vocab, int
  *  - Types: TCU_F32, TCU_F16 or TCU_BF16. Query rows and outputs have the
  *    cache's type, or are float32 over a TCU_F16 cache. Sums, norms and
  *    softmax statistics are float32 or wider; a result is rounded once, when
- *    it is stored (softmax weights over 16-bit caches also to 16 bits, each
- *    by at most half a step of the cache's type).
+ *    it is stored. Softmax weights are operands of 16-bit matrix products over
+ *    16-bit caches: with 16-bit rows each is rounded to the cache's type (by
+ *    half a step of it; binary16 weights below 2^-25 of a part's largest by 2^-36
+ *    of that at most), with float32 rows to a pair of binary16 values (22
+ *    bits; below 2^-17 of the largest by 2^-39 of that).
  *  - Strides count values, and the last dimension (a head's values) is
  *    contiguous. Rows, strides and bases of q, out, k and v are multiples of
  *    16 bytes. Head sizes: multiples of 8 up to TCU_PAGED_MAX_HEAD_DIM.

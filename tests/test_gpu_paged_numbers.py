@@ -1,0 +1,61 @@
+"""Numbers that attention over a paged KV cache has to keep: weights far below
+a row's largest one.
+
+Tolerances. u = eps / 2 of a type, as in test_gpu_paged.py.
+ - Heavy positions before a light tail: every score is a product of one
+   feature, so scores are exact and a weight errs by the exponential (2^-22,
+   twice where states are joined) and by its own rounding: u where it is stored
+   in 16 bits, 2^-22 where it is a pair of binary16 values, nothing in float32.
+   Binary16 values stop shrinking at a step of 2^-24: weights are kept times
+   2^11 (binary16 rows) or 2^14 (float32 rows) of the row's largest, which
+   leaves each an absolute error of 2^-36 or 2^-39 of it (2^4 more on the
+   tensor cores of a shared prefix, whose reference may lag that far). The
+   sums' chains add up to n / 32 terms a lane of equal sign: n * 2^-29 of the
+   result at most; an instruction's sixteen truncated additions, the joins and
+   the exponentials 2^-18.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import DEV, PAIRS, TYPES, near, unit  # noqa: E402
+
+if torch.cuda.is_available():
+    from tinyoai_b200 import paged
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("rows, heads, n, shared", [(1, 1, 32768, False), (64, 8, 2048, False), (48, 8, 8192, True), (200, 16, 4096, True)])
+@pytest.mark.parametrize("below", [13.0, 20.0, 24.0, 25.125, 26.5, 30.0])
+def test_light_tail_behind_heavy_positions(qt, kt, rows, heads, n, shared, below):
+    """Runs of 256 positions with value 0 before tails of 1,792 whose weights
+    are 2^-below of theirs and whose values are 1,024: the output is the tail's
+    share. Histories of the requests' own, and one that they share."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    hd, P = 64, 32
+    pages = n // P
+    ids = torch.randperm(pages, generator=torch.Generator(device=DEV).manual_seed(n), device=DEV).to(torch.int32)
+    k, v = (torch.zeros((pages, heads, P, hd), dtype=kt, device=DEV) for _ in range(2))
+    t = torch.arange(n, device=DEV)
+    heavy = t % 2048 < 256
+    page = ids[t // P].long()
+    k[page[heavy], :, t[heavy] % P, 0] = below  # exact in every type
+    v[page[~heavy], :, t[~heavy] % P] = 1024.0
+    q = torch.zeros((rows, heads, hd), dtype=qt, device=DEV)
+    q[:, :, 0] = 1.0
+    starts, lengths = torch.arange(rows + 1, dtype=torch.int32, device=DEV), torch.full((rows,), n, dtype=torch.int32, device=DEV)
+    table = ids[None].expand(rows, -1).contiguous()
+    out = paged.Cache(k, v).attend(q, table, starts, lengths, 1, prefix=ids if shared else None, scale=math.log(2.0))
+    w, ht, lt = 2.0 ** -below, int(heavy.sum()), int((~heavy).sum())
+    want = 1024 * lt * w / (ht + lt * w)
+    if qt == torch.float32:
+        weight, floor = (2.0 ** -22, 2.0 ** -39) if kt == torch.float16 else (0.0, 0.0)
+    else:
+        weight, floor = unit(kt), (2.0 ** -36 * (2 ** 4 if shared else 1) if kt == torch.float16 else 0.0)
+    # The scale is ln 2 in float32, and so is its product with log2 e: 2^-24 of the exponent each.
+    rel = 2 * below * 2.0 ** -24 + weight + n * 2.0 ** -29 + 2.0 ** -18 + unit(qt)
+    tol = rel * want + 1024 * lt * floor / ht + (2.0 ** -25 if qt == torch.float16 else 0.0)
+    near(out, torch.full_like(out, want, dtype=torch.float64), tol)

@@ -609,8 +609,8 @@ __global__ void __launch_bounds__(128) k_page_means(MeansArgs a) {
 // up to its own. A "row" is one query and one of the G = H / KVH query heads
 // of a KV head. The history is cut into parts handled by separate CTAs; each
 // leaves (sum_t 2^(s_t - m) v_t, m, sum_t 2^(s_t - m)) of its rows, with s in
-// units of log2 (the scale carries log2 e), and k_attend_join adds the parts
-// up in part order. A row that sees nothing leaves m = -inf and l = 0 and its
+// units of log2 (the scale carries log2 e) and both sums times 2^weight_bias,
+// and k_attend_join adds the parts up in part order. A row that sees nothing leaves m = -inf and l = 0 and its
 // output is zero.
 struct AttendArgs {
   int n, T, H, KVH, G, hd, max_fresh;
@@ -720,15 +720,30 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Weights that become 16-bit operands are 2^(score - m + weight_bias): binary16
+// has no values below 2^-24, so that weights relative to a largest of 1 would
+// lose bits from 2^-14 of it on and vanish from the products, though not from
+// their float32 sum, below 2^-25. A long light tail behind a heavy position is
+// made of such weights. With 2^14 (float32 rows) both pieces of a weight keep
+// their bits down to 2^-17 of the largest and 2^-39 of it is the error of
+// any other; with 2^11 (binary16 rows, whose shared prefix needs the rest of
+// the range for a reference that lags behind, paged_tc.cuh) it is 11 bits down to
+// 2^-25, and 2^-36. Both sums of a row carry the factor, which cancels; kernels
+// whose parts are joined have the same. bfloat16 has float32's exponents.
+template <typename TQ, typename TK>
+__host__ __device__ constexpr float weight_bias() {
+  return sizeof(TK) == 4 || __is_same(TK, bf16) ? 0.f : sizeof(TQ) == 4 ? 14.f : 11.f;
+}
+
 // 1 / l, 0 for a row that saw nothing; NaN stays NaN.
 __device__ __forceinline__ float inverse_sum(float l) { return l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l); }
 
 // A matrix product takes in every position of its tile, those a row does not
 // attend to with weight 0; an infinity or NaN among their values makes the
 // row's sums NaN. Such rows (not finite, and short of the part's last
-// position) are summed again by this: a warp adds 2^(score - m) v over the
-// part's positions up to `last` one by one, score and m in units of log2, and
-// writes the sums to dst. The part is the tiles of `tile` positions every `step`
+// position) are summed again by this: a warp adds 2^(score - m + weight_bias) v
+// over the part's positions up to `last` one by one, score and m in units of
+// log2, and writes the sums to dst. The part is the tiles of `tile` positions every `step`
 // from u0 on, up to u1.
 template <typename TQ, typename TK, int HD, int SRC>
 __device__ __noinline__ void sum_row(const AttendArgs& a, int row, int g, int request, int u0, int u1, int tile, int step, int last, float m, float* dst) {
@@ -762,7 +777,7 @@ __device__ __noinline__ void sum_row(const AttendArgs& a, int row, int g, int re
       }
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-      const float p = ex2(fmaf(s, a.scale, -ref));
+      const float p = ex2(fmaf(s, a.scale, -ref) + weight_bias<TQ, TK>());
 #pragma unroll
       for (int c = 0; c < NCH; c++) {
         const int d = (c * 32 + lane) * 4;

@@ -19,9 +19,10 @@
 //  - P^T leaves the first product with positions in rows; one 8 x 8 transpose
 //    within the warp (movmatrix) gives the second product's operand.
 // The softmax statistics are float32, one running maximum per warp and query
-// row; the weights are rounded to the cache's type as operands. Float32
-// queries over a binary16 cache keep 22 bits: q * 2^sx and the weights are
-// each two binary16 values and each product two instructions.
+// row; the weights are rounded to the cache's type as operands (binary16: times
+// 2^weight_bias, paged.cuh). Float32 queries over a binary16 cache keep 22 bits:
+// q * 2^sx and the weights are each two binary16 values and each product two
+// instructions.
 //
 // A CTA's warps take alternate 16-position tiles of the CTA's part and join
 // their states through shared memory in warp order. Four CTAs (16 warps of
@@ -315,8 +316,9 @@ __device__ __forceinline__ void mm_part(const AttendArgs& a, int row_tiles) {
         const float ref = mx == -INFINITY ? 0.f : mx;
         alpha[t][e] = ex2(m[t][e] - ref);
         m[t][e] = mx;
-        s[t][e] = ex2(s[t][e] - ref);
-        s[t][2 + e] = ex2(s[t][2 + e] - ref);
+        // Two subtractions, so that a large score's rounding cannot lift its weight.
+        s[t][e] = ex2((s[t][e] - ref) + weight_bias<TQ, TK>());
+        s[t][2 + e] = ex2((s[t][2 + e] - ref) + weight_bias<TQ, TK>());
         l[t][e] = fmaf(l[t][e], alpha[t][e], s[t][e] + s[t][2 + e]);
       }
 #pragma unroll

@@ -18,9 +18,10 @@
 // are there, while the others bring the queries), warp 9 the products.
 //
 // A row's reference m moves only when a block's maximum passes it by more
-// than 2^8 (weights up to 256 fit both types), which spares the
-// multiplication of O in TMEM for almost every block; the sums stay exact in
-// float32 since the same m enters numerator and denominator. A stream's
+// than a factor 2^lag, which spares the multiplication of O in TMEM for almost
+// every block; the sums stay exact in float32 since the same m enters numerator
+// and denominator. bfloat16: lag 8; binary16: lag 4, whose largest weight
+// 2^(4 + weight_bias) = 2^15 is within the type. A stream's
 // product S(i + 1) overwrites the columns of P(i): the tensor core runs a
 // CTA's products in the order they are issued, P(i) V before S(i + 1).
 //
@@ -344,6 +345,8 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     const uint32_t ts = tmem + t * 128 + lanes, to = tmem + 256 + t * 128 + lanes;
     // Not zero, so that a masked score times it stays -inf.
     const float scale = fmaxf(fabsf(a.scale), 1.17549435e-38f);
+    constexpr float BIAS = weight_bias<T, T>(), LAG = BIAS == 0.f ? 8.f : 4.f;
+    static_assert(BIAS == 0.f || BIAS + LAG < 16.f, "the largest binary16 weight");
     float m = -INFINITY, l = 0.f;
     bool ok = true;
     for (int i = 0; i < count[t]; i++) {
@@ -378,7 +381,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
         mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
       }
       mx *= scale;
-      const bool move = mx > m + 8.f;  // from -inf as well
+      const bool move = mx > m + LAG;  // from -inf as well
       if (__any_sync(0xffffffffu, move)) {
         const float alpha = move ? (m == -INFINITY ? 0.f : ex2(m - mx)) : 1.f;
         if (move) m = mx;
@@ -386,7 +389,7 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
         // S(i) is complete, so P(i - 1) V is, which was issued before it.
         if (i > 0) pt_scale_rows(to, p.hdp, alpha);
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = (m == -INFINITY ? 0.f : m) - BIAS;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       // Weights of the second half, then of the first, packed into the
       // second half of S's columns, which is read by then.
