@@ -13,6 +13,9 @@ Tolerances. u = eps / 2 of a type, as in test_gpu_paged.py.
    sums' chains add up to n / 32 terms a lane of equal sign: n * 2^-29 of the
    result at most; an instruction's sixteen truncated additions, the joins and
    the exponentials 2^-18.
+ - Scores so large that float32 has no halves, or no ones, there: equal keys
+   have equal weights, and a larger score takes all. The sums, weights and the
+   store as in test_gpu_paged.py, 2^-13 + u and u.
 """
 import math
 
@@ -21,7 +24,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import DEV, PAIRS, TYPES, near, unit  # noqa: E402
+from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, near, unit  # noqa: E402
 
 if torch.cuda.is_available():
     from tinyoai_b200 import paged
@@ -59,3 +62,33 @@ def test_light_tail_behind_heavy_positions(qt, kt, rows, heads, n, shared, below
     rel = 2 * below * 2.0 ** -24 + weight + n * 2.0 ** -29 + 2.0 ** -18 + unit(qt)
     tol = rel * want + 1024 * lt * floor / ht + (2.0 ** -25 if qt == torch.float16 else 0.0)
     near(out, torch.full_like(out, want, dtype=torch.float64), tol)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [4, 48, 200])
+@pytest.mark.parametrize("power", [17, 22, 27, 30, 35, 100])
+def test_scores_past_float32_steps(t, rows, power):
+    """Scores of -0.7 * 1.75 * 2^power at every position, then one of the other sign
+    among them: in a shared prefix, joined with the requests' own positions."""
+    dt, P, prefix, hd = TYPES[t], 32, 20, 64
+    if power > 35 and dt == torch.float16:
+        power = 34  # binary16 rows have no such scores
+    lens = [prefix * P + 1 + i % 40 for i in range(rows)]
+    s = attention_state(lens, [1] * rows, 2, 2, hd, P, dt, dt, seed=8, prefix=prefix, fill=0.0)
+    c = paged.Cache(s["k"], s["v"])
+    a, b = 1.75 * 2.0 ** ((power - 6) // 2), 2.0 ** (power - 6 - (power - 6) // 2)  # 64 products of three bits: exact sums
+    s["q"].fill_(a)
+
+    def check(at):
+        out = c.attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], scale=0.7)
+        for i in range(0, rows, 7):
+            x = torch.arange(lens[i], device=DEV)
+            page = torch.where(x // P < prefix, s["prefix"][(x // P).clamp(max=prefix - 1)], s["table"][i][x // P]).long()
+            v = s["v"][page, :, x % P].double()
+            v = v if at is None else v[at:at + 1]
+            near(out[i], v.mean(0), (2.0 ** -13 + unit(dt)) * v.abs().mean(0) + unit(dt) * v.mean(0).abs())
+
+    s["k"].fill_(-b)
+    check(None)
+    s["k"][s["prefix"][9].long(), :, 3] = b
+    check(9 * P + 3)

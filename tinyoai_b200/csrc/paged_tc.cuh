@@ -346,9 +346,13 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     // Not zero, so that a masked score times it stays -inf.
     const float scale = fmaxf(fabsf(a.scale), 1.17549435e-38f);
     constexpr float BIAS = weight_bias<T, T>(), LAG = BIAS == 0.f ? 8.f : 4.f;
+    // From here on a score's rounding to float32 shows in its weight: the
+    // reference does not lag, and a score is rounded as the reference was before
+    // that is taken off, so that no weight passes 2^BIAS.
+    constexpr float LARGE = 262144.f;
     static_assert(BIAS == 0.f || BIAS + LAG < 16.f, "the largest binary16 weight");
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
+    float m = -INFINITY, l = 0.f, lag = LAG;
+    bool ok = true, large = false;  // large: a row of the warp has such scores
     for (int i = 0; i < count[t]; i++) {
       const int key0 = (blk0 + (p.split_keys ? 2 * i + t : i)) * PT_KEYS;
       ok = mbar_wait(&sh.s_full[t], i & 1, &sh.err);
@@ -381,25 +385,31 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
         mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
       }
       mx *= scale;
-      const bool move = mx > m + LAG;  // from -inf as well
+      const bool move = mx > m + lag;  // from -inf as well
       if (__any_sync(0xffffffffu, move)) {
         const float alpha = move ? (m == -INFINITY ? 0.f : ex2(m - mx)) : 1.f;
         if (move) m = mx;
+        if (move) lag = fabsf(m) < LARGE ? LAG : 0.f;
+        large = __any_sync(0xffffffffu, lag == 0.f);
         l *= alpha;
         // S(i) is complete, so P(i - 1) V is, which was issued before it.
         if (i > 0) pt_scale_rows(to, p.hdp, alpha);
       }
-      const float ref = (m == -INFINITY ? 0.f : m) - BIAS;
+      const float ref = m == -INFINITY ? 0.f : m;
+      const float mul = large ? 1.f : scale, add = large ? BIAS : BIAS - ref;
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       // Weights of the second half, then of the first, packed into the
       // second half of S's columns, which is read by then.
 #pragma unroll
       for (int half = 1; half >= 0; half--) {
         if (half == 0) load(0);
+        if (large)
+#pragma unroll
+          for (int q = 0; q < HALF; q++) s[q] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(s[q]), scale), ref));
         uint32_t w[HALF / 2];
 #pragma unroll
         for (int q = 0; q < HALF; q += 2) {
-          const float2 x = fma2(make_float2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), make_float2(scale, scale), make_float2(-ref, -ref));
+          const float2 x = fma2(make_float2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), make_float2(mul, mul), make_float2(add, add));
           const float2 e = make_float2(ex2(x.x), ex2(x.y));
           sum[(q / 2) & 1] = add2(sum[(q / 2) & 1], e);
           w[q / 2] = pack2<T>(e.x, e.y);
