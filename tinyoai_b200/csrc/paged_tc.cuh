@@ -42,6 +42,7 @@
 
 #include "paged.cuh"
 #include "paged_mma.cuh"
+#include "ring.h"
 #include "tcgen05.cuh"
 
 namespace tcu {
@@ -88,8 +89,8 @@ __device__ __forceinline__ void pt_load(void* dst, const CUtensorMap* map, int x
       : "memory");
 }
 
-// After a failed wait: the phase's copies or products must have landed
-// before the CTA leaves (bounded as well).
+// After a wait that ran out: what was issued must have landed before the CTA
+// leaves (bounded as well).
 __device__ __forceinline__ void pt_drain(uint64_t* bar, uint32_t parity) {
   const unsigned long long t0 = global_ns();
   while (!mbar_try_wait(bar, parity))
@@ -241,17 +242,17 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
     tmem = *reinterpret_cast<volatile uint32_t*>(&sh.tmem);
   }
 
+  int sent_k = 0, sent_v = 0;  // blocks of keys and of values whose copies were queued (by warp 8's first lane)
   if (warp == 8) {
     if (lane == 0) {
       const uint32_t bytes = (uint32_t)SUB * PT_SUB;
       const int boxes = PT_KEYS / p.box;
-      int b = 0;
-      for (; b < nblk; b++) {
+      bool ok = true;
+      for (int b = 0; b < nblk && ok; b++) {
         const int st = b % p.stages, round = b / p.stages;
         const int key0 = (blk0 + b) * PT_KEYS;
-        bool ok = true;
 #pragma unroll 1
-        for (int kv = 0; kv < 2 && ok; kv++) {
+        for (int kv = 0; kv < 2; kv++) {
           uint64_t* full = kv ? &sh.v_full[st] : &sh.k_full[st];
           if (round > 0) ok = mbar_wait(kv ? &sh.v_empty[st] : &sh.k_empty[st], (round - 1) & 1, &sh.err);
           if (!ok) break;
@@ -264,17 +265,9 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
             if (id < 0) id = a.kv.num_pages;  // behind the pool: zeros
             for (int s = 0; s < SUB; s++) pt_load(dst + (size_t)s * PT_SUB + x * p.box * 128, kv ? &vmap : &kmap, s * 64, row0, g, id, full);
           }
+          if (kv) sent_v++; else sent_k++;
         }
-        if (!ok) break;
       }
-      if (b < nblk)  // gave up: the copies of the last rounds must have landed
-        for (int i = 0; i < p.stages; i++) {
-          const int last = b - 1 - i;
-          if (last >= 0) {
-            pt_drain(&sh.k_full[last % p.stages], (last / p.stages) & 1);
-            pt_drain(&sh.v_full[last % p.stages], (last / p.stages) & 1);
-          }
-        }
     }
   } else if (warp == 9) {
     // The whole warp runs the schedule, so that descriptors stay in uniform
@@ -332,11 +325,6 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
           if (i + 1 < count[t]) scores(t, i + 1);
         }
     }
-    if (!ok && leader) {  // products in flight read shared memory: let them finish
-      tc_commit(&sh.gone);
-      pt_drain(&sh.gone, 0);
-    }
-    __syncwarp();
   } else {
     const int t = warp >> 2, r = tid & 127;
     const int at = p.split_keys ? r : tid;  // this thread's row
@@ -454,6 +442,21 @@ __global__ void __maxnreg__(PT_REGS) k_attend_prefix_tc(const __grid_constant__ 
   }
   tc_fence_before();
   __syncthreads();
+  // Every copy and product was waited for above, unless a wait ran out. Then
+  // some may be on their way still, whichever warp gave up.
+  if (*(volatile int*)&sh.err) {
+    if (warp == 8 && lane == 0)
+      for (int st = 0; st < p.stages; st++) {
+        const int pk = ring_last_parity(sent_k, st, p.stages), pv = ring_last_parity(sent_v, st, p.stages);
+        if (pk >= 0) pt_drain(&sh.k_full[st], pk);
+        if (pv >= 0) pt_drain(&sh.v_full[st], pv);
+      }
+    if (warp == 9 && tc_elect()) {  // the lane that issued the products
+      tc_commit(&sh.gone);
+      pt_drain(&sh.gone, 0);
+    }
+    __syncthreads();
+  }
   if (warp == 9) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
