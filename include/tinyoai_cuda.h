@@ -351,8 +351,11 @@ int tcu_batch_sample_candidates(tcu_batch* batch, int32_t n, const int32_t* hist
  * (forks of one session, tcu_session_fork) read those pages once for all of
  * them: a step of two rows or more that share at least min_positions positions
  * in whole pages attends through tcu_paged_append and tcu_paged_attend (below)
- * instead of row by row. 0 (the default) turns it off. The rows then differ
- * from the unshared step's by float32 rounding, not in what they compute.
+ * instead of row by row. 0 (the default) turns it off. A layer's attention then
+ * differs from the unshared step's by the order of float32 sums (and, over
+ * binary16 KV, by weights of 22 bits), not in what it computes; keys and values
+ * are rotated and rounded alike. What a later layer appends follows from
+ * attention so rounded: a binary16 key or value there may be its neighbour.
  * Allocates the step's buffers; a step whose workspace has to grow allocates
  * again. Not for tensor-parallel models, nor for shapes outside the limits of
  * the operators below (TCU_EUNSUP). */
@@ -463,7 +466,8 @@ int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, 
 
 /* Rotary table: max_positions x pairs float32 pairs (cos, sin), 8-byte
  * aligned. Pair i is features (i, i + pairs) of a head, or (2i, 2i + 1) when
- * adjacent != 0; features from 2 * pairs on pass unchanged. */
+ * adjacent != 0; features from 2 * pairs on pass unchanged. Products and sums
+ * are each rounded to float32. */
 typedef struct {
   const float* table;
   int32_t max_positions, pairs, adjacent;

@@ -1,5 +1,5 @@
-"""Numbers that attention over a paged KV cache has to keep: weights far below
-a row's largest one.
+"""Numbers that the operators over a paged KV cache have to keep: weights far
+below a row's largest one, scores at the end of float32, the rotation's roundings.
 
 Tolerances. u = eps / 2 of a type, as in test_gpu_paged.py.
  - Heavy positions before a light tail: every score is a product of one
@@ -16,6 +16,8 @@ Tolerances. u = eps / 2 of a type, as in test_gpu_paged.py.
  - Scores so large that float32 has no halves, or no ones, there: equal keys
    have equal weights, and a larger score takes all. The sums, weights and the
    store as in test_gpu_paged.py, 2^-13 + u and u.
+ - Append without a norm: the stored numbers themselves, products and sum of the
+   rotation each rounded to float32, then to the stored type.
 """
 import math
 
@@ -24,7 +26,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, near, unit  # noqa: E402
+from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, gen, i32, near, normal, unit  # noqa: E402
 
 if torch.cuda.is_available():
     from tinyoai_b200 import paged
@@ -92,3 +94,66 @@ def test_scores_past_float32_steps(t, rows, power):
     check(None)
     s["k"][s["prefix"][9].long(), :, 3] = b
     check(9 * P + 3)
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("pairs, adjacent", [(16, False), (32, False), (6, False), (20, True), (32, True)])
+def test_rotation_rounds_each_operation(qt, kt, pairs, adjacent):
+    """Queries and keys of an append equal, bit for bit, a rotation whose
+    products and sums are rounded one by one."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    H, KVH, hd, P, T = 4, 2, 64, 16, 96
+    g = gen(pairs + adjacent)
+    k, v = (torch.zeros((T // P, KVH, P, hd), dtype=kt, device=DEV) for _ in range(2))
+    angle = torch.rand((512, pairs), generator=g, device=DEV, dtype=torch.float64) * 6.3
+    table = torch.stack([angle.cos(), angle.sin()], -1).float().contiguous()
+    pos = torch.randint(0, 512, (T,), generator=g, device=DEV)
+    slots = torch.randperm(T, generator=g, device=DEV)
+    x = normal((T, (H + 2 * KVH) * hd), g, qt)
+    q = paged.Cache(k, v).append(x, H, pos.to(torch.int32), slots, rotary=paged.Rotary(table, adjacent))
+    y = x.float().reshape(T, -1, hd)[:, :H + KVH].clone()
+    ia = torch.arange(pairs, device=DEV) * (2 if adjacent else 1)
+    ib = ia + (1 if adjacent else pairs)
+    a, b, c, s = y[..., ia].clone(), y[..., ib].clone(), table[pos][:, None, :, 0], table[pos][:, None, :, 1]
+    y[..., ia], y[..., ib] = a * c - b * s, b * c + a * s
+    assert torch.equal(q, y[:, :H].to(qt))
+    assert torch.equal(k[slots // P, :, slots % P], y[:, H:].to(kt))
+    assert torch.equal(v[slots // P, :, slots % P], x.reshape(T, -1, hd)[:, H + KVH:].to(kt))
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("heads, kv_heads, hidden", [(4, 4, 320), (8, 2, 512)])
+def test_a_shared_step_stores_what_an_unshared_one_does(kv, heads, kv_heads, hidden, tmp_path):
+    """First-layer keys and values do not depend on attention: with share_prefix
+    on, the cache of a one-layer model holds the same bytes as without."""
+    from tinyoai_b200 import Model
+    from tinyoai_b200.synth import prompt_ids, synth_stablelm
+
+    cfg, tensors = synth_stablelm(dict(model_type="stablelm", vocab_size=2048, hidden_size=hidden, intermediate_size=864, num_hidden_layers=1,
+                                       num_attention_heads=heads, num_key_value_heads=kv_heads, max_position_embeddings=512, layer_norm_eps=1e-5,
+                                       rope_theta=10000.0, partial_rotary_factor=0.25, use_parallel_residual=True, use_qkv_bias=False,
+                                       qk_layernorm=False, tie_word_embeddings=False, hidden_act="silu", bos_token_id=0, eos_token_id=0), "Q8_0", seed=11)
+    m = Model.load_stablelm(cfg, tensors)
+    opened = []
+    try:
+        parent = m.session(kv)
+        opened.append(parent)
+        ids = list(prompt_ids(200, cfg["vocab_size"], seed=1))
+        parent.forward(0, ids, want_logits=False)
+        files = []
+        for share in (128, 0):
+            forks = [parent.fork() for _ in range(5)]
+            batch = m.batch(5)
+            opened.extend([*forks, batch])
+            batch.share_prefix(share)
+            added = [prompt_ids(5, cfg["vocab_size"], seed=30 + step) for step in range(4)]
+            for toks in added:
+                batch.forward(forks, toks)
+            for i, f in enumerate(forks):
+                f.save_cache(tmp_path / f"{share}-{i}", bytes(32), ids + [int(t[i]) for t in added])
+            files.append([(tmp_path / f"{share}-{i}").read_bytes() for i in range(5)])
+        assert files[0] == files[1]
+    finally:
+        for x in reversed(opened):
+            x.close()
+        m.close()

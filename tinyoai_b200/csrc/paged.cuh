@@ -371,6 +371,11 @@ struct Raw4<float> {
   }
 };
 
+// u c + v s, both products and the sum rounded, as the sessions' own rotation
+// rounds them (rope_pair in attention.cuh): a batch step that appends here
+// stores the keys, binary16 ones too, that it would store there.
+__device__ __forceinline__ float turned(float u, float c, float v, float s) { return __fadd_rn(__fmul_rn(u, c), __fmul_rn(v, s)); }
+
 // grid: x = tokens x, x + gridDim.x, ...; y = share of the heads (heads_per_cta of them).
 template <typename TQ, typename TK, int LPH, int TURN, int NORM>
 __global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int heads_per_cta) {
@@ -498,8 +503,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int 
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const float u = x[e], v = x[4 + e];
-              x[e] = fmaf(u, cs[e], -(v * sn[e]));
-              x[4 + e] = fmaf(v, cs[e], u * sn[e]);
+              x[e] = turned(u, cs[e], v, -sn[e]);
+              x[4 + e] = turned(v, cs[e], u, sn[e]);
             }
         } else if (TURN == TURN_BESIDE) {
           if (rot[i])
@@ -507,8 +512,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int 
             for (int e = 0; e < 4; e++)
               if (lane * 4 + e < a.pairs) {
                 const float u = x[2 * e], v = x[2 * e + 1];
-                x[2 * e] = fmaf(u, cs[e], -(v * sn[e]));
-                x[2 * e + 1] = fmaf(v, cs[e], u * sn[e]);
+                x[2 * e] = turned(u, cs[e], v, -sn[e]);
+                x[2 * e + 1] = turned(v, cs[e], u, sn[e]);
               }
         } else if (TURN == TURN_SHARED) {
           float* st = stage[grp];
@@ -520,7 +525,7 @@ __global__ void __launch_bounds__(APPEND_THREADS, 3) k_append(AppendArgs a, int 
 #pragma unroll
             for (int e = 0; e < 8; e++) {
               const int f = da + e;
-              if (f < 2 * a.pairs) x[e] = fmaf(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs] * sn[e]);
+              if (f < 2 * a.pairs) x[e] = turned(x[e], cs[e], st[f >= a.pairs ? f - a.pairs : f + a.pairs], sn[e]);
             }
         }
         if (on[i]) {
