@@ -457,7 +457,9 @@ typedef struct {
  *   counts[0 .. 3)      requests planned, tokens planned, pages taken
  * Requests are planned in order up to the first that does not fit (capacity
  * tokens, n_free pages, table_width) or has a negative count; that one and
- * the later ones keep lengths[i] = held[i] and get no tokens. A page that a
+ * the later ones keep lengths[i] = held[i] and get no tokens. lengths may be
+ * the array held (or fresh) itself, starts the array fresh; no other arrays may
+ * overlap. A page that a
  * request appends to (its last, partly filled one) must be its own.
  * page_tokens P: 1 .. TCU_PAGED_MAX_PAGE_TOKENS. */
 int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, const int32_t* fresh, int32_t page_tokens, int32_t* tables,

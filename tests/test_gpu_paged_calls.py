@@ -1,0 +1,80 @@
+"""Calls of the operators over a paged KV cache that users make beside the
+plain ones: arrays that are inputs and outputs at once, overlapping outputs,
+inputs that want gradients, launches that overlap on two streams."""
+import ctypes as C
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+from test_gpu_paged import DEV, TYPES, attention_state, gen, i32, normal, plan_case, plan_ref  # noqa: E402
+from tinyoai_b200 import BackendError, _lib  # noqa: E402
+
+if torch.cuda.is_available():
+    from tinyoai_b200 import paged
+
+
+@pytest.mark.parametrize("n, capacity", [(5, 300), (256, 6000), (1000, 13312)])
+@pytest.mark.parametrize("own", ["lengths", "fresh", "starts"])
+def test_plan_in_place(n, capacity, own):
+    """Lengths that are the next step's held, and lengths or starts over fresh,
+    with more tokens than one CTA fills elsewhere: step after step as with arrays apart."""
+    P, width = 16, 40
+    held, fresh, tables, pages, _, _ = plan_case(n, P, 200, 1, width, 40000, capacity, seed=n)
+    plan = paged.StepPlan(n, capacity, P, DEV)
+    t = i32(tables)
+    starts, lengths, positions, counts = (torch.full((x,), -9, dtype=torch.int32, device=DEV) for x in (n + 1, n, capacity, 3))
+    slots = torch.full((capacity,), -9, dtype=torch.int64, device=DEV)
+    g = torch.Generator().manual_seed(n)
+    h = lengths if own == "lengths" else i32(held)
+    for step in range(4):
+        fresh = torch.randint(0, 2 * capacity // n + 1 if step % 2 else 2, (n,), generator=g).tolist()
+        want = plan_ref(held, fresh, tables, pages, P, capacity)
+        free = i32(pages)
+        f = i32(fresh)
+        if own == "lengths":
+            lengths.copy_(i32(held))  # the first step's held
+        elif own == "fresh":
+            lengths = f
+        else:
+            starts = torch.cat([f, i32([77])])
+            f = starts[:n]
+        if own != "lengths":
+            h = i32(held)
+        rc = _lib.lib().tcu_plan_step(0, torch.cuda.current_stream().cuda_stream, n, h.data_ptr(), f.data_ptr(), P, t.data_ptr(), width, width,
+                                      free.data_ptr(), len(pages), capacity, starts.data_ptr(), lengths.data_ptr(), positions.data_ptr(),
+                                      slots.data_ptr(), counts.data_ptr())
+        assert rc == _lib.TCU_OK, _lib.lib().tcu_last_error()
+        got = [x.tolist() for x in (t, starts, lengths, positions, slots, counts)]
+        assert got == [list(x) for x in want]
+        tables, held, pages = want[0], want[2], pages[want[5][2]:]
+    if own == "lengths":  # the plan's own arrays, as the Python class is used
+        t2 = t.clone()
+        plan.build(i32(held), i32([1] * n), t, i32(pages))
+        first = plan.counts.tolist()
+        plan.build(plan.lengths, i32([1] * n), t, i32(pages[first[2]:]))
+        a = plan_ref(held, [1] * n, t2.tolist(), pages, P, capacity)
+        b = plan_ref(a[2], [1] * n, a[0], pages[a[5][2]:], P, capacity)
+        assert [t.tolist(), plan.lengths.tolist(), plan.slots.tolist()] == [b[0], b[2], b[4]]
+
+
+def test_plan_refuses_overlapping_arrays():
+    n, cap, width = 8, 32, 4
+    buf = torch.zeros(4096, dtype=torch.int32, device=DEV)
+    base = buf.data_ptr()
+    apart = dict(held=0, fresh=64, tables=128, free=256, starts=384, lengths=512, positions=640, slots=768, counts=1024)
+
+    def call(stride=width, **over):
+        at = {k: base + 4 * x for k, x in {**apart, **over}.items()}
+        return _lib.lib().tcu_plan_step(0, None, n, at["held"], at["fresh"], 4, at["tables"], width, stride, at["free"], 16, cap, at["starts"], at["lengths"],
+                                        at["positions"], at["slots"], at["counts"])
+
+    assert call() == _lib.TCU_OK
+    for over in (dict(lengths=0), dict(lengths=64), dict(starts=64), dict(stride=16, held=128 + 4), dict(stride=40, tables=2048, positions=2048 + 4)):
+        assert call(**over) == _lib.TCU_OK, over
+    for over in (dict(lengths=1), dict(lengths=7), dict(starts=0), dict(starts=60), dict(positions=384), dict(slots=640), dict(counts=8 + 512 - 1),
+                 dict(positions=250), dict(tables=0), dict(held=128 + 31), dict(free=128), dict(stride=16, held=128 + 3), dict(stride=16, held=128 + 12),
+                 dict(stride=16, positions=128 + 4), dict(starts=64, lengths=64)):
+        assert call(**over) == _lib.TCU_EINVAL and b"overlap" in _lib.lib().tcu_last_error(), over

@@ -590,6 +590,41 @@ int check_sparse(const tcu_paged_kv* kv, int32_t first, int32_t last, int32_t to
   return TCU_OK;
 }
 
+// The arrays of a plan lie apart, but for lengths or starts that are an input's
+// own array (a decode loop's lengths are the next step's held): *in_place.
+int check_plan_arrays(const PlanArgs& a, bool* in_place) {
+  struct Array {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+    bool output;
+  };
+  const int64_t n = a.n, cap = a.capacity;
+  const Array arrays[] = {{"held", a.held, 4 * n, false},         {"fresh", a.fresh, 4 * n, false},          {"free_pages", a.free_pages, 4ll * a.n_free, false},
+                          {"starts", a.starts, 4 * (n + 1), true}, {"lengths", a.lengths, 4 * n, true},       {"positions", a.positions, 4 * cap, true},
+                          {"slots", a.slots, 8 * cap, true},       {"counts", a.counts, 12, true}};
+  for (const Array& x : arrays) {
+    if (x.bytes == 0) continue;
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x.at), x1 = x0 + x.bytes;
+    for (const Array& y : arrays) {
+      if (&y == &x) break;
+      const uintptr_t y0 = reinterpret_cast<uintptr_t>(y.at), y1 = y0 + y.bytes;
+      if (!(x.output || y.output) || x0 >= y1 || y0 >= x1) continue;
+      if (x0 == y0 && !y.output && ((x.at == a.lengths && (y.at == a.held || y.at == a.fresh)) || (x.at == a.starts && y.at == a.fresh)))
+        *in_place = true;
+      else
+        return fail(TCU_EINVAL, "%s and %s overlap", y.name, x.name);
+    }
+    // The tables' rows, not what lies between them.
+    const uintptr_t t0 = reinterpret_cast<uintptr_t>(a.tables);
+    const uint64_t row = 4ull * a.width, step = 4ull * a.table_stride;
+    if (n == 0 || row == 0 || x1 <= t0 || x0 >= t0 + (n - 1) * step + row) continue;
+    const uint64_t into = x0 < t0 ? 0 : (x0 - t0) % step;
+    if (into < row || into + x.bytes > step) return fail(TCU_EINVAL, "tables and %s overlap", x.name);
+  }
+  return TCU_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -636,9 +671,12 @@ int tcu_plan_step(int32_t device, void* stream, int32_t n, const int32_t* held, 
   a.slots = slots;
   a.counts = counts;
   a.divP = FastDiv::of((uint32_t)page_tokens);
-  const unsigned grid = (unsigned)std::max<int64_t>(1, ceil_div(capacity, PLAN_TILE));
+  bool in_place = false;
+  TRY(check_plan_arrays(a, &in_place));
+  a.tile = in_place ? std::max(capacity, 1) : PLAN_TILE;
+  const unsigned grid = (unsigned)std::max<int64_t>(1, ceil_div(capacity, a.tile));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return n <= 256 ? launch("k_plan_step", k_plan_step<256>, dim3(grid), 256, 0, s, a) : launch("k_plan_step", k_plan_step<1024>, dim3(grid), 1024, 0, s, a);
+  return n <= 256 && capacity / grid <= PLAN_TILE ? launch("k_plan_step", k_plan_step<256>, dim3(grid), 256, 0, s, a) : launch("k_plan_step", k_plan_step<1024>, dim3(grid), 1024, 0, s, a);
 }
 
 int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t dtype, int32_t rows, int32_t heads, const void* qkv,

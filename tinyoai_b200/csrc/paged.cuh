@@ -130,12 +130,15 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
 // free pages or table width) or whose counts are negative. All arithmetic is
 // on integers, so every CTA scans the n requests for itself (two L2 reads
 // each) and the step needs one launch and no communication: CTA c then fills
-// the tokens [c * tile, (c + 1) * tile) and CTA 0 the per-request outputs.
+// the tokens [c * tile, (c + 1) * tile) and CTA 0 the per-request outputs. Where
+// an output is an input's own array, one CTA does all: others could read what
+// CTA 0 has written (it reads a tile of requests before it writes any of it).
 // Latency bounds it, a chain of three or four L2 reads: 3.4 us for 64 decoding
 // requests, 6.2 us for 1,024 with 13,312 token places (a call takes 9 us of
 // the host's time from Python).
 struct PlanArgs {
   int n, P, width, n_free, capacity;
+  int tile;  // tokens a CTA fills
   const int *held, *fresh;
   int* tables;
   int64_t table_stride;
@@ -146,7 +149,7 @@ struct PlanArgs {
   FastDiv divP;
 };
 
-constexpr int PLAN_TILE = 1024;  // tokens a CTA fills
+constexpr int PLAN_TILE = 1024;
 
 struct PlanSum {
   long long tok, pg;
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
   __shared__ int s_start[PLAN_THREADS + 1], s_page[PLAN_THREADS], s_held[PLAN_THREADS];
   __shared__ int s_bad;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const long long t_lo = (long long)blockIdx.x * PLAN_TILE, t_hi = min((long long)a.capacity, t_lo + PLAN_TILE);
+  const long long t_lo = (long long)blockIdx.x * a.tile, t_hi = min((long long)a.capacity, t_lo + a.tile);
   long long tok0 = 0, pg0 = 0;  // totals of the requests before this tile
   int planned = 0;
   bool open = true;

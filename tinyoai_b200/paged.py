@@ -142,9 +142,9 @@ class StepPlan:
         self._outs = tuple(t.data_ptr() for t in (self._starts, self._lengths, self.positions, self.slots, self.counts))
 
     def build(self, held, fresh, tables, free_pages, stream=None):
-        """held, fresh: int32 [requests], positions held and tokens added;
-        tables: int32 [requests, width], updated in place; free_pages: int32.
-        Returns self."""
+        """held, fresh: int32 [requests], positions held and tokens added (held
+        may be this plan's lengths: a loop's next step); tables: int32
+        [requests, width], updated in place; free_pages: int32. Returns self."""
         d, index = self.device, self.index
         h, f = _whole("held", held, torch.int32, d), _whole("fresh", fresh, torch.int32, d)
         t, p = _whole("tables", tables, torch.int32, d, 2), _whole("free_pages", free_pages, torch.int32, d)
