@@ -423,6 +423,8 @@ int tcu_shortlist_static(int32_t device, const float* logits, int32_t vocab, int
  *  - Strides count values, and the last dimension (a head's values) is
  *    contiguous. Rows, strides and bases of q, out, k and v are multiples of
  *    16 bytes. Head sizes: multiples of 8 up to TCU_PAGED_MAX_HEAD_DIM.
+ *    Rows that are written (out, and k and v in an append) must not overlap;
+ *    rows that are read may (stride 0: one head, or one row, for several).
  *  - Page ids outside [0, num_pages) stand for no page: their positions are
  *    not attended and nothing is written there. Values in a page behind a
  *    request's length are never read into a result.

@@ -74,6 +74,21 @@ int check_ptr(const char* name, const void* p, int device, size_t align) {
   return TCU_OK;
 }
 
+// Whether two of n1 x n2 rows of `hd` values, s1 and s2 apart, share values.
+bool rows_overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t hd) {
+  if (n1 < 2) s1 = 0;
+  if (n2 < 2) s2 = 0;
+  if (s1 > s2) std::swap(s1, s2), std::swap(n1, n2);
+  if ((n1 > 1 && s1 < hd) || (n2 > 1 && s2 < hd)) return true;
+  // Rows i s1 and j s2 meet where they are nearer than hd: none do where the
+  // steps of s2 pass all rows of s1, the common case.
+  for (int64_t j = 1; n1 > 1 && j < n2 && j * s2 < (n1 - 1) * s1 + hd; j++) {
+    const int64_t r = j * s2 % s1;
+    if (r < hd || (s1 - r < hd && j * s2 / s1 + 1 < n1)) return true;
+  }
+  return false;
+}
+
 int elem_bytes(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == TCU_F32 || dtype == TCU_F16 || dtype == TCU_BF16; }
 
@@ -514,6 +529,7 @@ int check_queries(const tcu_paged_kv* kv, const tcu_paged_queries* q) {
   if (q->q_token_stride % per16 || q->q_head_stride % per16 || q->out_token_stride % per16 || q->out_head_stride % per16)
     return fail(TCU_EINVAL, "query and output strides must be multiples of 16 bytes");
   if (q->q_token_stride < 0 || q->q_head_stride < 0 || q->out_token_stride < 0 || q->out_head_stride < 0) return fail(TCU_EINVAL, "negative query stride");
+  if (rows_overlap(q->rows, q->out_token_stride, q->heads, q->out_head_stride, kv->head_dim)) return fail(TCU_EINVAL, "output rows overlap");
   if (!(q->scale == q->scale)) return fail(TCU_EINVAL, "scale is not a number");
   return TCU_OK;
 }
@@ -690,6 +706,10 @@ int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32
   if ((int64_t)rows * (heads + 2 * kv->kv_heads) > 0x7fffffffll) return fail(TCU_EINVAL, "too many rows for one call");
   if (qkv_stride < width || q_stride < (int64_t)heads * hd) return fail(TCU_EINVAL, "a row's stride is below its width");
   if (qkv_stride % per16 || q_stride % per16) return fail(TCU_EINVAL, "row strides must be multiples of 16 bytes");
+  if (rows_overlap(kv->num_pages, kv->page_stride, kv->kv_heads, kv->head_stride, hd) ||
+      rows_overlap(kv->num_pages, kv->page_stride, kv->page_tokens, kv->token_stride, hd) ||
+      rows_overlap(kv->kv_heads, kv->head_stride, kv->page_tokens, kv->token_stride, hd))
+    return fail(TCU_EINVAL, "the cache's rows overlap: it cannot be appended to");
   AppendArgs a{};
   if (rotary && rotary->pairs > 0) {
     if (rotary->pairs * 2 > hd) return fail(TCU_EINVAL, "%d rotary pairs in a head of %d", rotary->pairs, hd);
