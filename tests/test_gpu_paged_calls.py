@@ -78,3 +78,33 @@ def test_plan_refuses_overlapping_arrays():
                  dict(positions=250), dict(tables=0), dict(held=128 + 31), dict(free=128), dict(stride=16, held=128 + 3), dict(stride=16, held=128 + 12),
                  dict(stride=16, positions=128 + 4), dict(starts=64, lengths=64)):
         assert call(**over) == _lib.TCU_EINVAL and b"overlap" in _lib.lib().tcu_last_error(), over
+
+
+def test_inputs_that_want_gradients():
+    """The operators record no gradients: with autograd on such inputs are
+    refused, each in its turn; without it they are values like others."""
+    H, KVH, hd, P = 4, 2, 64, 16
+    g = gen(3)
+    k, v = (normal((6, KVH, P, hd), g) for _ in range(2))
+    c = paged.Cache(k, v)
+    x, table = normal((3, (H + 2 * KVH) * hd), g), torch.rand((64, 8, 2), generator=g, device=DEV)
+    qw, kw, means, q = normal((1, hd), g), normal((1, hd), g), normal((6, KVH, hd), g), normal((3, H, hd), g)
+    pos, slots, tables, starts, lengths = i32([0, 1, 2]), torch.tensor([0, 1, 2], device=DEV), i32([[0, 1]]), i32([0, 3]), i32([20])
+    calls = {
+        "append": lambda: c.append(x, H, pos, slots, rotary=paged.Rotary(table), norm=paged.HeadNorm("rms", qw, kw, 1e-5)),
+        "page_means": lambda: c.page_means(slots, means),
+        "attend": lambda: c.attend(q, tables, starts, lengths, 3),
+        "attend_sparse": lambda: c.attend_sparse(q, means, tables, starts, lengths, 3, top=1)[0],
+    }
+    uses = {"append": (x, k, v, table, qw, kw), "page_means": (k, means), "attend": (q, k, v), "attend_sparse": (q, k, v, means)}
+    for name, call in calls.items():
+        for t in uses[name]:
+            t.requires_grad_(True)
+            before = k.detach().clone()
+            with pytest.raises(BackendError, match="no gradients") as e:
+                call()
+            assert e.value.code == _lib.TCU_EUNSUP and torch.equal(k.detach(), before)
+            with torch.no_grad():
+                out = call()
+            t.requires_grad_(False)
+            assert torch.equal(out, call())

@@ -17,7 +17,9 @@ current stream of the cache's device) and returns. Nothing synchronises, so
 the calls can be captured into CUDA graphs; results and workspaces come from
 torch's allocator, on that stream, unless `out` is given. A tensor that was
 made on another stream has to be ordered with `stream` by the caller, as for
-any torch call. The operators serve; they record no gradients.
+any torch call. The operators serve and record no gradients: where autograd is
+on, floating-point inputs that require gradients are refused (use
+torch.no_grad, or detach them).
 Bad arguments raise BackendError with the library's TCU_EINVAL or TCU_EUNSUP.
 """
 import ctypes as C
@@ -75,6 +77,13 @@ def _on_gpu(name, t):
     if t.device.type != "cuda":
         raise _bad(f"{name} must be on a GPU, got {t.device}")
     return t.device
+
+
+def _no_grad(*tensors):
+    """Refuses tensors whose gradients a call would lose without a word."""
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise BackendError(_lib.TCU_EUNSUP, "the paged operators record no gradients: call them under torch.no_grad(), or with detached tensors")
 
 
 class Rotary:
@@ -188,6 +197,7 @@ class Cache:
         [rows, heads, head size]; rows that are skipped (slot -1) keep what
         `out` held."""
         d, index, hd = self.device, self.index, self.head_dim
+        _no_grad(qkv, self.k, self.v)
         width = (heads + 2 * self.kv_heads) * hd
         if qkv.dim() != 2 or qkv.device != d or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise _bad(f"qkv must be rows of ({heads} + 2 * {self.kv_heads}) * {hd} values on {d}, got {tuple(qkv.shape)} on {qkv.device}")
@@ -206,12 +216,14 @@ class Cache:
         if rotary is not None:
             if rotary.table.device != d:
                 raise _bad("the rotary table is on another device")
+            _no_grad(rotary.table)
             rot = rotary.ref
         if norm is not None:
             if norm.device != d or norm.head_dim != hd:
                 raise _bad(f"norm weights of head size {norm.head_dim} on {norm.device}, the cache has {hd} on {d}")
             if not norm.shared and norm.heads != (heads, self.kv_heads):
                 raise _bad("norm weights per head must be [heads, head size] and [KV heads, head size]")
+            _no_grad(norm.q_weight, norm.k_weight)
             nrm = norm.ref
         check(self._lib.tcu_paged_append(index, _stream(stream, index), self._ref, _code("qkv", qkv), rows, heads, qkv.data_ptr(),
                                          qkv.stride(0) if rows > 1 else width, p, s, rot, nrm, out.data_ptr(), stride))
@@ -221,6 +233,7 @@ class Cache:
         """Mean keys of the pages that the step's slots complete
         (tcu_paged_means), into means [pages, KV heads, head size] of the
         cache's type. Returns means."""
+        _no_grad(self.k, means)
         self._check_means(means)
         s = _whole("slots", slots, torch.int64, self.device)
         check(self._lib.tcu_paged_means(self.index, _stream(stream, self.index), self._ref, len(slots), s, means.data_ptr()))
@@ -254,6 +267,7 @@ class Cache:
         heads, first + last + top], the logical pages read, ascending, -1
         behind them."""
         d, index = self.device, self.index
+        _no_grad(means)
         self._check_means(means)
         out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out, stream)
         if min(first, top) < 0 or last < 1:
@@ -284,6 +298,7 @@ class Cache:
 
     def _queries(self, q, tables, starts, lengths, max_fresh, scale, out, stream):
         d, hd = self.device, self.head_dim
+        _no_grad(q, self.k, self.v)
         if q.dim() != 3 or q.shape[2] != hd or q.device != d or q.stride(2) != 1:
             raise _bad(f"q must be [rows, heads, {hd}] on {d}, its last dimension contiguous, got {tuple(q.shape)} on {q.device}")
         rows, heads, _ = q.shape
