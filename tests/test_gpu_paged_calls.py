@@ -108,3 +108,40 @@ def test_inputs_that_want_gradients():
                 out = call()
             t.requires_grad_(False)
             assert torch.equal(out, call())
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [40, 150])
+def test_overlapping_launches_on_two_streams(t, n):
+    """The shared prefix's kernel with the requests' own positions beside it, on
+    two streams at once, eagerly and as captured graphs: the same bits as alone."""
+    H, KVH, hd, P, prefix = 4, 2, 128, 32, 40
+    lens = [prefix * P + 1 + (i * 37) % 400 for i in range(n)]
+    s = attention_state(lens, [1] * n, H, KVH, hd, P, TYPES[t], TYPES[t], seed=n, prefix=prefix)
+    c = paged.Cache(s["k"], s["v"])
+    qs = [s["q"], s["q"].flip(0).contiguous()]
+    call = [lambda out=None, stream=None, q=q: c.attend(q, s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], out=out, stream=stream) for q in qs]
+    want = [f()[:n].clone() for f in call]
+    assert all(bool(w.isfinite().all()) for w in want)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[f(stream=st) for _ in range(30)] for f, st in zip(call, streams)]
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(x[:n], w) for x in o)
+    graphs = []
+    for f in call:
+        out = torch.zeros_like(s["q"])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            for _ in range(4):  # one call's kernels behind another's
+                f(out=out)
+        graphs.append((g, out))
+    for _ in range(10):
+        for (g, out), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                out.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, out), w in zip(graphs, want):
+        assert torch.equal(out[:n], w)
