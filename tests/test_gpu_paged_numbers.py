@@ -26,6 +26,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
+import paged_rows as R  # noqa: E402
 from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, gen, i32, near, normal, unit  # noqa: E402
 
 if torch.cuda.is_available():
@@ -157,3 +158,28 @@ def test_a_shared_step_stores_what_an_unshared_one_does(kv, heads, kv_heads, hid
         for x in reversed(opened):
             x.close()
         m.close()
+
+
+@pytest.mark.parametrize("kt", ["f32", "f16"])
+@pytest.mark.parametrize("case", R.SHORT + R.LONG)
+def test_float32_rows_keep_their_bits(kt, case):
+    """Float32 rows within a bound that a lost piece of a query or a weight passes (test_paged_rows.py)."""
+    kt = TYPES[kt]
+    lens, H, KVH, hd, P, prefix = case
+    q, ks, vs = R.inputs(case, kt, seed=2)
+    width = max(-(-n // P) for n in lens)
+    pages = prefix + sum(-(-n // P) - prefix for n in lens) + 2
+    ids = torch.randperm(pages, generator=torch.Generator().manual_seed(3)).to(torch.int32)
+    k, v = (torch.full((pages, KVH, P, hd), math.nan, dtype=kt) for _ in range(2))
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    at = prefix
+    for i, n in enumerate(lens):
+        have = -(-n // P)
+        table[i, :have] = torch.cat([ids[:prefix], ids[at:at + have - prefix]])
+        at += have - prefix
+        t = torch.arange(n)
+        k[table[i][t // P].long(), :, t % P], v[table[i][t // P].long(), :, t % P] = ks[i], vs[i]
+    starts = torch.arange(len(lens) + 1, dtype=torch.int32, device=DEV)
+    out = paged.Cache(k.to(DEV), v.to(DEV)).attend(q.to(DEV), table.to(DEV), starts, i32(lens), 1, prefix=ids[:prefix].to(DEV) if prefix else None)
+    o, wv, size = R.attend(case, q, ks, vs)
+    near(out.cpu(), o, R.bound(case, kt, o, wv, size))
