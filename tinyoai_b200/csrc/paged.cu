@@ -380,12 +380,12 @@ int prepare_kernel(size_t most, int carveout = -1) {
   return TCU_OK;
 }
 
-template <typename TQ, typename TK, int NCH, int R, int SRC>
+template <int NCH, int R, int SRC>
 int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, R, &tiles);
   const size_t smem = sizeof(float) * (CC_GROUPS + (a.cluster ? R : 0)) * (NCH * 32 + 2);
-  return launch_cluster("k_attend_cc", k_attend_cc<TQ, TK, NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, CC_WARPS * 32, smem, s, a, tiles);
+  return launch_cluster("k_attend_cc", k_attend_cc<NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, CC_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int NT, int SRC>
@@ -416,10 +416,10 @@ int launch_parts(const AttendArgs& a, int rows, int parts, cudaStream_t s) {
   if (parts == 0) return TCU_OK;
   if constexpr (sizeof(TK) == 4) {
     const int nch = (a.hd + 31) / 32;
-    if (nch <= 2) return launch_cc_r<TQ, TK, 2, 4, SRC>(a, parts, s);
-    if (nch <= 3) return launch_cc_r<TQ, TK, 3, 4, SRC>(a, parts, s);
-    if (nch <= 4) return launch_cc_r<TQ, TK, 4, 4, SRC>(a, parts, s);
-    return launch_cc_r<TQ, TK, 8, 2, SRC>(a, parts, s);
+    if (nch <= 2) return launch_cc_r<2, 4, SRC>(a, parts, s);
+    if (nch <= 3) return launch_cc_r<3, 4, SRC>(a, parts, s);
+    if (nch <= 4) return launch_cc_r<4, 4, SRC>(a, parts, s);
+    return launch_cc_r<8, 2, SRC>(a, parts, s);
   } else {
     if (a.hd <= 64) return launch_mma<TQ, TK, 64, SRC>(a, rows, parts, s);
     if (a.hd <= 96) return launch_mma<TQ, TK, 96, SRC>(a, rows, parts, s);
@@ -474,10 +474,9 @@ int launch_attend(AttendArgs a, const AttendPlan& p, cudaStream_t s) {
   return launch("k_attend_join", k_attend_join<TQ, 0>, dim3((unsigned)((int64_t)a.n * a.max_fresh), (a.H + 3) / 4), 128, 0, s, a);
 }
 
-template <typename T>
 int launch_scores_cc(const AttendArgs& a, const ChooseArgs& c, unsigned queries, cudaStream_t s) {
-  TRY((prepare_kernel<k_page_scores_cc<T, T>>(sizeof(float) * TCU_PAGED_MAX_GROUP * TCU_PAGED_MAX_HEAD_DIM)));
-  return launch("k_page_scores_cc", k_page_scores_cc<T, T>, dim3(queries, a.KVH, c.tiles), 128, sizeof(float) * a.G * a.hd, s, a, c);
+  TRY((prepare_kernel<k_page_scores_cc>(sizeof(float) * TCU_PAGED_MAX_GROUP * TCU_PAGED_MAX_HEAD_DIM)));
+  return launch("k_page_scores_cc", k_page_scores_cc, dim3(queries, a.KVH, c.tiles), 128, sizeof(float) * a.G * a.hd, s, a, c);
 }
 
 template <typename TQ, typename TK, int HD>
@@ -493,7 +492,7 @@ int launch_sparse(const AttendArgs& a, const ChooseArgs& c, const AttendPlan& p,
   // No query has more than width pages: with room for all, none is scored.
   if (c.top > 0 && c.width - c.first - c.last > c.top) {
     if constexpr (sizeof(TK) == 4)
-      TRY(launch_scores_cc<TQ>(a, c, queries, s));
+      TRY(launch_scores_cc(a, c, queries, s));
     else if (a.hd <= 64)
       TRY((launch_scores<TQ, TK, 64>(a, c, queries, s)));
     else if (a.hd <= 96)

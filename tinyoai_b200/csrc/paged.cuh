@@ -1,6 +1,6 @@
 // Operators over a paged KV cache that the caller holds: the step plan, the
-// append of normalised and rotated keys, page means, and attention on CUDA
-// cores (every type, float32 caches in particular).
+// append of normalised and rotated keys, page means, page choice, and attention
+// on CUDA cores (float32 caches).
 //
 // A cache is pages of P positions: value d of position r of page p, KV head g
 // is at p * page_stride + g * head_stride + r * token_stride + d. A request's
@@ -62,10 +62,6 @@ __device__ __forceinline__ float4 load4(const bf16* p) {
   return make_float4(__uint_as_float(r.x << 16), __uint_as_float(r.x & 0xffff0000u), __uint_as_float(r.y << 16), __uint_as_float(r.y & 0xffff0000u));
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = load4(p), b = load4(p + 4);
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 __device__ __forceinline__ void unpack2(__half, uint32_t r, float& lo, float& hi) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
   lo = f.x;
@@ -74,14 +70,6 @@ __device__ __forceinline__ void unpack2(__half, uint32_t r, float& lo, float& hi
 __device__ __forceinline__ void unpack2(bf16, uint32_t r, float& lo, float& hi) {
   lo = __uint_as_float(r << 16);
   hi = __uint_as_float(r & 0xffff0000u);
-}
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
-  const uint4 r = *reinterpret_cast<const uint4*>(p);
-  unpack2(T(), r.x, x[0], x[1]);
-  unpack2(T(), r.y, x[2], x[3]);
-  unpack2(T(), r.z, x[4], x[5]);
-  unpack2(T(), r.w, x[6], x[7]);
 }
 
 // One rounding (to nearest even) to the stored type.
@@ -112,10 +100,6 @@ template <>
 __device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(x[4], x[5]), pack2<T>(x[6], x[7]));
 }
 
 // ---------------------------------------------------------------------------
@@ -314,9 +298,7 @@ constexpr int APPEND_THREADS = 256;
 template <typename T>
 struct Raw8 {
   uint4 v;
-  __device__ __forceinline__ void load(const T* p) { v = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void stream(const T* p) { v = ld_stream16(p); }  // read once, and not moved among other such loads
-  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     unpack2(T(), v.x, x[0], x[1]);
     unpack2(T(), v.y, x[2], x[3]);
@@ -327,16 +309,11 @@ struct Raw8 {
 template <>
 struct Raw8<float> {
   float4 a, b;
-  __device__ __forceinline__ void load(const float* p) {
-    a = load4(p);
-    b = load4(p + 4);
-  }
   __device__ __forceinline__ void stream(const float* p) {
     const uint4 u = ld_stream16(p), w = ld_stream16(p + 4);
     a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
     b = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
   }
-  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
   __device__ __forceinline__ void get(float (&x)[8]) const {
     x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
   }
@@ -874,7 +851,7 @@ __device__ __forceinline__ void cluster_join(const AttendArgs& a, float* rows, i
 constexpr int CC_WARPS = 4;
 constexpr int CC_GROUPS = CC_WARPS * 4;
 
-template <typename TQ, typename TK, int NCH, int R, int SRC>
+template <int NCH, int R, int SRC>
 __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int row_tiles) {
   pdl_wait();
   extern __shared__ __align__(16) float cc_smem[];
@@ -887,7 +864,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
   int request = 0, token0 = -1, most = -1;
   const int tile = SRC == SRC_PREFIX ? blockIdx.x : blockIdx.x % row_tiles;
   if (SRC != SRC_PREFIX) request = blockIdx.x / row_tiles;
-  const TQ* qp[R];
+  const float* qp[R];
 #pragma unroll
   for (int r = 0; r < R; r++) {
     const int row = tile * R + r;
@@ -906,7 +883,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     }
     limit[r] = q.token < 0 ? -1 : q.pos;
     row_out[r] = q.token < 0 ? -1 : q.token * a.H + g * a.G + hh;
-    qp[r] = q.token < 0 ? nullptr : reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + hh) * a.q_hs;
+    qp[r] = q.token < 0 ? nullptr : reinterpret_cast<const float*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + hh) * a.q_hs;
     if (q.token >= 0) {
       token0 = q.token;
       most = max(most, q.pos);
@@ -951,8 +928,8 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
       for (int j = 0; j < 4; j++) o[r][c][j] = 0.f;
     }
   }
-  const TK* kb = reinterpret_cast<const TK*>(a.kv.k) + (int64_t)g * a.kv.sh;
-  const TK* vb = reinterpret_cast<const TK*>(a.kv.v) + (int64_t)g * a.kv.sh;
+  const float* kb = reinterpret_cast<const float*>(a.kv.k) + (int64_t)g * a.kv.sh;
+  const float* vb = reinterpret_cast<const float*>(a.kv.v) + (int64_t)g * a.kv.sh;
   constexpr int U = 2;  // positions of a group per round
   for (int u = u0 + warp * 4 + grp; u - grp < u1; u += CC_GROUPS * U) {
     float4 kx[U][NCH], vx[U][NCH];
@@ -1052,7 +1029,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
     const int64_t slot = (int64_t)row_out[r] * a.slots + (SRC == SRC_OWN ? a.prefix_slots : 0) + part;
     const bool direct = a.slots == 1;  // the only part: the output itself
     const float inv = inverse_sum(ls);
-    TQ* out = reinterpret_cast<TQ*>(a.out) + (int64_t)(row_out[r] / a.H) * a.o_ts + (int64_t)(row_out[r] % a.H) * a.o_hs;
+    float* out = reinterpret_cast<float*>(a.out) + (int64_t)(row_out[r] / a.H) * a.o_ts + (int64_t)(row_out[r] % a.H) * a.o_hs;
     float* mine = cc_smem + CC_GROUPS * (width + 2) + r * (width + 2);  // this part of the row, for its cluster
     for (int d = threadIdx.x; d < hd; d += CC_WARPS * 32) {
       float s = 0.f;
@@ -1061,7 +1038,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
       if (a.cluster)
         mine[2 + d] = s;
       else if (direct)
-        store_as(out + d, s * inv);
+        out[d] = s * inv;
       else
         a.part_o[slot * hd + d] = s;
     }
@@ -1074,7 +1051,7 @@ __global__ void __launch_bounds__(CC_WARPS * 32) k_attend_cc(AttendArgs a, int r
   }
   if (a.cluster) {
     float* rows = cc_smem + CC_GROUPS * (width + 2);
-    cluster_join<TQ>(a, rows, width + 2, R, [&](int r) {
+    cluster_join<float>(a, rows, width + 2, R, [&](int r) {
       int x = -1;
 #pragma unroll
       for (int i = 0; i < R; i++)
@@ -1185,7 +1162,6 @@ __device__ __forceinline__ Candidates candidates_of(const AttendArgs& a, const C
 
 // Float32 scores on CUDA cores (float32 caches), eight lanes a page.
 // grid: x = request * max_fresh + query, y = KV head, z = page tile.
-template <typename TQ, typename TK>
 __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs c) {
   extern __shared__ __align__(16) float cq[];  // [G][hd]
   __shared__ float s_eps[4];
@@ -1198,7 +1174,7 @@ __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs
   if (lo >= hi || cand.hi - cand.lo <= c.top) return;  // nothing to choose here
   for (int e = threadIdx.x * 4; e < a.G * hd; e += 128 * 4) {
     const int h = e / hd, d = e - h * hd;
-    *reinterpret_cast<float4*>(cq + e) = load4(reinterpret_cast<const TQ*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs + d);
+    *reinterpret_cast<float4*>(cq + e) = load4(reinterpret_cast<const float*>(a.q) + (int64_t)q.token * a.q_ts + (int64_t)(g * a.G + h) * a.q_hs + d);
   }
   __syncthreads();
   const int* table = a.tables + (int64_t)q.request * a.table_stride;
@@ -1208,7 +1184,7 @@ __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs
     const int b = b0 + (threadIdx.x >> 3);
     const int id = b >= lo && b < hi ? table[b] : -1;
     const bool on = id >= 0 && id < a.kv.num_pages;
-    const TK* mp = reinterpret_cast<const TK*>(c.means) + ((int64_t)(on ? id : 0) * a.KVH + g) * hd;
+    const float* mp = reinterpret_cast<const float*>(c.means) + ((int64_t)(on ? id : 0) * a.KVH + g) * hd;
     float best = -INFINITY;
     bool nan = false;
     for (int h = 0; h < a.G; h++) {
