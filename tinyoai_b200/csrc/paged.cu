@@ -134,22 +134,31 @@ PagedView view_of(const tcu_paged_kv* kv) {
 
 // Queues a kernel that may start while the one before it on the stream
 // drains (every kernel here waits for that one before it reads, paged.cuh), in
-// clusters of `cluster` CTAs along z.
+// clusters of `cluster` CTAs along z. carveout: the share of an SM's cache that
+// this launch wants as shared memory (percent, -1: left to the driver).
 template <typename... P, typename... A>
-int launch_cluster(const char* name, void (*kern)(P...), dim3 grid, int cluster, int block, size_t smem, cudaStream_t s, const A&... args) {
+int launch_cluster(const char* name, void (*kern)(P...), dim3 grid, int cluster, int carveout, int block, size_t smem, cudaStream_t s, const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[2];
+  cudaLaunchAttribute attr[3];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = (unsigned)cluster;
   cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cfg.numAttrs = 1;
+  if (cluster > 1) {
+    cudaLaunchAttribute& c = attr[cfg.numAttrs++];
+    c.id = cudaLaunchAttributeClusterDimension;
+    c.val.clusterDim.x = c.val.clusterDim.y = 1;
+    c.val.clusterDim.z = (unsigned)cluster;
+  }
+  if (carveout >= 0) {
+    cudaLaunchAttribute& c = attr[cfg.numAttrs++];
+    c.id = cudaLaunchAttributePreferredSharedMemoryCarveout;
+    c.val.sharedMemCarveout = (unsigned)carveout;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -160,7 +169,7 @@ int launch_cluster(const char* name, void (*kern)(P...), dim3 grid, int cluster,
 
 template <typename... P, typename... A>
 int launch(const char* name, void (*kern)(P...), dim3 grid, int block, size_t smem, cudaStream_t s, const A&... args) {
-  return launch_cluster(name, kern, grid, 1, block, smem, s, args...);
+  return launch_cluster(name, kern, grid, 1, -1, block, smem, s, args...);
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -365,17 +374,15 @@ int64_t grid_x(const AttendArgs& a, int rows, int* tiles) {
 }
 
 // Once per kernel and device: lets the kernel have up to `most` bytes of
-// dynamic shared memory, and states the share of an SM's cache it wants as
-// shared memory (percent, -1: left to the driver).
+// dynamic shared memory.
 template <auto Kern>
-int prepare_kernel(size_t most, int carveout = -1) {
+int prepare_kernel(size_t most) {
   static std::atomic<uint64_t> done{0};
   int device = 0;
   CK(cudaGetDevice(&device));
   const uint64_t bit = 1ull << (device & 63);
   if (done.load(std::memory_order_acquire) & bit) return TCU_OK;
   CK(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
-  if (carveout >= 0) CK(cudaFuncSetAttribute(Kern, cudaFuncAttributePreferredSharedMemoryCarveout, carveout));
   done.fetch_or(bit, std::memory_order_release);
   return TCU_OK;
 }
@@ -385,7 +392,7 @@ int launch_cc_r(const AttendArgs& a, int parts, cudaStream_t s) {
   int tiles;
   const int64_t x = grid_x<SRC>(a, R, &tiles);
   const size_t smem = sizeof(float) * (CC_GROUPS + (a.cluster ? R : 0)) * (NCH * 32 + 2);
-  return launch_cluster("k_attend_cc", k_attend_cc<NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, CC_WARPS * 32, smem, s, a, tiles);
+  return launch_cluster("k_attend_cc", k_attend_cc<NCH, R, SRC>, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, -1, CC_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int NT, int SRC>
@@ -394,11 +401,14 @@ int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   const int64_t x = grid_x<SRC>(a, 8 * NT, &tiles);
   const size_t smem = mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(a.cluster);
   constexpr auto kern = k_attend_mma<TQ, TK, HD, NT, SRC>;
-  // Beside the prefix's kernel: with half of the cache as shared memory, which
-  // its own four CTAs fill, 256 requests over 32,768 shared positions take 241 us,
-  // with the driver's choice 271, with all of it (no cache left for its loads) 282.
-  TRY((prepare_kernel<kern>(mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(true), SRC == SRC_OWN ? 50 : -1)));
-  return launch_cluster("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, MM_WARPS * 32, smem, s, a, tiles);
+  TRY((prepare_kernel<kern>(mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(true))));
+  // Beside the prefix's kernel: half of the cache as shared memory, which this
+  // kernel's own four CTAs fill: 256 requests over 32,768 shared positions take
+  // 241 us, with the driver's choice 271, with all of it (no cache left for its
+  // loads) 282. Alone it is left to the driver: half would keep a second CTA of
+  // the larger variants off an SM (64 requests of 2,048 positions, heads of 256
+  // in groups of 16: 219 us, 130 so).
+  return launch_cluster("k_attend_mma", kern, dim3((unsigned)x, a.KVH, parts), a.cluster ? parts : 1, a.overlap ? 50 : -1, MM_WARPS * 32, smem, s, a, tiles);
 }
 
 template <typename TQ, typename TK, int HD, int SRC>
@@ -454,10 +464,10 @@ int launch_prefix_tc(const AttendArgs& a, const AttendPlan& p, cudaStream_t s) {
   const size_t smem = pt_smem(sub, p.tc_args.split_keys, p.tc_args.stages);
   const dim3 grid(p.tc_tiles, a.KVH, p.tc_parts);
   if (sub == 2) {
-    TRY((prepare_kernel<k_attend_prefix_tc<T, 2>>(PT_MAX_SMEM, 50)));
+    TRY((prepare_kernel<k_attend_prefix_tc<T, 2>>(PT_MAX_SMEM)));
     return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 2>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
   }
-  TRY((prepare_kernel<k_attend_prefix_tc<T, 1>>(PT_MAX_SMEM, 50)));
+  TRY((prepare_kernel<k_attend_prefix_tc<T, 1>>(PT_MAX_SMEM)));
   return launch("k_attend_prefix_tc", k_attend_prefix_tc<T, 1>, grid, PT_THREADS, smem, s, a, p.tc_args, km, vm);
 }
 
