@@ -1,7 +1,7 @@
 """Calls of the operators over a paged KV cache that users make beside the
 plain ones: arrays that are inputs and outputs at once, overlapping outputs,
-inputs that want gradients, launches that overlap on two streams."""
-import ctypes as C
+inputs that want gradients, launches that overlap on two streams, bounds inside a
+prefix, pages named twice."""
 import math
 
 import pytest
@@ -9,7 +9,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_paged import DEV, TYPES, attention_state, gen, i32, normal, plan_case, plan_ref  # noqa: E402
+from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, expected, gen, i32, near, normal, plan_case, plan_ref  # noqa: E402
 from tinyoai_b200 import BackendError, _lib  # noqa: E402
 
 if torch.cuda.is_available():
@@ -145,3 +145,32 @@ def test_overlapping_launches_on_two_streams(t, n):
     torch.cuda.synchronize()
     for (_, out), w in zip(graphs, want):
         assert torch.equal(out[:n], w)
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("n, most", [(3, 700), (48, 700), (48, 1), (48, 1280), (200, 1100)])
+def test_a_max_length_within_the_prefix(qt, kt, n, most):
+    """No position from max_length on is attended, also where that ends inside the shared prefix."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    H, KVH, hd, P, prefix = 4, 2, 64, 32, 40
+    lens = [prefix * P + 1 + i % 90 for i in range(n)]
+    s = attention_state(lens, [1] * n, H, KVH, hd, P, qt, kt, seed=n, prefix=prefix)
+    out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"], max_length=most)
+    cut = [min(x, most) for x in lens]
+    want, tol = expected(s, cut, [1] * n, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
+    near(out[:n], want, tol)
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("n", [2, 48])
+def test_one_page_in_many_places(qt, kt, n):
+    """A page that a prefix and a table name again and again: its positions count each time."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    H, KVH, hd, P, prefix = 4, 2, 64, 32, 24
+    lens = [prefix * P + 70 + i % 20 for i in range(n)]
+    s = attention_state(lens, [1] * n, H, KVH, hd, P, qt, kt, seed=n, prefix=prefix)
+    s["prefix"][1::2] = s["prefix"][0]
+    s["table"][:, prefix:prefix + 2] = s["prefix"][2]
+    out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"])
+    want, tol = expected(s, lens, [1] * n, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
+    near(out[:n], want, tol)
