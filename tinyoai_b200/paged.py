@@ -79,11 +79,10 @@ def _on_gpu(name, t):
     return t.device
 
 
-def _no_grad(*tensors):
-    """Refuses tensors whose gradients a call would lose without a word."""
-    for t in tensors:
-        if t.requires_grad and torch.is_grad_enabled():
-            raise BackendError(_lib.TCU_EUNSUP, "the paged operators record no gradients: call them under torch.no_grad(), or with detached tensors")
+def _lost_gradients():
+    """Refuses a call, one of whose inputs requires gradients, where autograd is on: it would lose them without a word."""
+    if torch.is_grad_enabled():
+        raise BackendError(_lib.TCU_EUNSUP, "the paged operators record no gradients: call them under torch.no_grad(), or with detached tensors")
 
 
 class Rotary:
@@ -197,7 +196,8 @@ class Cache:
         [rows, heads, head size]; rows that are skipped (slot -1) keep what
         `out` held."""
         d, index, hd = self.device, self.index, self.head_dim
-        _no_grad(qkv, self.k, self.v)
+        if qkv.requires_grad or self.k.requires_grad or self.v.requires_grad:
+            _lost_gradients()
         width = (heads + 2 * self.kv_heads) * hd
         if qkv.dim() != 2 or qkv.device != d or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise _bad(f"qkv must be rows of ({heads} + 2 * {self.kv_heads}) * {hd} values on {d}, got {tuple(qkv.shape)} on {qkv.device}")
@@ -216,14 +216,16 @@ class Cache:
         if rotary is not None:
             if rotary.table.device != d:
                 raise _bad("the rotary table is on another device")
-            _no_grad(rotary.table)
+            if rotary.table.requires_grad:
+                _lost_gradients()
             rot = rotary.ref
         if norm is not None:
             if norm.device != d or norm.head_dim != hd:
                 raise _bad(f"norm weights of head size {norm.head_dim} on {norm.device}, the cache has {hd} on {d}")
             if not norm.shared and norm.heads != (heads, self.kv_heads):
                 raise _bad("norm weights per head must be [heads, head size] and [KV heads, head size]")
-            _no_grad(norm.q_weight, norm.k_weight)
+            if norm.q_weight.requires_grad or norm.k_weight.requires_grad:
+                _lost_gradients()
             nrm = norm.ref
         check(self._lib.tcu_paged_append(index, _stream(stream, index), self._ref, _code("qkv", qkv), rows, heads, qkv.data_ptr(),
                                          qkv.stride(0) if rows > 1 else width, p, s, rot, nrm, out.data_ptr(), stride))
@@ -233,7 +235,8 @@ class Cache:
         """Mean keys of the pages that the step's slots complete
         (tcu_paged_means), into means [pages, KV heads, head size] of the
         cache's type. Returns means."""
-        _no_grad(self.k, means)
+        if means.requires_grad or self.k.requires_grad:
+            _lost_gradients()
         self._check_means(means)
         s = _whole("slots", slots, torch.int64, self.device)
         check(self._lib.tcu_paged_means(self.index, _stream(stream, self.index), self._ref, len(slots), s, means.data_ptr()))
@@ -267,7 +270,8 @@ class Cache:
         heads, first + last + top], the logical pages read, ascending, -1
         behind them."""
         d, index = self.device, self.index
-        _no_grad(means)
+        if means.requires_grad:
+            _lost_gradients()
         self._check_means(means)
         out, ref = self._queries(q, tables, starts, lengths, max_fresh, scale, out, stream)
         if min(first, top) < 0 or last < 1:
@@ -298,7 +302,8 @@ class Cache:
 
     def _queries(self, q, tables, starts, lengths, max_fresh, scale, out, stream):
         d, hd = self.device, self.head_dim
-        _no_grad(q, self.k, self.v)
+        if q.requires_grad or self.k.requires_grad or self.v.requires_grad:
+            _lost_gradients()
         if q.dim() != 3 or q.shape[2] != hd or q.device != d or q.stride(2) != 1:
             raise _bad(f"q must be [rows, heads, {hd}] on {d}, its last dimension contiguous, got {tuple(q.shape)} on {q.device}")
         rows, heads, _ = q.shape
