@@ -546,8 +546,12 @@ typedef struct {
  * lengths (0: what the tables and the prefix map); positions from it on are
  * not attended. workspace: at least the bytes that the _workspace call
  * reports for the same arguments (it reads no device memory; 0: the call
- * needs none and workspace may be NULL), 256-byte aligned, its content irrelevant before and after; calls that may run at
- * the same time (two streams, two captured graphs) need one each. */
+ * needs none and workspace may be NULL), 256-byte aligned, its content
+ * irrelevant before and after; calls that may run at the same time (two
+ * streams, two captured graphs) need one each. A wait inside the kernel that
+ * runs out after about a second (it should not: nothing but the kernel's own
+ * copies and products is waited for) leaves NaN in the rows concerned; the call
+ * has returned by then and gives no status. */
 int tcu_paged_attend_workspace(const tcu_paged_kv* kv, const tcu_paged_queries* queries, int32_t prefix_pages, int32_t max_length,
                                uint64_t* bytes);
 int tcu_paged_attend(int32_t device, void* stream, const tcu_paged_kv* kv, const tcu_paged_queries* queries, const int32_t* prefix,

@@ -281,10 +281,11 @@ void plan_tc(const tcu_paged_kv* kv, const tcu_paged_queries* q, int prefix_page
   // Blocks per part: waves of one CTA per SM, three blocks' worth of set-up,
   // and the join's traffic of every part. A block takes 1.3 us on an SM whose
   // products never wait (half of that where the streams share the blocks) and
-  // about 2.5 as they do; the lower figure stands because SMs that a short last
-  // wave leaves idle go to the requests' own positions: 256 requests over
-  // 32,768 positions take 242 us in 4 parts (128 CTAs), 273 in the 9 (288
-  // CTAs, 2 waves) that 2.5 would choose.
+  // about 2.5 as they do, but with 2.5 second waves look cheaper than they are:
+  // 256 requests over 32,768 positions take 175 us in 4 parts (128 CTAs) and 191
+  // in the 9 (288 CTAs, 2 waves) that 2.5 would choose, 242 and 272 with up to
+  // 1,024 positions of their own each, which run on the SMs left over (times in
+  // a graph); the seven other shapes tried chose the same parts with both.
   double best = 1e30;
   const double join = 1e-6 * q->rows * q->heads * hd * 8 / 4.0 * (split ? 2 : 1);  // us a part at 4 TB/s
   for (int64_t parts = ceil_div(blocks, most); parts <= std::min<int64_t>(blocks, ceil_div(blocks, most) + 64); parts++) {
@@ -404,7 +405,7 @@ int launch_mma_n(const AttendArgs& a, int parts, cudaStream_t s) {
   TRY((prepare_kernel<kern>(mm_smem<HD, NT, sizeof(TQ) == 4 ? 2 : 1>(true))));
   // Beside the prefix's kernel: half of the cache as shared memory, which this
   // kernel's own four CTAs fill: 256 requests over 32,768 shared positions take
-  // 241 us, with the driver's choice 271, with all of it (no cache left for its
+  // 242 us in a graph, with the driver's choice 271, with all of it (no cache left for its
   // loads) 282. Alone it is left to the driver: half would keep a second CTA of
   // the larger variants off an SM (64 requests of 2,048 positions, heads of 256
   // in groups of 16: 219 us, 130 so).

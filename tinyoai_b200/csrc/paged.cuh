@@ -22,7 +22,8 @@ typedef __nv_bfloat16 bf16;
 
 // Division of t < 2^31 by a run-time constant d: floor(t / d) =
 // (t * m) >> 32 >> s with m = ceil(2^(32 + s) / d), s = ceil(log2 d), where m
-// needs 33 bits; the missing top bit is the "+ t" (the usual round-up method).
+// needs 33 bits; the missing top bit is the "+ t" (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994).
 struct FastDiv {
   uint32_t d, m, s;
   __host__ static FastDiv of(uint32_t d) {
@@ -271,7 +272,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) k_plan_step(PlanArgs a) {
 // sines and shared norm weights in registers. Instructions count here beside
 // bytes (4,096 bfloat16 rows of 32 + 8 + 8 heads of 128, 103 MB: 33 us with a
 // rotary pair's other value fetched from another lane and addresses taken
-// anew for every token, 22.6 so, 15.7 at the copy rate): where pairs come in
+// anew for every token, 22.8 so, 15.7 at the copy rate): where pairs come in
 // fours a lane holds both values of four pairs, two runs of four features.
 enum { NORM_NONE = 0, NORM_RMS = 1, NORM_LAYER = 2 };
 
