@@ -499,8 +499,9 @@ typedef struct {
  * apart, same type) and keys and values to the cache at slots[row] =
  * page * page_tokens + offset. Rows whose slot is outside the pool (-1: a
  * padding row) or whose position is outside the rotary table are skipped:
- * nothing of theirs is written. Two rows must not name one slot. q_out must
- * not overlap qkv. */
+ * nothing of theirs is written. Two rows must not name one slot. q_out may be
+ * the queries' own place in qkv (the same address and stride) and must not
+ * overlap it otherwise. */
 int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32_t dtype, int32_t rows, int32_t heads, const void* qkv,
                      int64_t qkv_stride, const int32_t* positions, const int64_t* slots, const tcu_rotary* rotary, const tcu_head_norm* norm,
                      void* q_out, int64_t q_stride);
@@ -522,7 +523,8 @@ int tcu_paged_means(int32_t device, void* stream, const tcu_paged_kv* kv, int32_
  * starts[requests] are left as they were. A row at a negative position
  * attends to nothing and is zero. What lies at positions that a row does not
  * attend to never reaches it, infinities and NaN among them. heads is a
- * multiple of kv_heads; query head h reads KV head h / (heads / kv_heads). The
+ * multiple of kv_heads; query head h reads KV head h / (heads / kv_heads). out
+ * may be q itself (address and strides) and must not overlap it otherwise. The
  * weight of position t is softmax(scale * q . k_t). */
 typedef struct {
   int32_t dtype;

@@ -174,3 +174,60 @@ def test_one_page_in_many_places(qt, kt, n):
     out = paged.Cache(s["k"], s["v"]).attend(s["q"], s["table"], s["starts"], s["lengths"], 1, prefix=s["prefix"])
     want, tol = expected(s, lens, [1] * n, H, KVH, hd, P, 1 / math.sqrt(hd), prefix)
     near(out[:n], want, tol)
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("pairs, norm", [(0, "none"), (6, "rms"), (16, "layer"), (32, "rms")])
+def test_append_in_place(qt, kt, pairs, norm):
+    """Queries written where they were read from, beside queries in a tensor of their own."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    H, KVH, hd, P, T = 8, 2, 64, 16, 900
+    g = gen(pairs)
+    x = normal((T, (H + 2 * KVH) * hd), g, qt)
+    table = torch.rand((1000, max(pairs, 1), 2), generator=g, device=DEV)
+    rot = paged.Rotary(table) if pairs else None
+    nrm = None if norm == "none" else paged.HeadNorm(norm, normal((1, hd), g), normal((1, hd), g), 1e-5)
+    pos, slots = torch.arange(T, dtype=torch.int32, device=DEV), torch.randperm(T, generator=g, device=DEV)
+    ks = [torch.zeros((2, T // P + 1, KVH, P, hd), dtype=kt, device=DEV) for _ in range(2)]
+    want = paged.Cache(*ks[0]).append(x, H, pos, slots, rotary=rot, norm=nrm)
+    y = x.clone()
+    got = paged.Cache(*ks[1]).append(y, H, pos, slots, rotary=rot, norm=nrm, out=y[:, :H * hd].view(T, H, hd))
+    assert got.data_ptr() == y.data_ptr() and torch.equal(got, want) and torch.equal(ks[0], ks[1])
+    assert torch.equal(y[:, H * hd:], x[:, H * hd:])
+
+
+def test_outputs_that_overlap_their_inputs():
+    """Views of one buffer: apart they are taken, on top of each other refused."""
+    H, KVH, hd, T = 4, 2, 64, 6
+    g = gen(1)
+    k, v = (normal((3, KVH, 8, hd), g) for _ in range(2))
+    c = paged.Cache(k, v)
+    args = (i32([[0, 1, 2]]), i32([0, T]), i32([20]), T)
+    means = normal((3, KVH, hd), g)
+
+    def attend(q, out):
+        want = c.attend(q.clone(), *args)
+        assert torch.equal(c.attend(q, *args, out=out), want)
+        c.attend_sparse(q, means, *args, top=1, out=out)
+
+    buf = normal((T, 2, H, hd), g)
+    attend(buf[:, 0], buf[:, 1])                                  # queries and outputs side by side
+    buf = normal((2, H, T, hd), g)
+    attend(buf[0].transpose(0, 1), buf[1].transpose(0, 1))        # one behind the other
+    buf = normal((T, H, 2, hd), g)
+    attend(buf[:, :, 1], buf[:, :, 0])                            # head beside head
+    long = normal((T + 2, H, hd), g)
+    wide = normal((T, H + 1, hd), g)
+    shifted = normal((T * H * hd + 256,), g)
+    for q, out in ((long[:T], long[1:T + 1]), (long[2:], long[:T]), (wide[:, :H], wide[:, 1:]), (wide[:, 1:], wide[:, :H]),
+                   (shifted[:T * H * hd].view(T, H, hd), shifted[32:32 + T * H * hd].view(T, H, hd))):
+        for call in (lambda: c.attend(q, *args, out=out), lambda: c.attend_sparse(q, means, *args, top=1, out=out)):
+            with pytest.raises(BackendError, match="out overlaps q"):
+                call()
+    width = (H + 2 * KVH) * hd
+    rows = normal((T, width + H * hd), g)
+    pos, slots = torch.arange(T, dtype=torch.int32, device=DEV), torch.arange(T, device=DEV)
+    c.append(rows[:, :width], H, pos, slots, out=rows[:, width:].view(T, H, hd))
+    for at in (64, width - 64, KVH * hd):
+        with pytest.raises(BackendError, match="q_out overlaps qkv"):
+            c.append(rows[:, :width], H, pos, slots, out=rows[:, at:at + H * hd].view(T, H, hd))

@@ -89,6 +89,39 @@ bool rows_overlap(int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t hd) {
   return false;
 }
 
+// Rows read and rows written of one call: `dims` of them in each dimension,
+// `from` and `to` apart, of r and w bytes. False where they are known to share
+// bytes without being the same rows (each is then read before it is written):
+// decided for steps that agree, which views of one buffer have.
+struct Rows {
+  const void* at;
+  int64_t step[2];  // bytes
+  int64_t bytes;
+};
+bool same_or_apart(const Rows& in, const Rows& out, const int64_t (&dims)[2]) {
+  int64_t end_in = in.bytes, end_out = out.bytes;
+  bool equal = true;
+  for (int i = 0; i < 2; i++) {
+    end_in += (dims[i] - 1) * in.step[i];
+    end_out += (dims[i] - 1) * out.step[i];
+    equal = equal && (dims[i] == 1 || in.step[i] == out.step[i]);
+  }
+  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(out.at) - reinterpret_cast<uintptr_t>(in.at));
+  if (d == 0 || d >= end_in || -d >= end_out || !equal) return true;
+  // Row (i, j) of the output begins d + di s0 + dj s1 behind one of the input.
+  const int64_t s0 = dims[0] > 1 ? out.step[0] : 0, s1 = dims[1] > 1 ? out.step[1] : 0;
+  for (int64_t dj = -(dims[1] - 1); dj < dims[1]; dj++) {
+    const int64_t rest = d + dj * s1;
+    const int64_t near = s0 > 0 ? -rest / s0 : 0;
+    for (int64_t di = near - 1; di <= near + 1; di++) {
+      if (di <= -dims[0] || di >= dims[0]) continue;
+      const int64_t gap = rest + di * s0;
+      if (gap < in.bytes && -gap < out.bytes) return false;
+    }
+  }
+  return true;
+}
+
 int elem_bytes(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
 bool dtype_ok(int dtype) { return dtype == TCU_F32 || dtype == TCU_F16 || dtype == TCU_BF16; }
 
@@ -552,6 +585,10 @@ int check_query_ptrs(const tcu_paged_kv* kv, const tcu_paged_queries* q, int dev
   TRY(check_ptr("starts", q->starts, device, 4));
   TRY(check_ptr("lengths", q->lengths, device, 4));
   if (q->table_width > 0) TRY(check_ptr("tables", q->tables, device, 4));
+  const int64_t es = elem_bytes(q->dtype), dims[2] = {q->rows, q->heads};
+  if (!same_or_apart(Rows{q->q, {q->q_token_stride * es, q->q_head_stride * es}, kv->head_dim * es},
+                     Rows{q->out, {q->out_token_stride * es, q->out_head_stride * es}, kv->head_dim * es}, dims))
+    return fail(TCU_EINVAL, "out overlaps q");
   return TCU_OK;
 }
 
@@ -749,6 +786,9 @@ int tcu_paged_append(int32_t device, void* stream, const tcu_paged_kv* kv, int32
   TRY(check_ptr("v", kv->v, device, 16));
   TRY(check_ptr("qkv", qkv, device, 16));
   TRY(check_ptr("q_out", q_out, device, 16));
+  const int64_t es = elem_bytes(dtype), one_row[2] = {rows, 1};
+  if (!same_or_apart(Rows{qkv, {qkv_stride * es, 0}, width * es}, Rows{q_out, {q_stride * es, 0}, (int64_t)heads * hd * es}, one_row))
+    return fail(TCU_EINVAL, "q_out overlaps qkv");
   TRY(check_ptr("positions", positions, device, 4));
   TRY(check_ptr("slots", slots, device, 8));
   if (a.pairs) TRY(check_ptr("rotary table", a.table, device, 8));
