@@ -419,7 +419,8 @@ int tcu_shortlist_static(int32_t device, const float* logits, int32_t vocab, int
  *    16-bit caches: with 16-bit rows each is rounded to the cache's type (by
  *    half a step of it; binary16 weights below 2^-25 of a part's largest by 2^-36
  *    of that at most), with float32 rows to a pair of binary16 values (22
- *    bits; below 2^-17 of the largest by 2^-39 of that).
+ *    bits; below 2^-17 of the largest by 2^-39 of that), and so are those rows'
+ *    queries (below 2^-16 of a row's largest by 2^-38 of that).
  *  - Strides count values, and the last dimension (a head's values) is
  *    contiguous. Rows, strides and bases of q, out, k and v are multiples of
  *    16 bytes. Head sizes: multiples of 8 up to TCU_PAGED_MAX_HEAD_DIM.

@@ -27,7 +27,7 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import paged_rows as R  # noqa: E402
-from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, gen, i32, near, normal, unit  # noqa: E402
+from test_gpu_paged import DEV, PAIRS, TYPES, attention_state, choose_ref, gen, i32, near, normal, unit  # noqa: E402
 
 if torch.cuda.is_available():
     from tinyoai_b200 import paged
@@ -183,3 +183,29 @@ def test_float32_rows_keep_their_bits(kt, case):
     out = paged.Cache(k.to(DEV), v.to(DEV)).attend(q.to(DEV), table.to(DEV), starts, i32(lens), 1, prefix=ids[:prefix].to(DEV) if prefix else None)
     o, wv, size = R.attend(case, q, ks, vs)
     near(out.cpu(), o, R.bound(case, kt, o, wv, size))
+
+
+@pytest.mark.parametrize("qt, kt", PAIRS)
+@pytest.mark.parametrize("kind", ["small beside large", "subnormal", "tiny"])
+@pytest.mark.parametrize("hd", [64, 136])
+def test_page_choice_where_float32_scores_fail(qt, kt, kind, hd):
+    """The order of pages is float64's: values of a query far below its largest
+    one, which meets means of zero, and products that float32 does not hold."""
+    qt, kt = TYPES[qt], TYPES[kt]
+    H, KVH, P, n = 8, 2, 4, 1200
+    small, of_means = {"small beside large": (1e-12, 1.0), "subnormal": (3e-23, 1e-22), "tiny": (1e-24, 1e-24)}[kind]
+    if kt == torch.float16 and kind != "small beside large":  # the least values of the types
+        small, of_means = (1e-37 if kind == "subnormal" else 1e-43) if qt == torch.float32 else 6e-8, 1e-7
+    s = attention_state([n], [1], H, KVH, hd, P, qt, kt, seed=hd, fill=0.0)
+    g = gen(7)
+    means = (normal((len(s["k"]), KVH, hd), g) * of_means).to(kt)
+    q = normal((1, H, hd), g) * small
+    if kind == "small beside large":
+        if qt == torch.float16:
+            q = q * (1e-7 / small)  # of the type's least values
+        q[..., 0] = 1.0
+        means[..., 0] = 0.0
+    q = q.to(qt)
+    _, pages = paged.Cache(s["k"], s["v"]).attend_sparse(q, means, s["table"], s["starts"], s["lengths"], 1, top=100, first=1, last=1)
+    want = choose_ref(q.reshape(KVH, H // KVH, hd), means, s["table"][0], n - 1, P, 1, 1, 100, len(s["k"]))
+    assert pages[0].tolist() == want

@@ -1145,9 +1145,16 @@ struct ChooseArgs {
   int* pages;                // [T][KVH][budget]
 };
 
-// c above: (2 hd + 32) steps of 2^-23 cover hd products and additions (the
-// tensor core's may truncate) and the 22-bit split of float32 queries.
-__host__ __device__ inline float score_slack(int hd) { return (float)(2 * hd + 32) * 1.1920929e-7f; }
+// The bound on a score's error from most, the largest sum |q_d| |mean_d|: c
+// above, (2 hd + 32) steps of 2^-23, covers hd products and additions (the
+// tensor core's may truncate) and the 22-bit split of float32 queries. Two errors
+// are no part of the sum: products that end among float32's subnormal numbers
+// or below (2^-126 each), and what the split leaves out of values far below a
+// query's largest, 2^-25 of the step `scale` its pieces are counted in, times a
+// binary16 mean (0: not split).
+__device__ __forceinline__ float score_error(float most, int hd, float scale) {
+  return fmaf(most, (float)(2 * hd + 32) * 1.1920929e-7f, (float)hd * fmaf(scale, 0x1p-9f, 0x1p-125f));
+}
 
 // Candidate pages [lo, hi) of a query.
 struct Candidates {
@@ -1214,7 +1221,7 @@ __global__ void __launch_bounds__(128) k_page_scores_cc(AttendArgs a, ChooseArgs
   if (threadIdx.x == 0) {
     uint32_t x = 0;
     for (int i = 0; i < 4; i++) x = max(x, __float_as_uint(s_eps[i]));
-    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = __uint_as_float(x) * score_slack(hd);
+    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = score_error(__uint_as_float(x), hd, 0.f);
   }
 }
 

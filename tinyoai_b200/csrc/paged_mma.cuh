@@ -564,7 +564,10 @@ __global__ void __launch_bounds__(MM_WARPS * 32, HD <= 128 ? 4 : 2) k_page_score
   if (tid == 0) {
     uint32_t x = 0;
     for (int i = 0; i < MM_WARPS; i++) x = max(x, s_eps[i]);
-    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = __uint_as_float(x) * score_slack(hd);
+    float scale = 0.f;  // of the coarsest split
+    if (PIECES == 2)
+      for (int i = 0; i < a.G; i++) scale = fmaxf(scale, s_scale[i]);
+    c.eps[((int64_t)q.token * a.KVH + g) * c.tiles + blockIdx.z] = score_error(__uint_as_float(x), hd, scale);
   }
 }
 
